@@ -10,7 +10,8 @@ for f in *.hip; do
   stale=0
   for h in *.h ../../include/gpx.h; do [ "$h" -nt "$o" ] && stale=1; done   # every header: tile_order.h, gemm_flags.h ... too
   if [ ! -f "$o" ] || [ "$f" -nt "$o" ] || [ $stale = 1 ]; then
-    hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -c "$f" -o "$o" &
+    # no packed fp32 instructions: some of their forms have given wrong results on this hardware
+    hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops -c "$f" -o "$o" &
     pids+=($!)
   fi
 done

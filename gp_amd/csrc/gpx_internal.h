@@ -28,6 +28,28 @@ typedef double v2d __attribute__((ext_vector_type(2)));
         }                                                                                   \
     } while (0)
 
+// Entry points that launch on a caller's stream run on that stream's device, whichever is current, and restore the
+// caller's current device.  (The null stream belongs to the current device.)
+struct StreamDevice {
+    int status = GPX_OK, back = -1;
+    explicit StreamDevice(hipStream_t st) {
+        if (!st) return;
+        hipDevice_t dev = 0;
+        int cur = 0;
+        if (hipStreamGetDevice(st, &dev) != hipSuccess || hipGetDevice(&cur) != hipSuccess) {
+            status = GPX_ERR_HIP;
+        } else if (cur != dev) {
+            if (hipSetDevice(dev) == hipSuccess) back = cur;
+            else status = GPX_ERR_HIP;
+        }
+    }
+    ~StreamDevice() {
+        if (back >= 0) (void)hipSetDevice(back);
+    }
+    StreamDevice(const StreamDevice&) = delete;
+    StreamDevice& operator=(const StreamDevice&) = delete;
+};
+
 // leading dimension for internal column-major matrices: multiple of 16 doubles (128 B), never a
 // multiple of 256 doubles so that column strides do not alias on HBM channels
 static inline long gpx_ld(long n) {

@@ -1,0 +1,224 @@
+// mm_tile.h — one workgroup's output tile D = P Q^T on the matrix cores, for double, float, bf16 and f16 operands.
+//
+// D(i, j) = sum_k P(i, k) Q(j, k), i < BM, j < BN.  Either operand is stored with k contiguous (KC: element (i, k) at
+// base + i*ld + k) or with its own index contiguous (base + k*ld + i).  Products of 16-bit elements and of floats are summed
+// in 32 bits, those of doubles in 64: the accumulator of the matrix instruction, never narrower.
+//
+// LDS image of one K step: 128 bytes of k per row (BK = 16 doubles, 32 floats, 64 16-bit elements), always written in 16-byte
+// chunks, chunk number = thread number, so that the image is the same whether a chunk arrives through registers or straight
+// from memory.  KC operands: [row][8 chunks], chunk c of row r sits at c ^ (r & 7): the 16 rows that one fragment read
+// touches would otherwise share one 128-byte bank window.  The others: [k][ROWS], blocks of 16 columns permuted by a function
+// of k (strided_swizzle) for the same reason.  Fragments: lane l holds row l & 15 and the k group l >> 4 of its 16x16 tile;
+// both operands use one assignment of k to lanes, so any assignment is right and the one that reads 16 contiguous bytes is taken.
+// 16-bit operands with k strided are turned by the transposing LDS read (ds_read_b64_tr_b16: in each 16 lanes, lane n
+// addresses 8 bytes of row n / 4 and receives column n of the 4 x 16 block).
+#pragma once
+#include "gpx_internal.h"
+
+namespace mm {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+template <class T> struct Acc { typedef v4f vec; typedef float one; };
+template <> struct Acc<double> { typedef v4d vec; typedef double one; };
+
+template <class T> constexpr int chunk_elems() { return 16 / (int)sizeof(T); }
+template <class T> constexpr int step_k() { return 128 / (int)sizeof(T); }
+
+// ---- fragments: 16 rows x (64 bytes of k), one v4i per lane --------------------------------------------------------
+template <class T> __device__ __forceinline__ int strided_swizzle(int k) {
+    if (sizeof(T) == 8) return (k >> 1) & 1;   // the k groups 2q of one read: halves of the 256-byte bank window
+    if (sizeof(T) == 4) return (k >> 2) & 3;   // the k groups 4q: quarters
+    return (k & 3) | ((k >> 3) & 1) << 2;      // 32-byte blocks: rows k..k+3 of the k groups 8q
+}
+
+template <class T, int ROWS, bool KC>
+__device__ __forceinline__ v4i frag(const char* s, int row0, int kk, int lane) {
+    const int r = lane & 15, q = lane >> 4;
+    if constexpr (KC) {
+        const int row = row0 + r;
+        return *reinterpret_cast<const v4i*>(s + row * 128 + (((kk * 4 + q) ^ (row & 7)) << 4));
+    } else if constexpr (sizeof(T) == 2) {
+        constexpr int mask = ROWS / 16 < 8 ? ROWS / 16 - 1 : 7;
+        const int k = kk * 32 + 8 * q + (r >> 2);
+        const int b = (row0 >> 4) ^ (strided_swizzle<T>(k) & mask);
+        const char* p = s + k * (ROWS * 2) + b * 32 + (r & 3) * 8;
+        typedef __attribute__((address_space(3))) v4s lds4;
+        union { v4s h[2]; v4i v; } u;
+        u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p));
+        u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * ROWS * 2));
+        return u.v;
+    } else {
+        constexpr int E = chunk_elems<T>(), mask = ROWS / 16 < 4 ? ROWS / 16 - 1 : 3;
+        const int k = kk * 4 * E + E * q;
+        const int b = (row0 >> 4) ^ (strided_swizzle<T>(k) & mask);
+        const T* p = reinterpret_cast<const T*>(s) + k * ROWS + b * 16 + r;
+        union { T e[E]; v4i v; } u;
+#pragma unroll
+        for (int x = 0; x < E; ++x) u.e[x] = p[x * ROWS];
+        return u.v;
+    }
+}
+
+// D += A B^T over the 64 bytes of k of the fragments.  The lane holds D rows (index of `a`) 4q + r (doubles: q + 4r),
+// r = 0..3, and the column (index of `b`) lane & 15.
+template <class T> __device__ __forceinline__ typename Acc<T>::vec mma(v4i a, v4i b, typename Acc<T>::vec c) {
+    if constexpr (sizeof(T) == 8) {
+        union { v4i v; double e[2]; } x{a}, y{b};
+        c = __builtin_amdgcn_mfma_f64_16x16x4f64(x.e[0], y.e[0], c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f64_16x16x4f64(x.e[1], y.e[1], c, 0, 0, 0);
+    } else if constexpr (sizeof(T) == 4) {
+        union { v4i v; float e[4]; } x{a}, y{b};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x.e[s], y.e[s], c, 0, 0, 0);
+        return c;
+    } else if constexpr (__is_same(T, __bf16)) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    }
+}
+
+// ---- one operand's tile of one K step, through registers: any alignment, any extent ---------------------------------
+// `valid` elements of the 16 bytes at p may be read, the others are zero
+template <class T> __device__ __forceinline__ v4i load_chunk(const char* p, int valid) {
+    constexpr int E = chunk_elems<T>();
+    v4i v = {0, 0, 0, 0};
+    if (valid >= E) {
+        __builtin_memcpy(&v, p, 16);
+    } else if (valid > 0) {
+        union { v4i v; T e[E]; } u;
+        u.v = v;
+#pragma unroll
+        for (int x = 0; x < E; ++x)
+            if (x < valid) u.e[x] = reinterpret_cast<const T*>(p)[x];
+        v = u.v;
+    }
+    return v;
+}
+
+template <class T, int ROWS, bool KC, int NT> struct Operand {
+    static constexpr int E = chunk_elems<T>(), BK = step_k<T>();
+    static constexpr int NL = ROWS * 8 / NT;   // chunks per thread
+    static constexpr int BYTES = ROWS * 128;
+    static_assert(ROWS * 8 % NT == 0, "whole chunks per thread");
+    const char* base;   // element (0, 0) of the tile's rows
+    long ld;            // bytes between rows (KC) or between k (otherwise)
+    int rows, K;        // rows of the tile and extent of k that exist
+
+    __device__ __forceinline__ void place(int c, int& row, int& k) const {   // first element of chunk c
+        if (KC) {
+            row = c >> 3;
+            k = ((c & 7) ^ (row & 7)) * E;
+        } else {
+            constexpr int PER = ROWS / E;              // chunks per k
+            constexpr int HB = 16 / E;                 // chunks per block of 16 columns
+            constexpr int mask = ROWS / 16 < 8 ? ROWS / 16 - 1 : 7;
+            k = c / PER;
+            const int slot = c % PER;
+            row = ((slot / HB) ^ (strided_swizzle<T>(k) & mask)) * 16 + slot % HB * E;
+        }
+    }
+    __device__ __forceinline__ void load(v4i (&r)[NL], int k0) const {
+#pragma unroll
+        for (int it = 0; it < NL; ++it) {
+            int row, k;
+            place(it * NT + (int)threadIdx.x, row, k);
+            k += k0;
+            if (KC) r[it] = load_chunk<T>(base + row * ld + (long)k * sizeof(T), row < rows ? K - k : 0);
+            else r[it] = load_chunk<T>(base + k * ld + (long)row * sizeof(T), k < K ? rows - row : 0);
+        }
+    }
+    __device__ __forceinline__ void stash(char* s, const v4i (&r)[NL]) const {
+#pragma unroll
+        for (int it = 0; it < NL; ++it) *reinterpret_cast<v4i*>(s + (it * NT + (int)threadIdx.x) * 16) = r[it];
+    }
+};
+
+// ---- the tile ----------------------------------------------------------------------------------------------------
+// Waves in a WR (rows i) x WC (columns j) grid; each owns TI x TJ fragments of 16.  SWAP: the accumulator's contiguous
+// lanes run along j (doubles and floats: whole 64..128-byte runs per store); otherwise its four registers do (16-bit
+// results: 8-byte stores instead of single elements).
+template <class T, int BM, int BN, int WR, int WC, bool PKC, bool QKC> struct Tile {
+    static constexpr int NT = WR * WC * 64;
+    static constexpr int TI = BM / WR / 16, TJ = BN / WC / 16;
+    static constexpr bool SWAP = sizeof(T) != 2;
+    typedef Operand<T, BM, PKC, NT> OpP;
+    typedef Operand<T, BN, QKC, NT> OpQ;
+    typedef typename Acc<T>::vec vec;
+    typedef typename Acc<T>::one one;
+    static constexpr int STAGE = OpP::BYTES + OpQ::BYTES;
+    static constexpr int LDS = 2 * STAGE;
+    vec acc[TI][TJ];
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) acc[i][j] = vec{};
+    }
+    __device__ __forceinline__ void multiply(const char* s) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int i0 = wave / WC * (BM / WR), j0 = wave % WC * (BN / WC);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            v4i fp[TI], fq[TJ];
+#pragma unroll
+            for (int i = 0; i < TI; ++i) fp[i] = frag<T, BM, PKC>(s, i0 + 16 * i, kk, lane);
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) fq[j] = frag<T, BN, QKC>(s + OpP::BYTES, j0 + 16 * j, kk, lane);
+#pragma unroll
+            for (int i = 0; i < TI; ++i)
+#pragma unroll
+                for (int j = 0; j < TJ; ++j)
+                    acc[i][j] = SWAP ? mma<T>(fp[i], fq[j], acc[i][j]) : mma<T>(fq[j], fp[i], acc[i][j]);
+        }
+    }
+    // register-staged K loop: the chunks of step k + 1 are in flight while step k is multiplied, two LDS stages, one barrier
+    __device__ __forceinline__ void run_staged(char* lds, const OpP& p, const OpQ& q, int K) {
+        v4i rp[OpP::NL], rq[OpQ::NL];
+        const int steps = (K + OpP::BK - 1) / OpP::BK;
+        if (steps == 0) return;
+        p.load(rp, 0);
+        q.load(rq, 0);
+        for (int s = 0; s < steps; ++s) {
+            char* st = lds + (s & 1) * STAGE;
+            p.stash(st, rp);
+            q.stash(st + OpP::BYTES, rq);
+            if (s + 1 < steps) {
+                p.load(rp, (s + 1) * OpP::BK);
+                q.load(rq, (s + 1) * OpP::BK);
+            }
+            __syncthreads();   // also: nobody reads the other stage any more when the next step writes it
+            multiply(st);
+        }
+    }
+    // f(i, j, value pointer, count): count consecutive columns j.. of row i of the tile
+    template <class F> __device__ __forceinline__ void each(F&& f) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+        const int i0 = wave / WC * (BM / WR), j0 = wave % WC * (BN / WC);
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) {
+                if constexpr (SWAP) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        one v = acc[i][j][x];
+                        f(i0 + 16 * i + (sizeof(T) == 8 ? q + 4 * x : 4 * q + x), j0 + 16 * j + r, &v, std::integral_constant<int, 1>{});
+                    }
+                } else {
+                    one v[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) v[x] = acc[i][j][x];
+                    f(i0 + 16 * i + r, j0 + 16 * j + 4 * q, v, std::integral_constant<int, 4>{});
+                }
+            }
+    }
+};
+
+}  // namespace mm

@@ -333,3 +333,149 @@ def chol_solve(A, B=None, want_inverse=False):
                              Inv.ctypes.data if want_inverse else None), "chol_solve")
     X = Bc.reshape(nrhs, n).T.copy() if nrhs else None
     return bool(spd.value), ld.value, X, (Inv.reshape(n, n).T.copy() if want_inverse else None)
+
+
+# ---- products grouped by expert, orthogonalised update ---------------------------------------------
+# These take torch tensors on the GPU (rows of any stride, the last dimension contiguous), launch on torch's current stream
+# of the tensors' device and return `out`; nothing is recorded for autograd.  torch is imported only when one is called.
+F64, F32, BF16, F16 = 0, 1, 2, 3
+
+lib.gpx_grouped_gemm.argtypes = [_i, _i, _i64, _i64, _i64, _i64, _d, _vp, _i64, _vp, _i64, _i64, _vp, _d, _vp, _i64, _vp]
+lib.gpx_grouped_gemm_dw.argtypes = [_i, _i, _i64, _i64, _i64, _i64, _d, _vp, _i64, _vp, _i64, _vp, _d, _vp, _i64, _i64, _vp, _i64, _vp]
+lib.gpx_grouped_gemm_dw_work.argtypes = [_i, _i64, _i64, _i64, _i64, C.POINTER(_i64)]
+lib.gpx_orthogonalize.argtypes = [_i, _i64, _i64, _i64, _vp, _i64, _i64, _i, _vp, _d, _vp, _i64, _i64, _vp, _i64, _vp]
+lib.gpx_orthogonalize_work.argtypes = [_i, _i64, _i64, _i64, C.POINTER(_i64)]
+
+_dtype_codes = {}
+
+
+def _dtype(t, what):
+    if not _dtype_codes:
+        import torch
+        _dtype_codes.update({torch.float64: F64, torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+    code = _dtype_codes.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what}: float64, float32, bfloat16 or float16, not {t.dtype}")
+    return code
+
+
+def _rows(t, dims, what):
+    """(stride between matrices, stride between rows) of a tensor of `dims` dimensions with contiguous rows."""
+    if t.dim() != dims:
+        raise ValueError(f"{what}: {dims} dimensions, not {t.dim()}")
+    cols, count = t.shape[-1], t.shape[-2]
+    if cols > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: the last dimension has to be contiguous")
+    ld = t.stride(-2) if count > 1 else max(cols, 1)
+    if ld < cols:
+        raise ValueError(f"{what}: rows overlap (stride {ld} for {cols} elements)")
+    return (t.stride(0) if dims == 3 and t.shape[0] > 1 else 0), ld
+
+
+def _one_device(*tensors):
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise ValueError(f"tensors on the GPU are wanted, not on {dev}")
+    for t in tensors[1:]:
+        if t.device != dev:
+            raise ValueError(f"all tensors on one device are wanted: {dev} and {t.device}")
+    return dev.index
+
+
+def _launch(fn, what, index, *args):
+    """fn(..., stream) on torch's current stream of device `index`; the null stream belongs to the current device."""
+    import torch
+    stream = torch.cuda.current_stream(index).cuda_stream
+    if stream or index == torch.cuda.current_device():
+        check(fn(*args, stream), what)
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args, stream), what)
+
+
+def _offsets(offsets, groups):
+    if str(offsets.dtype) != "torch.int64" or offsets.dim() != 1 or not offsets.is_contiguous():
+        raise ValueError("offsets: a contiguous vector of int64 is wanted")
+    if offsets.shape[0] != groups + 1:
+        raise ValueError(f"offsets: {groups + 1} values for {groups} groups, not {offsets.shape[0]}")
+
+
+def _work(query, like, *args):
+    """Workspace from torch's allocator, ordered with torch's current stream like every other temporary of it."""
+    n = _i64(0)
+    check(query(*args, C.byref(n)), "workspace query")
+    if n.value == 0:
+        return None, 0
+    w = like.new_empty(-(-n.value // like.element_size()))
+    return w, n.value
+
+
+def grouped_gemm(x, w, offsets, out, w_kc=True, alpha=1.0, beta=0.0):
+    """out[t] = alpha * W_g x[t] + beta * out[t] for the rows offsets[g] <= t < offsets[g+1] of every group g; the others stay.
+
+    x (T, K), out (T, N); w (G, N, K) for w_kc, else (G, K, N); offsets (G + 1,) int64 on the device.  The gradient of x is
+    grouped_gemm(dy, w, offsets, dx, w_kc=not w_kc); that of w is grouped_gemm_dw."""
+    index = _one_device(x, w, offsets, out)
+    code = _dtype(x, "x")
+    if w.dtype != x.dtype or out.dtype != x.dtype:
+        raise ValueError("x, w and out have to be of one type")
+    (_, ldx), (_, ldy) = _rows(x, 2, "x"), _rows(out, 2, "out")
+    stride_w, ldw = _rows(w, 3, "w")
+    groups, n, k = w.shape if w_kc else (w.shape[0], w.shape[2], w.shape[1])
+    rows = x.shape[0]
+    if x.shape[1] != k or tuple(out.shape) != (rows, n):
+        raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, w {tuple(w.shape)}, out {tuple(out.shape)}")
+    _offsets(offsets, groups)
+    _launch(lib.gpx_grouped_gemm, "grouped_gemm", index, code, int(w_kc), groups, rows, n, k, alpha, x.data_ptr(), ldx, w.data_ptr(),
+            ldw, stride_w, offsets.data_ptr(), beta, out.data_ptr(), ldy)
+    return out
+
+
+def grouped_gemm_dw(x, dy, offsets, out, alpha=1.0, beta=0.0):
+    """out[g] = alpha * dy_g^T x_g + beta * out[g] over the rows of every group: x (T, K), dy (T, N), out (G, N, K) of their type,
+    or float32 for 16-bit rows.  For weights in the (G, K, N) layout exchange x and dy."""
+    index = _one_device(x, dy, offsets, out)
+    code, code_out = _dtype(x, "x"), _dtype(out, "out")
+    if dy.dtype != x.dtype:
+        raise ValueError("x and dy have to be of one type")
+    if code_out != code and not (code_out == F32 and code in (BF16, F16)):
+        raise ValueError(f"out: {x.dtype}, or float32 for 16-bit rows, not {out.dtype}")
+    (_, ldx), (_, ldz) = _rows(x, 2, "x"), _rows(dy, 2, "dy")
+    stride_c, ldc = _rows(out, 3, "out")
+    groups, n, k = out.shape
+    rows = x.shape[0]
+    if x.shape[1] != k or tuple(dy.shape) != (rows, n):
+        raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, dy {tuple(dy.shape)}, out {tuple(out.shape)}")
+    _offsets(offsets, groups)
+    work, size = _work(lib.gpx_grouped_gemm_dw_work, x, code, groups, rows, k, n)
+    _launch(lib.gpx_grouped_gemm_dw, "grouped_gemm_dw", index, code, code_out, groups, rows, k, n, alpha, x.data_ptr(), ldx,
+            dy.data_ptr(), ldz, offsets.data_ptr(), beta, out.data_ptr(), ldc, stride_c, work.data_ptr() if size else None, size)
+    return out
+
+
+def orthogonalize(g, out, steps=5, coef=None, eps=1e-7):
+    """The Newton-Schulz update of g (M, N) or (B, M, N) into out (of g's shape and type; g itself is allowed): g / (|g|_F + eps),
+    then `steps` times x <- a x + (b A + c A A) x with A = x x^T.  coef: (a, b, c), or one such triple for every step."""
+    index = _one_device(g, out)
+    code = _dtype(g, "g")
+    if out.dtype != g.dtype or out.shape != g.shape:
+        raise ValueError("out has to be of g's shape and type")
+    if g.dim() == 2:
+        g3, out3 = g.unsqueeze(0), out.unsqueeze(0)
+    else:
+        g3, out3 = g, out
+    (stride_g, ldg), (stride_o, ldo) = _rows(g3, 3, "g"), _rows(out3, 3, "out")
+    batch, rows, cols = g3.shape
+    table = None
+    if coef is not None:
+        table = _c(coef)
+        if table.shape == (3,):
+            table = np.tile(table, steps)
+        elif table.shape != (steps, 3):
+            raise ValueError("coef: three values, or three for every step")
+        table = np.ascontiguousarray(table)
+    work, size = _work(lib.gpx_orthogonalize_work, g, code, batch, cols, rows)
+    _launch(lib.gpx_orthogonalize, "orthogonalize", index, code, batch, cols, rows, g.data_ptr(), ldg, stride_g, steps,
+            table.ctypes.data if table is not None and steps else None, eps, out.data_ptr(), ldo, stride_o,
+            work.data_ptr() if size else None, size)
+    return out

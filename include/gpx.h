@@ -71,6 +71,47 @@ int gpx_dgemm_splitk_noalloc(int a_kc, int b_kc, int64_t M, int64_t N, int64_t K
                              int64_t lda, const double* B, int64_t ldb, double beta, double* C, int64_t ldc,
                              int flags, void* hip_stream);
 
+/* ---- products grouped by expert, and the orthogonalised update (no reference counterpart) -----------
+ * Local experts (groups of training rows, each with a feature map z = W_g x of its own): all their products in one call,
+ * the gradients of both operands, and the Newton-Schulz update of a batch of weight matrices.  All buffers are DEVICE
+ * memory of hip_stream's device (NULL: the legacy stream of the current device); every call is asynchronous, allocates
+ * nothing, waits for nothing and may be captured into a HIP graph; the caller's current device is restored.  Element
+ * types: dtype below; pointers are aligned to their element, rows of any length and leading dimension are taken.
+ * Products of F64 are summed in 64 bits, all others in 32; results are rounded once to the type they are stored in.
+ * No result depends on the order in which workgroups run.  Status 1 (GPX_ERR_ARG): an argument is refused, nothing was
+ * launched. */
+enum { GPX_F64 = 0, GPX_F32 = 1, GPX_BF16 = 2, GPX_F16 = 3 };
+
+/* Rows t (points, K contiguous elements at X + t*ldx) with offsets[g] <= t < offsets[g+1] belong to group g:
+ *   Y(:,t) = alpha * W_g * X(:,t) + beta * Y(:,t)         (N elements at Y + t*ldy)
+ * W_g at W + g*stride_w: w_kc = 1: W_g(n,k) at k + n*ldw (ldw >= K); w_kc = 0: at n + k*ldw (ldw >= N).  The gradient of
+ * the points is the same call with the layout flag turned: dX(:,t) = W_g^T dY(:,t).  stride_w = 0: one W for all groups.
+ * offsets: groups + 1 DEVICE values, non-decreasing, in [0, T]; groups may be empty.  Rows of Y that belong to no group are
+ * left as they were; with beta = 0 Y is not read.  Offsets outside [0, T] are taken as the nearer end and a decreasing
+ * pair as an empty group: a wrong table gives wrong rows, never an access outside X and Y.  groups <= 65535. */
+int gpx_grouped_gemm(int dtype, int w_kc, int64_t groups, int64_t T, int64_t N, int64_t K, double alpha, const void* X,
+                     int64_t ldx, const void* W, int64_t ldw, int64_t stride_w, const int64_t* offsets, double beta, void* Y,
+                     int64_t ldy, void* hip_stream);
+/* The gradient of the weights: C_g = alpha * sum over the group's rows t of X(:,t) Z(:,t)^T + beta * C_g, M x N column-major
+ * at C + g*stride_c (X: M elements a row, Z = dY: N elements a row).  An empty group gives beta * C_g (zeros for beta = 0).
+ * With M = K this is dW of the w_kc = 1 layout; X and Z exchanged, of the other.  X = Z: the Gram matrix of each group's
+ * rows.  c_dtype: dtype, or GPX_F32 for 16-bit rows (gradients kept in 32 bits).  work: work_bytes of DEVICE memory,
+ * 16-byte aligned, at least what gpx_grouped_gemm_dw_work says (NULL if that is 0); calls that overlap in time must not
+ * share it. */
+int gpx_grouped_gemm_dw_work(int dtype, int64_t groups, int64_t T, int64_t M, int64_t N, int64_t* work_bytes);
+int gpx_grouped_gemm_dw(int dtype, int c_dtype, int64_t groups, int64_t T, int64_t M, int64_t N, double alpha, const void* X,
+                        int64_t ldx, const void* Z, int64_t ldz, const int64_t* offsets, double beta, void* C, int64_t ldc,
+                        int64_t stride_c, void* work, int64_t work_bytes, void* hip_stream);
+/* batch matrices G_b (M x N column-major at G + b*stride_g): X = G / (|G|_F + eps), then `steps` (0..64) times
+ *   A = X X^T,  X = a X + (b A + c A A) X        (the odd polynomial a s + b s^3 + c s^5 of the singular values s)
+ * into O.  coef: HOST, 3*steps finite values a, b, c of every step; NULL: (3.4445, -4.7750, 2.0315) in each.  eps > 0: a
+ * zero matrix gives zeros.  A matrix that holds an infinity or NaN gives non-finite values in its own result only.  O may
+ * be G (same ld and stride).  work: as above, gpx_orthogonalize_work bytes. */
+int gpx_orthogonalize_work(int dtype, int64_t batch, int64_t M, int64_t N, int64_t* work_bytes);
+int gpx_orthogonalize(int dtype, int64_t batch, int64_t M, int64_t N, const void* G, int64_t ldg, int64_t stride_g, int steps,
+                      const double* coef, double eps, void* O, int64_t ldo, int64_t stride_o, void* work, int64_t work_bytes,
+                      void* hip_stream);
+
 /* ---- measurement hooks (no reference counterpart) ------------------------------------------ */
 /* HIP-event timing of every GEMM launch with >= min_flops useful flops, on the launch stream; a
  * negative min_flops selects exactly the launches of the 128x128-tile kernel (the one bench.py's MFMA

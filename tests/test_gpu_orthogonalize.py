@@ -1,0 +1,202 @@
+"""GPU tests of the orthogonalised update (gp_amd/csrc/ortho.hip) against its definition in 64 bits, and of a training step
+that uses it with the grouped products."""
+import pytest
+
+torch = pytest.importorskip("torch")
+import grouped_oracle as oracle  # noqa: E402
+from test_gpu_grouped import data, framed, table, untouched  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float64, torch.float32, torch.bfloat16, torch.float16]
+
+
+def _lib():
+    from gp_amd import lib
+    return lib
+
+
+def check(got, g, **kw):
+    for o, m in zip(got, g):
+        want, tol = oracle.orthogonalize(m, **kw)
+        off = float(torch.linalg.norm(o.double() - want)) / max(float(torch.linalg.norm(want)), 1e-300)
+        assert off <= tol, (off, tol, tuple(m.shape))
+
+
+SIZES = [(1, 1), (1, 7), (5, 1), (2, 3), (16, 16), (17, 50), (50, 20), (64, 64), (65, 63), (128, 128), (130, 127), (96, 520),
+         (520, 97), (256, 384), (300, 300), (33, 1500)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: f"{s[0]}x{s[1]}")
+@pytest.mark.parametrize("frame", [(0, 0), (3, 1)], ids=["plain", "odd"])
+def test_orthogonalize(dtype, size, frame):
+    lib = _lib()
+    g = framed(data(1, dtype, 3, *size), *frame)[1]
+    flat, out = framed(torch.zeros(3, *size, dtype=dtype, device="cuda"), *frame)
+    assert lib.orthogonalize(g, out) is out
+    assert untouched(flat, out)
+    check(out, g)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_low_rank_and_wide_spectrum(dtype):
+    """Singular values over many orders of magnitude, and matrices of rank one."""
+    lib = _lib()
+    u, v = data(1, torch.float64, 2, 80, 40), data(2, torch.float64, 2, 40, 120)
+    s = torch.logspace(0, -9, 40, device="cuda", dtype=torch.float64)
+    g = torch.stack([(u[0] * s) @ v[0], u[1][:, :1] @ v[1][:1]]).to(dtype)
+    check(lib.orthogonalize(g, torch.empty_like(g)), g)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("steps,coef", [(0, None), (1, None), (12, (1.5, -0.5, 0.0)), (2, [(3.0, -3.2, 1.2), (2.0, -1.5, 0.5)]),
+                                        (3, (1.0, 0.0, 0.0)), (2, (-2.0, 1.5, -0.5))])
+def test_steps_and_coefficients(dtype, steps, coef):
+    lib = _lib()
+    g = data(1, dtype, 2, 40, 72)
+    check(lib.orthogonalize(g, torch.empty_like(g), steps=steps, coef=coef), g, steps=steps, coef=coef)
+
+
+def test_cubic_steps_reach_the_polar_factor():
+    """(1.5, -0.5, 0) converges to U V^T: the rows of the result are orthonormal."""
+    lib = _lib()
+    g = data(1, torch.float64, 24, 60)
+    o = lib.orthogonalize(g, torch.empty_like(g), steps=30, coef=(1.5, -0.5, 0.0))
+    assert float((o @ o.T - torch.eye(24, device="cuda", dtype=torch.float64)).abs().max()) < 1e-12
+    u, _, vt = torch.linalg.svd(g.cpu(), full_matrices=False)
+    assert float((o.cpu() - u @ vt).abs().max()) < 1e-12
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_scales_zeros_and_non_finite_values(dtype):
+    lib = _lib()
+    big = {torch.float64: 1e300, torch.float32: 1e37, torch.bfloat16: 1e37, torch.float16: 1e4}[dtype]
+    # double: its square overflows as it does in any 64-bit norm
+    big = 1e150 if dtype == torch.float64 else big
+    base = data(1, torch.float64, 30, 44).clamp(-3, 3)
+    g = torch.stack([base.to(dtype), (base * big).to(dtype), torch.zeros(30, 44, dtype=dtype, device="cuda"), base.to(dtype),
+                     base.to(dtype), base.to(dtype)])
+    g[3, 7, 9] = float("nan")
+    g[5, 0, 0] = float("inf")
+    out = lib.orthogonalize(g, torch.empty_like(g))
+    check(out[:2], g[:2])
+    check(out[4:5], g[4:5])
+    assert not bool(out[2].any())
+    assert torch.isnan(out[3]).all()
+    assert not bool(torch.isfinite(out[5]).all())
+    tiny = (base * (1e-30 if dtype in (torch.float32, torch.bfloat16) else 1e-3 if dtype == torch.float16 else 1e-150)).to(dtype)
+    eps = 1e-300 if dtype == torch.float64 else 1e-36
+    check(lib.orthogonalize(tiny, torch.empty_like(tiny), eps=eps)[None], tiny[None], eps=eps)
+
+
+def test_in_place_and_two_dimensions():
+    lib = _lib()
+    for dtype in TYPES:
+        for size in ((40, 72), (72, 40), (300, 140)):
+            g = data(1, dtype, *size)
+            want = lib.orthogonalize(g, torch.empty_like(g))
+            same = g.clone()
+            assert lib.orthogonalize(same, same) is same and torch.equal(same, want)
+            want0 = lib.orthogonalize(g, torch.empty_like(g), steps=0)
+            lib.orthogonalize(g, g, steps=0)
+            assert torch.equal(g, want0)
+
+
+def test_batches_do_not_mix_and_order_does_not_matter():
+    lib = _lib()
+    for dtype in TYPES:
+        for size in ((20, 33), (150, 140)):
+            g = data(1, dtype, 5, *size)
+            alone = lib.orthogonalize(g, torch.empty_like(g))
+            check(alone, g)
+            other = g.clone()
+            other[[0, 1, 3, 4]] = data(2, dtype, 4, *size)
+            assert torch.equal(alone[2], lib.orthogonalize(other, torch.empty_like(other))[2])
+            turned = g.transpose(1, 2).contiguous()
+            check(lib.orthogonalize(turned, torch.empty_like(turned)), turned)
+
+
+def test_nothing_to_do():
+    lib = _lib()
+    for shape in ((0, 4, 4), (2, 0, 4), (2, 4, 0)):
+        g = torch.empty(shape, device="cuda")
+        assert lib.orthogonalize(g, torch.empty_like(g)).shape == shape
+
+
+def test_captured_replayed_and_on_two_streams():
+    lib = _lib()
+    for size in ((3, 64, 100), (1, 260, 200)):
+        g, out = data(1, torch.float32, *size), torch.zeros(size, device="cuda")
+        graphs = []
+        for _ in range(2):   # two graphs, each with a workspace of its own
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                lib.orthogonalize(g, out)
+            torch.cuda.synchronize()
+            graph, mine = torch.cuda.CUDAGraph(), torch.zeros(size, device="cuda")
+            with torch.cuda.graph(graph):
+                lib.orthogonalize(g, mine)
+            graphs.append((graph, mine))
+        for seed in range(5):
+            g.copy_(data(10 + seed, torch.float32, *size))
+            torch.cuda.synchronize()
+            for (graph, _), s in zip(graphs, [torch.cuda.Stream() for _ in graphs]):
+                with torch.cuda.stream(s):
+                    graph.replay()
+            torch.cuda.synchronize()
+            lib.orthogonalize(g, out)
+            check(out, g)
+            assert all(torch.equal(mine, out) for _, mine in graphs)
+
+
+def test_refusals():
+    lib = _lib()
+    g = torch.zeros(2, 4, 6, device="cuda")
+    for bad in (
+        lambda: lib.orthogonalize(g.cpu(), g),
+        lambda: lib.orthogonalize(g, g.half()),
+        lambda: lib.orthogonalize(g, torch.zeros(2, 4, 5, device="cuda")),
+        lambda: lib.orthogonalize(g.int(), g.int()),
+        lambda: lib.orthogonalize(g.transpose(1, 2), g.transpose(1, 2)),
+        lambda: lib.orthogonalize(g[0, 0], g[0, 0]),
+        lambda: lib.orthogonalize(g, g, steps=3, coef=[(1.0, 0.0, 0.0)] * 2),
+        lambda: lib.orthogonalize(g, g, coef=(1.0, 0.0)),
+    ):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (
+        lambda: lib.orthogonalize(g, g, steps=-1),
+        lambda: lib.orthogonalize(g, g, steps=65),
+        lambda: lib.orthogonalize(g, g, eps=0.0),
+        lambda: lib.orthogonalize(g, g, eps=float("nan")),
+        lambda: lib.orthogonalize(g, g, coef=(float("inf"), 0.0, 0.0)),
+        lambda: lib.orthogonalize(g, g[:1].expand(2, 4, 6)),
+    ):
+        with pytest.raises(lib.GpxError):
+            bad()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_training_step_of_experts_with_learned_projections(dtype):
+    """Forward, both gradients and the orthogonalised update of every expert, against autograd and the definition in double."""
+    lib = _lib()
+    sizes, n, k = [60, 0, 130, 5], 24, 50
+    rows, off = sum(sizes), table(sizes)
+    x, w, target = data(1, dtype, rows, k), (data(2, torch.float64, 4, n, k) / 7).to(dtype), data(3, dtype, rows, n)
+    y = lib.grouped_gemm(x, w, off, torch.empty(rows, n, dtype=dtype, device="cuda"))
+    dy = y - target   # of L = |Y - target|^2 / 2
+    dx = lib.grouped_gemm(dy, w, off, torch.empty_like(x), w_kc=False)
+    dw = lib.grouped_gemm_dw(x, dy, off, torch.empty_like(w))
+    update = lib.orthogonalize(dw, torch.empty_like(dw))
+    new = w - 0.1 * update
+
+    xd, wd = x.double().cpu().requires_grad_(), w.double().cpu().requires_grad_()
+    ends = off.tolist()
+    yd = torch.cat([xd[a:b] @ wd[g].T for g, (a, b) in enumerate(zip(ends[:-1], ends[1:]))])
+    (0.5 * (yd - target.double().cpu()).square().sum()).backward()
+    # dy is rounded twice before the products take it, w and x not at all: norm-wise 4 half steps cover dx and dw
+    half = 4 * oracle.HALF[dtype] + (1e-14 if dtype == torch.float64 else 1e-6)
+    for got, want in ((y, yd.detach()), (dx, xd.grad), (dw, wd.grad)):
+        assert float(torch.linalg.norm(got.double().cpu() - want)) <= half * float(torch.linalg.norm(want))
+    check(update, dw)
+    assert torch.equal(new[1], w[1])   # the expert without rows: zero gradient, zero update
