@@ -95,7 +95,7 @@ __device__ __forceinline__ void put(char* row, int j, int N, const A* v, A alpha
         if (j + x < N) p[x] = (O)(beta != A(0) ? alpha * v[x] + beta * (A)p[x] : alpha * v[x]);
 }
 
-template <class T, int BM, int BN, int WR, int WC, bool WKC>
+template <class T, int BM, int BN, int WR, int WC, bool WKC, bool DIRECT>
 __global__ __launch_bounds__(WR * WC * 64, 2) void grouped_kernel(const GroupedArgs g) {
     typedef mm::Tile<T, BM, BN, WR, WC, true, WKC> Tile;
     typedef typename Tile::one A;
@@ -108,7 +108,8 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void grouped_kernel(const GroupedA
     typename Tile::OpQ q = {g.W + rt.group * g.stride_w + (WKC ? n0 * g.ldw : n0 * (long)sizeof(T)), g.ldw, min(g.N - n0, BN), g.K};
     Tile t;
     t.clear();
-    t.run_staged(lds, p, q, g.K);
+    if (DIRECT) t.run_direct(lds, p, q, g.K);
+    else t.run_staged(lds, p, q, g.K);
     char* y = g.Y + rt.row0 * g.ldy;
     const A alpha = (A)g.alpha, beta = (A)g.beta;
     t.each([&](int i, int j, const A* v, auto cnt) {
@@ -126,7 +127,12 @@ struct GroupedDwArgs {
     int vec;
 };
 
-template <class T, class O, int BM, int BN, int WR, int WC>
+// rows in whole, aligned 16-byte chunks: what a direct-to-LDS load needs
+bool whole_chunks(const void* p, long ld_bytes, long stride_bytes, long extent, long elem) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld_bytes % 16 == 0 && stride_bytes % 16 == 0 && extent * elem % 16 == 0;
+}
+
+template <class T, class O, int BM, int BN, int WR, int WC, bool DIRECT>
 __global__ __launch_bounds__(WR * WC * 64, 2) void grouped_dw_kernel(const GroupedDwArgs g) {
     typedef mm::Tile<T, BM, BN, WR, WC, false, false> Tile;
     typedef typename Tile::one A;
@@ -140,7 +146,8 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void grouped_dw_kernel(const Group
     typename Tile::OpQ q = {g.X + lo * g.ldx + m0 * (long)sizeof(T), g.ldx, min(g.M - m0, BN), rows};
     Tile t;
     t.clear();
-    t.run_staged(lds, p, q, rows);
+    if (DIRECT) t.run_direct(lds, p, q, rows);
+    else t.run_staged(lds, p, q, rows);
     char* c = g.C + group * g.stride_c + n0 * g.ldc;
     const A alpha = (A)g.alpha, beta = (A)g.beta;
     t.each([&](int i, int j, const A* v, auto cnt) {
@@ -148,25 +155,53 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void grouped_dw_kernel(const Group
     });
 }
 
-template <class T> int grouped_typed(hipStream_t st, int w_kc, GroupedArgs& g) {
-    constexpr int BM = 128, BN = 128;
-    const long mt = g.T / BM + (g.groups < g.T ? g.groups : g.T);   // sum of ceil(rows / BM) is never more
-    const long nt = (g.N + BN - 1) / BN;
-    if (mt * nt >= 1L << 31) return GPX_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)(mt * nt));
-    if (w_kc) grouped_kernel<T, BM, BN, 2, 2, true><<<grid, 256, 0, st>>>(g);
-    else grouped_kernel<T, BM, BN, 2, 2, false><<<grid, 256, 0, st>>>(g);
+// A row-tile count that is never less than sum of ceil(rows / BM)
+long row_tiles(long T, int groups, int BM) { return T / BM + (groups < T ? groups : T); }
+
+template <class T, int BM, int BN, int WR, int WC> int grouped_launch(hipStream_t st, bool w_kc, bool direct, const GroupedArgs& g) {
+    const long tiles = row_tiles(g.T, g.groups, BM) * ((g.N + BN - 1) / BN);
+    if (tiles >= 1L << 31) return GPX_ERR_UNSUPPORTED;
+    auto go = [&](auto kc, auto dir) {
+        grouped_kernel<T, BM, BN, WR, WC, decltype(kc)::value, decltype(dir)::value><<<(unsigned)tiles, WR * WC * 64, 0, st>>>(g);
+    };
+    if (w_kc && direct) go(std::true_type{}, std::true_type{});
+    else if (w_kc) go(std::true_type{}, std::false_type{});
+    else if (direct) go(std::false_type{}, std::true_type{});
+    else go(std::false_type{}, std::false_type{});
+    HIP_TRY(hipGetLastError());
+    return GPX_OK;
+}
+// 16-bit products: 256 x 256 tiles (one workgroup of 8 waves per CU, 128 KB of LDS) once they fill the chip, else 128 x 128
+// (two workgroups of 4 waves per CU).  bf16, 8 x (4096 x 4096 x 7168): 1.17-1.23 PFLOP/s against 1.02-1.05; 8 groups of one
+// row, N = 1024, K = 512: 17.5 us against 11.5.
+bool tile256(long row_tiles256, long N) { return row_tiles256 * ((N + 255) / 256) >= 256; }
+
+template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArgs& g) {
+    // rows of X (k contiguous) and of W in 16-byte chunks, lane offsets of one K step within the buffer resource
+    const long wn = w_kc ? g.K : g.N;   // W's contiguous extent
+    const bool direct = whole_chunks(g.X, g.ldx, 0, g.K, sizeof(T)) && whole_chunks(g.W, g.ldw, g.stride_w, wn, sizeof(T)) &&
+                        256 * g.ldx < (long)mm::kRange && 256 * g.ldw < (long)mm::kRange;
+    if constexpr (sizeof(T) == 2)
+        if (tile256(g.T / 256 + g.groups / 2, g.N)) return grouped_launch<T, 256, 256, 2, 4>(st, w_kc, direct, g);
+    return grouped_launch<T, 128, 128, 2, 2>(st, w_kc, direct, g);
+}
+
+template <class T, class O, int BM, int BN, int WR, int WC> int grouped_dw_launch(hipStream_t st, bool direct, const GroupedDwArgs& g, int groups) {
+    const long tiles = (long)((g.N + BM - 1) / BM) * ((g.M + BN - 1) / BN);
+    if (tiles >= 1L << 31) return GPX_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)tiles, (unsigned)groups);
+    if (direct) grouped_dw_kernel<T, O, BM, BN, WR, WC, true><<<grid, WR * WC * 64, 0, st>>>(g);
+    else grouped_dw_kernel<T, O, BM, BN, WR, WC, false><<<grid, WR * WC * 64, 0, st>>>(g);
     HIP_TRY(hipGetLastError());
     return GPX_OK;
 }
 
-template <class T, class O> int grouped_dw_typed(hipStream_t st, GroupedDwArgs& g, int groups) {
-    constexpr int BM = 128, BN = 128;
-    const long tiles = (long)((g.N + BM - 1) / BM) * ((g.M + BN - 1) / BN);
-    if (tiles >= 1L << 31) return GPX_ERR_UNSUPPORTED;
-    grouped_dw_kernel<T, O, BM, BN, 2, 2><<<dim3((unsigned)tiles, (unsigned)groups), 256, 0, st>>>(g);
-    HIP_TRY(hipGetLastError());
-    return GPX_OK;
+template <class T, class O> int grouped_dw_typed(hipStream_t st, const GroupedDwArgs& g, int groups) {
+    const bool direct = whole_chunks(g.X, g.ldx, 0, g.M, sizeof(T)) && whole_chunks(g.Z, g.ldz, 0, g.N, sizeof(T)) &&
+                        64 * g.ldx < (long)mm::kRange && 64 * g.ldz < (long)mm::kRange;
+    if constexpr (sizeof(T) == 2)
+        if (tile256((long)groups * ((g.N + 255) / 256), g.M)) return grouped_dw_launch<T, O, 256, 256, 2, 4>(st, direct, g, groups);
+    return grouped_dw_launch<T, O, 128, 128, 2, 2>(st, direct, g, groups);
 }
 
 constexpr long kMaxExtent = (1L << 31) - 1024;   // row, column and k numbers within one product are 32-bit
@@ -197,10 +232,10 @@ extern "C" int gpx_grouped_gemm(int dtype, int w_kc, int64_t groups, int64_t T, 
                      stride_w * e, ldy * e, T, (int)groups, (int)N, (int)K, alpha, beta, rows4(Y, ldy * e, 0, e)};
     const hipStream_t st = static_cast<hipStream_t>(hip_stream);
     switch (dtype) {
-        case GPX_F64: return grouped_typed<double>(st, w_kc, g);
-        case GPX_F32: return grouped_typed<float>(st, w_kc, g);
-        case GPX_BF16: return grouped_typed<__bf16>(st, w_kc, g);
-        default: return grouped_typed<_Float16>(st, w_kc, g);
+        case GPX_F64: return grouped_typed<double>(st, w_kc != 0, g);
+        case GPX_F32: return grouped_typed<float>(st, w_kc != 0, g);
+        case GPX_BF16: return grouped_typed<__bf16>(st, w_kc != 0, g);
+        default: return grouped_typed<_Float16>(st, w_kc != 0, g);
     }
 }
 

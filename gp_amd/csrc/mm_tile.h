@@ -101,6 +101,9 @@ template <class T> __device__ __forceinline__ v4i load_chunk(const char* p, int 
     return v;
 }
 
+constexpr unsigned kRange = 0x7fff0000u;     // bytes that the lane offsets of one K step may span (checked by the host)
+constexpr unsigned kOutside = 0x7fff8000u;   // an offset behind them
+
 template <class T, int ROWS, bool KC, int NT> struct Operand {
     static constexpr int E = chunk_elems<T>(), BK = step_k<T>();
     static constexpr int NL = ROWS * 8 / NT;   // chunks per thread
@@ -132,6 +135,32 @@ template <class T, int ROWS, bool KC, int NT> struct Operand {
             if (KC) r[it] = load_chunk<T>(base + row * ld + (long)k * sizeof(T), row < rows ? K - k : 0);
             else r[it] = load_chunk<T>(base + k * ld + (long)row * sizeof(T), k < K ? rows - row : 0);
         }
+    }
+    // ---- straight from memory into LDS: 16-byte aligned rows whose contiguous extent is a multiple of E elements, so that
+    // a chunk exists as a whole or not at all.  A chunk that does not exist gets an offset behind the resource's
+    // range: the load returns zeros without touching memory.
+    struct Lanes { unsigned off[NL]; };
+    __device__ __forceinline__ Lanes lanes(int k_valid) const {   // of one K step that has k_valid values of k
+        Lanes l;
+#pragma unroll
+        for (int it = 0; it < NL; ++it) {
+            int row, k;
+            place(it * NT + (int)threadIdx.x, row, k);
+            const unsigned at = KC ? (unsigned)(row * ld) + k * (unsigned)sizeof(T) : (unsigned)(k * ld) + row * (unsigned)sizeof(T);
+            l.off[it] = row < rows && k < k_valid ? at : kOutside;
+        }
+        return l;
+    }
+    __device__ __forceinline__ void issue(unsigned lds_addr, const Lanes& l, int step) const {
+        const unsigned long long a = reinterpret_cast<unsigned long long>(base) + (unsigned long long)step * (KC ? 128 : BK * ld);
+        const v4i rsrc = {__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff)),
+                          (int)kRange, 0x00027000};
+        const unsigned wave_addr = __builtin_amdgcn_readfirstlane(lds_addr + (threadIdx.x >> 6) * 1024);
+#pragma unroll
+        for (int it = 0; it < NL; ++it)   // lane l of the wave writes the 16 bytes at M0 + 16 l
+            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(l.off[it]), "s"(rsrc),
+                         "s"(wave_addr + it * NT * 16)
+                         : "memory");
     }
     __device__ __forceinline__ void stash(char* s, const v4i (&r)[NL]) const {
 #pragma unroll
@@ -195,6 +224,30 @@ template <class T, int BM, int BN, int WR, int WC, bool PKC, bool QKC> struct Ti
             }
             __syncthreads();   // also: nobody reads the other stage any more when the next step writes it
             multiply(st);
+        }
+    }
+    // K loop on direct loads: step k + 1 is on its way into one LDS stage while step k is multiplied from the other
+    __device__ __forceinline__ void run_direct(char* lds, const OpP& p, const OpQ& q, int K) {
+        constexpr int BK = OpP::BK;
+        const int full = K / BK, rest = K - full * BK, steps = full + (rest != 0);
+        if (steps == 0) return;
+        typename OpP::Lanes lp = p.lanes(BK);
+        typename OpQ::Lanes lq = q.lanes(BK);
+        const unsigned at = (unsigned)reinterpret_cast<unsigned long long>((__attribute__((address_space(3))) char*)lds);
+        auto issue = [&](int s) {
+            if (s >= full) {
+                lp = p.lanes(rest);
+                lq = q.lanes(rest);
+            }
+            p.issue(at + (s & 1) * STAGE, lp, s);
+            q.issue(at + (s & 1) * STAGE + OpP::BYTES, lq, s);
+        };
+        issue(0);
+        for (int s = 0; s < steps; ++s) {
+            // this wave's part of step s has arrived, and it reads nothing of the stage that step s + 1 overwrites any more
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (s + 1 < steps) issue(s + 1);
+            multiply(lds + (s & 1) * STAGE);
         }
     }
     // f(i, j, value pointer, count): count consecutive columns j.. of row i of the tile
