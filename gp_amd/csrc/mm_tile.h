@@ -64,6 +64,24 @@ __device__ __forceinline__ v4i frag(const char* s, int row0, int kk, int lane) {
     }
 }
 
+// Split format (mm::Split): a matrix of values known to 22 bits as two f16 planes, v = hi + lo, in blocks of 32 columns:
+// element (r, c) has hi at r*ld + (c / 32)*64 + c % 32 and lo 32 elements behind it.  128 bytes are 32 values, so that a K step
+// has the geometry of 16-bit operands: its two 64-byte halves are the two planes.  Rows end in zeros up to a whole block.
+struct Split {};
+template <int ROWS, bool KC>
+__device__ __forceinline__ v4i frag_split(const char* s, int row0, int lo, int lane) {
+    if constexpr (KC) return frag<_Float16, ROWS, true>(s, row0, lo, lane);
+    const int r = lane & 15, q = lane >> 4;
+    const int k = 8 * q + (r >> 2);
+    const int b = ((row0 >> 5) * 4 + ((row0 >> 4) & 1) + 2 * lo) ^ strided_swizzle<_Float16>(k);
+    const char* p = s + k * (ROWS * 4) + b * 32 + (r & 3) * 8;
+    typedef __attribute__((address_space(3))) v4s lds4;
+    union { v4s h[2]; v4i v; } u;
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * ROWS * 4));
+    return u.v;
+}
+
 // D += A B^T over the 64 bytes of k of the fragments.  The lane holds D rows (index of `a`) 4q + r (doubles: q + 4r),
 // r = 0..3, and the column (index of `b`) lane & 15.
 template <class T> __device__ __forceinline__ typename Acc<T>::vec mma(v4i a, v4i b, typename Acc<T>::vec c) {
@@ -104,23 +122,29 @@ template <class T> __device__ __forceinline__ v4i load_chunk(const char* p, int 
 constexpr unsigned kRange = 0x7fff0000u;     // bytes that the lane offsets of one K step may span (checked by the host)
 constexpr unsigned kOutside = 0x7fff8000u;   // an offset behind them
 
-template <class T, int ROWS, bool KC, int NT> struct Operand {
-    static constexpr int E = chunk_elems<T>(), BK = step_k<T>();
+// what a type is stored as, and the values of k in a step
+template <class T> struct Stored { typedef T type; static constexpr int BK = step_k<T>(), WIDE = 1; static constexpr bool split = false; };
+template <> struct Stored<Split> { typedef _Float16 type; static constexpr int BK = 32, WIDE = 2; static constexpr bool split = true; };
+
+template <class F, int ROWS, bool KC, int NT> struct Operand {
+    typedef typename Stored<F>::type T;
+    static constexpr int E = chunk_elems<T>(), BK = Stored<F>::BK;
+    static constexpr int COLS = ROWS * Stored<F>::WIDE;   // elements per k of an operand with k strided
     static constexpr int NL = ROWS * 8 / NT;   // chunks per thread
     static constexpr int BYTES = ROWS * 128;
     static_assert(ROWS * 8 % NT == 0, "whole chunks per thread");
     const char* base;   // element (0, 0) of the tile's rows
     long ld;            // bytes between rows (KC) or between k (otherwise)
-    int rows, K;        // rows of the tile and extent of k that exist
+    int rows, K;        // rows of the tile (split, k strided: elements) and extent of k that exist
 
     __device__ __forceinline__ void place(int c, int& row, int& k) const {   // first element of chunk c
         if (KC) {
             row = c >> 3;
             k = ((c & 7) ^ (row & 7)) * E;
         } else {
-            constexpr int PER = ROWS / E;              // chunks per k
+            constexpr int PER = COLS / E;              // chunks per k
             constexpr int HB = 16 / E;                 // chunks per block of 16 columns
-            constexpr int mask = ROWS / 16 < 8 ? ROWS / 16 - 1 : 7;
+            constexpr int mask = COLS / 16 < 8 ? COLS / 16 - 1 : 7;
             k = c / PER;
             const int slot = c % PER;
             row = ((slot / HB) ^ (strided_swizzle<T>(k) & mask)) * 16 + slot % HB * E;
@@ -147,7 +171,7 @@ template <class T, int ROWS, bool KC, int NT> struct Operand {
             int row, k;
             place(it * NT + (int)threadIdx.x, row, k);
             const unsigned at = KC ? (unsigned)(row * ld) + k * (unsigned)sizeof(T) : (unsigned)(k * ld) + row * (unsigned)sizeof(T);
-            l.off[it] = row < rows && k < k_valid ? at : kOutside;
+            l.off[it] = row < rows && (k < k_valid || (KC && Stored<F>::split)) ? at : kOutside;
         }
         return l;
     }
@@ -172,16 +196,17 @@ template <class T, int ROWS, bool KC, int NT> struct Operand {
 // Waves in a WR (rows i) x WC (columns j) grid; each owns TI x TJ fragments of 16.  SWAP: the accumulator's contiguous
 // lanes run along j (doubles and floats: whole 64..128-byte runs per store); otherwise its four registers do (16-bit
 // results: 8-byte stores instead of single elements).
-template <class T, int BM, int BN, int WR, int WC, bool PKC, bool QKC> struct Tile {
+template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGES = 2> struct Tile {
+    typedef typename Stored<F>::type T;
     static constexpr int NT = WR * WC * 64;
     static constexpr int TI = BM / WR / 16, TJ = BN / WC / 16;
     static constexpr bool SWAP = sizeof(T) != 2;
-    typedef Operand<T, BM, PKC, NT> OpP;
-    typedef Operand<T, BN, QKC, NT> OpQ;
+    typedef Operand<F, BM, PKC, NT> OpP;
+    typedef Operand<F, BN, QKC, NT> OpQ;
     typedef typename Acc<T>::vec vec;
     typedef typename Acc<T>::one one;
     static constexpr int STAGE = OpP::BYTES + OpQ::BYTES;
-    static constexpr int LDS = 2 * STAGE;
+    static constexpr int LDS = STAGES * STAGE;
     vec acc[TI][TJ];
 
     __device__ __forceinline__ void clear() {
@@ -193,6 +218,26 @@ template <class T, int BM, int BN, int WR, int WC, bool PKC, bool QKC> struct Ti
     __device__ __forceinline__ void multiply(const char* s) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const int i0 = wave / WC * (BM / WR), j0 = wave % WC * (BN / WC);
+        if constexpr (Stored<F>::split) {
+            // (ph + pl)(qh + ql) without pl ql, which is 2^-22 of the product at most
+            v4i qh[TJ], ql[TJ];
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) {
+                qh[j] = frag_split<BN, QKC>(s + OpP::BYTES, j0 + 16 * j, 0, lane);
+                ql[j] = frag_split<BN, QKC>(s + OpP::BYTES, j0 + 16 * j, 1, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < TI; ++i) {
+                const v4i ph = frag_split<BM, PKC>(s, i0 + 16 * i, 0, lane), pl = frag_split<BM, PKC>(s, i0 + 16 * i, 1, lane);
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) acc[i][j] = mma<T>(ql[j], ph, acc[i][j]);
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) acc[i][j] = mma<T>(qh[j], pl, acc[i][j]);
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) acc[i][j] = mma<T>(qh[j], ph, acc[i][j]);
+            }
+            return;
+        }
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             v4i fp[TI], fq[TJ];
@@ -226,32 +271,48 @@ template <class T, int BM, int BN, int WR, int WC, bool PKC, bool QKC> struct Ti
             multiply(st);
         }
     }
-    // K loop on direct loads: step k + 1 is on its way into one LDS stage while step k is multiplied from the other
+    // K loop on direct loads, STAGES LDS stages: while step s is multiplied, steps s + 1 .. s + STAGES - 1 are on their way
     __device__ __forceinline__ void run_direct(char* lds, const OpP& p, const OpQ& q, int K) {
         constexpr int BK = OpP::BK;
+        constexpr int AHEAD = (STAGES - 2) * (OpP::NL + OpQ::NL);   // loads of this wave behind those of the step waited for
         const int full = K / BK, rest = K - full * BK, steps = full + (rest != 0);
-        if (steps == 0) return;
         typename OpP::Lanes lp = p.lanes(BK);
         typename OpQ::Lanes lq = q.lanes(BK);
         const unsigned at = (unsigned)reinterpret_cast<unsigned long long>((__attribute__((address_space(3))) char*)lds);
-        auto issue = [&](int s) {
+        auto issue = [&](int s, int stage) {
             if (s >= full) {
                 lp = p.lanes(rest);
                 lq = q.lanes(rest);
             }
-            p.issue(at + (s & 1) * STAGE, lp, s);
-            q.issue(at + (s & 1) * STAGE + OpP::BYTES, lq, s);
+            p.issue(at + stage * STAGE, lp, s);
+            q.issue(at + stage * STAGE + OpP::BYTES, lq, s);
         };
-        issue(0);
+        for (int s = 0; s < STAGES - 1 && s < steps; ++s) issue(s, s);
+        int stage = 0, into = STAGES - 1;   // of step s, of step s + STAGES - 1
         for (int s = 0; s < steps; ++s) {
-            // this wave's part of step s has arrived, and it reads nothing of the stage that step s + 1 overwrites any more
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (s + 1 < steps) issue(s + 1);
-            multiply(lds + (s & 1) * STAGE);
+            // this wave's part of step s has arrived, and it reads nothing of the stage that is overwritten next any more
+            if (STAGES > 2 && s + STAGES - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(AHEAD) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (s + STAGES - 1 < steps) issue(s + STAGES - 1, into);
+            multiply(lds + stage * STAGE);
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            into = into + 1 == STAGES ? 0 : into + 1;
         }
     }
+    // The accumulators of wave row `pass` (BM / WR rows of the tile) as floats in LDS, rows of SLAB_LD: what an epilogue that
+    // reads and writes whole 16-byte runs needs.  Between barriers of the caller.
+    static constexpr int SLAB_ROWS = BM / WR, SLAB_LD = BN + 4, SLAB = SLAB_ROWS * SLAB_LD * 4;
+    __device__ __forceinline__ void to_slab(float* slab, int pass) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+        if (wave / WC != pass) return;
+        const int j0 = wave % WC * (BN / WC);
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) *reinterpret_cast<v4f*>(slab + (16 * i + r) * SLAB_LD + j0 + 16 * j + 4 * q) = acc[i][j];
+    }
     // f(i, j, value pointer, count): count consecutive columns j.. of row i of the tile
-    template <class F> __device__ __forceinline__ void each(F&& f) {
+    template <class Put> __device__ __forceinline__ void each(Put&& f) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
         const int i0 = wave / WC * (BM / WR), j0 = wave % WC * (BN / WC);
 #pragma unroll

@@ -6,26 +6,60 @@
 // stay two, the square ones have the short side.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include "mm_tile.h"
 #include "../../include/gpx.h"
 
 namespace {
 
-constexpr int kParts = 64;   // partial sums of squares per matrix
+constexpr int kParts = 256;   // partial sums of squares per matrix, at most
 
 template <class T> __device__ __forceinline__ double as_double(T v) { return (double)v; }
 
-// sums of squares in double: neither overflow nor loss for any float input, one order of addition
+// Walks the runs of 8 neighbours of a rows x cols matrix, run number `first` and every `step`-th behind it, without a
+// division per run: f(row, first column of the run).
+template <class Body> __device__ __forceinline__ void each_run(int rows, int cols, long first, long step, Body&& f) {
+    const int n8 = (cols + 7) / 8;
+    long r = first / n8, dr = step / n8;
+    int c = (int)(first % n8), dc = (int)(step % n8);
+    while (r < rows) {
+        f((int)r, c * 8);
+        r += dr;
+        c += dc;
+        if (c >= n8) {
+            c -= n8;
+            ++r;
+        }
+    }
+}
+// v = the run at p, of which `count` elements exist
+template <class T> __device__ __forceinline__ void load_run(const T* p, int count, T (&v)[8]) {
+    if (count >= 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+        constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+        for (int x = 0; x < 8; x += E) {
+            union { mm::v4i w; T e[E]; } u;
+            u.w = *reinterpret_cast<const mm::v4i*>(p + x);
+#pragma unroll
+            for (int y = 0; y < E; ++y) v[x + y] = u.e[y];
+        }
+    } else {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = x < count ? p[x] : (T)0.0f;
+    }
+}
+
+// Sums of squares in double: neither overflow nor loss for any narrower input, one order of addition.
 template <class T>
 __global__ __launch_bounds__(256) void ortho_norm_kernel(const T* __restrict__ G, long ldg, long stride_g, int rows, int cols, double* __restrict__ part) {
     const T* g = G + blockIdx.y * stride_g;
-    const long total = (long)rows * cols, per = (total + kParts - 1) / kParts;
-    const long lo = blockIdx.x * per, hi = min(total, lo + per);
     double s = 0.0;
-    for (long e = lo + threadIdx.x; e < hi; e += 256) {
-        const double v = as_double(g[e / cols * ldg + e % cols]);
-        s = fma(v, v, s);
-    }
+    each_run(rows, cols, blockIdx.x * 256L + threadIdx.x, gridDim.x * 256L, [&](int r, int c) {
+        T v[8];
+        load_run(g + r * ldg + c, cols - c, v);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) s = fma(as_double(v[x]), as_double(v[x]), s);
+    });
 #pragma unroll
     for (int d = 32; d; d /= 2) s += __shfl_xor(s, d, 64);
     __shared__ double ws[4];
@@ -34,108 +68,608 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const T* __restrict__ G
     if (threadIdx.x == 0) part[blockIdx.y * kParts + blockIdx.x] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
 }
 
-template <class T, class O>
-__global__ __launch_bounds__(256) void ortho_scale_kernel(const T* G, long ldg, long stride_g, int rows, int cols, const double* __restrict__ part,
-                                                          double eps, O* X, long ldx, long stride_x) {
-    double s = part[blockIdx.y * kParts + (threadIdx.x & 63)];
+// the norm of one matrix from its partial sums, in every lane
+__device__ __forceinline__ double norm_of(const double* part, int parts) {
+    double s = 0.0;
+    for (int e = threadIdx.x & 63; e < parts; e += 64) s += part[e];
 #pragma unroll
     for (int d = 32; d; d /= 2) s += __shfl_xor(s, d, 64);
-    const double norm = sqrt(s) + eps;
-    const long total = (long)rows * cols;
-    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long)gridDim.x * 256) {
-        const long r = e / cols, c = e % cols;
-        X[blockIdx.y * stride_x + r * ldx + c] = (O)(as_double(G[blockIdx.y * stride_g + r * ldg + c]) / norm);
-    }
+    return sqrt(s);
 }
 
-// D = c1 P Q^T + c2 E over a batch; W: type of the iterates (float, or double for double matrices)
+// steps == 0: the normalised matrix itself.  G and X may be the same buffer.
+template <class T>
+__global__ __launch_bounds__(256) void ortho_normalize_kernel(const T* G, long ldg, long stride_g, int rows, int cols, const double* __restrict__ part,
+                                                              int parts, double eps, T* X, long ldx, long stride_x) {
+    const double norm = norm_of(part + blockIdx.y * kParts, parts) + eps;
+    each_run(rows, cols, blockIdx.x * 256L + threadIdx.x, gridDim.x * 256L, [&](int r, int c) {
+        T v[8];
+        load_run(G + blockIdx.y * stride_g + r * ldg + c, cols - c, v);
+        T* x = X + blockIdx.y * stride_x + r * ldx + c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c + e < cols) x[e] = (T)(as_double(v[e]) / norm);
+    });
+}
+
+// ---- the iterates ------------------------------------------------------------------------------------------------
+// Double matrices stay in double.  All others are iterated in the split format, two f16 planes under one power of two per
+// matrix and step: 22 bits of every value, the accumulators and all sums in 32.  One f16 product is 16 times the rate of a
+// product of floats here, the three that the split needs leave a factor of five.  The host bounds the singular values of
+// every iterate from the coefficients and places the largest possible element at 2^15: nothing overflows, and the smallest
+// step of the second plane is 2^-39 of that bound.
+template <class F> struct Iterate;
+template <> struct Iterate<double> {
+    static constexpr int PAD = 2;
+    __device__ static void store(char* row, int j, double v) { reinterpret_cast<double*>(row)[j] = v; }
+    __device__ static double load(const char* row, int j) { return reinterpret_cast<const double*>(row)[j]; }
+    static long bytes(long cols) { return cols * 8; }
+};
+template <> struct Iterate<mm::Split> {
+    static constexpr int PAD = 32;
+    __device__ static long at(int j) { return (long)(j >> 5) * 64 + (j & 31); }
+    __device__ static void store(char* row, int j, float v) {
+        _Float16* p = reinterpret_cast<_Float16*>(row) + at(j);
+        const _Float16 h = (_Float16)v;
+        p[0] = h;
+        p[32] = (_Float16)(v - (float)h);
+    }
+    __device__ static float load(const char* row, int j) {
+        const _Float16* p = reinterpret_cast<const _Float16*>(row) + at(j);
+        return (float)p[0] + (float)p[32];
+    }
+    static long bytes(long cols) { return cols * 4; }
+    // eight neighbours from column j on, j a multiple of 8
+    __device__ static void store8(char* row, int j, const float (&v)[8]) {
+        mm::v8h h, l;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            h[x] = (_Float16)v[x];
+            l[x] = (_Float16)(v[x] - (float)h[x]);
+        }
+        _Float16* p = reinterpret_cast<_Float16*>(row) + at(j);
+        *reinterpret_cast<mm::v8h*>(p) = h;
+        *reinterpret_cast<mm::v8h*>(p + 32) = l;
+    }
+    __device__ static void add8(const char* row, int j, float by, float (&v)[8]) {   // v += by * row
+        const _Float16* p = reinterpret_cast<const _Float16*>(row) + at(j);
+        const mm::v8h h = *reinterpret_cast<const mm::v8h*>(p), l = *reinterpret_cast<const mm::v8h*>(p + 32);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] += by * ((float)h[x] + (float)l[x]);
+    }
+};
+template <class F> int padded(int cols) { return (cols + Iterate<F>::PAD - 1) / Iterate<F>::PAD * Iterate<F>::PAD; }
+
+template <class T, class F>
+__global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ G, long ldg, long stride_g, int rows, int cols, int pcols,
+                                                          const double* __restrict__ part, int parts, double eps, double scale, char* __restrict__ X,
+                                                          long ldx, long stride_x) {
+    const double by = scale / (norm_of(part + blockIdx.y * kParts, parts) + eps);
+    each_run(rows, pcols, blockIdx.x * 256L + threadIdx.x, gridDim.x * 256L, [&](int r, int c) {
+        T v[8];
+        load_run(G + blockIdx.y * stride_g + r * ldg + c, cols - c, v);
+        char* x = X + blockIdx.y * stride_x + r * ldx;
+        if constexpr (mm::Stored<F>::split) {
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = (float)(as_double(v[e]) * by);
+            Iterate<F>::store8(x, c, w);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < pcols) Iterate<F>::store(x, c + e, as_double(v[e]) * by);
+        }
+    });
+}
+
+// D = c1 P Q^T + c2 E + c3 I over a batch, E and D in the format F, or (LAST) D in the type O of the result.
+// SYM: D is symmetric; tiles on and below the diagonal are computed, and those below it stored on both sides.
 struct OrthoArgs {
     const char* P; const char* Q; const char* E; char* D;
     long ldp, ldq, lde, ldd, sp, sq, se, sd;   // bytes
     int I, J, K;
-    double c1, c2;
+    double c1, c2, c3;
 };
-template <class W, class O, bool PKC, bool QKC>
-__global__ __launch_bounds__(256, 2) void ortho_mm_kernel(const OrthoArgs g) {
-    typedef mm::Tile<W, 128, 128, 2, 2, PKC, QKC> Tile;
-    __shared__ __attribute__((aligned(128))) char lds[Tile::LDS];
-    const int jt = (g.J + 127) / 128;
-    const int i0 = (int)(blockIdx.x / jt) * 128, j0 = (int)(blockIdx.x % jt) * 128;
-    typename Tile::OpP p = {g.P + blockIdx.y * g.sp + (PKC ? i0 * g.ldp : i0 * (long)sizeof(W)), g.ldp, min(g.I - i0, 128), g.K};
-    typename Tile::OpQ q = {g.Q + blockIdx.y * g.sq + (QKC ? j0 * g.ldq : j0 * (long)sizeof(W)), g.ldq, min(g.J - j0, 128), g.K};
+template <class F, class O, bool LAST, int B, int WR, int WC, int ST, bool PKC, bool QKC, bool SYM>
+__global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2) void ortho_mm_kernel(const OrthoArgs g) {
+    typedef mm::Tile<F, B, B, WR, WC, PKC, QKC, ST> Tile;
+    typedef typename Tile::one one;
+    constexpr int W = mm::Stored<F>::WIDE * (int)sizeof(typename Tile::T);   // bytes per value
+    constexpr int WE = mm::Stored<F>::WIDE;
+    constexpr int LDS = mm::Stored<F>::split && Tile::SLAB > Tile::LDS ? Tile::SLAB : Tile::LDS;
+    __shared__ __attribute__((aligned(128))) char lds[LDS];
+    const int jt = (g.J + B - 1) / B;
+    int ti, tj;
+    if (SYM) {   // number in the lower triangle, row by row
+        ti = (int)((sqrtf(8.0f * blockIdx.x + 1.0f) - 1.0f) * 0.5f);
+        while ((ti + 1) * (ti + 2) / 2 <= (int)blockIdx.x) ++ti;
+        while (ti * (ti + 1) / 2 > (int)blockIdx.x) --ti;
+        tj = blockIdx.x - ti * (ti + 1) / 2;
+    } else {
+        ti = blockIdx.x / jt;
+        tj = blockIdx.x % jt;
+    }
+    const int i0 = ti * B, j0 = tj * B;
+    const int Jp = (g.J + Iterate<F>::PAD - 1) / Iterate<F>::PAD * Iterate<F>::PAD, Ip = (g.I + Iterate<F>::PAD - 1) / Iterate<F>::PAD * Iterate<F>::PAD;
+    typename Tile::OpP p = {g.P + blockIdx.y * g.sp + (PKC ? i0 * g.ldp : i0 * (long)W), g.ldp, PKC ? min(g.I - i0, B) : min(Ip - i0, B) * WE, g.K};
+    typename Tile::OpQ q = {g.Q + blockIdx.y * g.sq + (QKC ? j0 * g.ldq : j0 * (long)W), g.ldq, QKC ? min(g.J - j0, B) : min(Jp - j0, B) * WE, g.K};
     Tile t;
     t.clear();
-    t.run_staged(lds, p, q, g.K);
-    const W c1 = (W)g.c1, c2 = (W)g.c2;
-    t.each([&](int i, int j, const W* v, auto) {
-        i += i0;
-        j += j0;
-        if (i >= g.I || j >= g.J) return;
-        const W e = g.c2 != 0.0 ? c2 * reinterpret_cast<const W*>(g.E + blockIdx.y * g.se + i * g.lde)[j] : W(0);
-        reinterpret_cast<O*>(g.D + blockIdx.y * g.sd + i * g.ldd)[j] = (O)(c1 * v[0] + e);
-    });
+    t.run_direct(lds, p, q, g.K);
+    const one c1 = (one)g.c1, c2 = (one)g.c2, c3 = (one)g.c3;
+    const char* E = g.E + blockIdx.y * g.se;
+    char* D = g.D + blockIdx.y * g.sd;
+    if constexpr (mm::Stored<F>::split) {
+        // Through LDS, one wave row of the tile at a time, so that planes are read and written in runs of 16 bytes, the mirrored
+        // tile too (single elements from the accumulators: 90 us for a 256 x 256 tile, most of it the mirrored stores).
+        float* slab = reinterpret_cast<float*>(lds);
+        constexpr int NT = WR * WC * 64, R = Tile::SLAB_ROWS, LD = Tile::SLAB_LD;
+        for (int pass = 0; pass < WR; ++pass) {
+            const int ib = i0 + pass * R;
+            __syncthreads();
+            t.to_slab(slab, pass);
+            __syncthreads();
+            for (int e = threadIdx.x; e < R * (B / 8); e += NT) {
+                const int i = ib + e / (B / 8), jl = e % (B / 8) * 8, j = j0 + jl;
+                if (i >= g.I || j >= Jp) continue;
+                float v[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) v[x] = c1 * slab[(i - ib) * LD + jl + x];
+                if (c2 != 0.0f) Iterate<F>::add8(E + i * g.lde, j, c2, v);
+                if (SYM && ti == tj) {
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) v[x] += j + x == i ? c3 : 0.0f;
+                }
+                if constexpr (LAST) {
+                    O* d = reinterpret_cast<O*>(D + i * g.ldd) + j;
+                    typedef O o8 __attribute__((ext_vector_type(8)));
+                    if (j + 8 <= g.J && reinterpret_cast<uintptr_t>(d) % 16 == 0) {
+                        o8 w;
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) w[x] = (O)v[x];
+                        *reinterpret_cast<o8*>(d) = w;
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            if (j + x < g.J) d[x] = (O)v[x];
+                    }
+                } else {
+                    Iterate<F>::store8(D + i * g.ldd, j, v);
+                }
+            }
+            if (SYM && ti != tj) {   // D(j, i): E is symmetric to the bit, so both triangles are
+                for (int e = threadIdx.x; e < B * (R / 8); e += NT) {
+                    const int jl = e / (R / 8), j = j0 + jl, il = e % (R / 8) * 8, i = ib + il;
+                    if (j >= g.J || i >= Ip) continue;
+                    float v[8];
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) v[x] = c1 * slab[(il + x) * LD + jl];
+                    if (c2 != 0.0f) Iterate<F>::add8(E + j * g.lde, i, c2, v);
+                    Iterate<F>::store8(D + j * g.ldd, i, v);
+                }
+            }
+        }
+    } else {
+        t.each([&](int i, int j, const one* v, auto) {
+            i += i0;
+            j += j0;
+            if (i >= g.I || j >= (LAST ? g.J : Jp)) return;
+            one d = c1 * v[0];
+            if (c2 != one(0) && j < g.J) d += c2 * Iterate<F>::load(E + i * g.lde, j);
+            if (SYM && i == j) d += c3;
+            if constexpr (LAST) {
+                reinterpret_cast<O*>(D + i * g.ldd)[j] = (O)d;
+            } else {
+                Iterate<F>::store(D + i * g.ldd, j, d);
+                if (SYM && ti != tj && j < g.J) Iterate<F>::store(D + j * g.ldd, i, d);
+            }
+        });
+        if (SYM && ti != tj && i0 + B >= g.I) {   // the zeros behind the rows that the mirrored tile ends
+            const int w = Ip - g.I;
+            for (int e = threadIdx.x; e < w * B; e += WR * WC * 64)
+                if (j0 + e / w < g.J) Iterate<F>::store(D + (j0 + e / w) * g.ldd, g.I + e % w, one(0));
+        }
+    }
 }
 
-struct OrthoWork {   // offsets in bytes
+struct OrthoWork {   // offsets and strides in bytes; rows of the iterates padded to whole blocks
     long part, x[2], a, b, total;
+    long ldx, sx, lda, sa;
 };
-OrthoWork ortho_work(int dtype, long batch, long rows, long cols) {
-    const long w = dtype == GPX_F64 ? 8 : 4, s = std::min(rows, cols);
+template <class F> OrthoWork ortho_work_of(long batch, int rows, int cols) {
+    const int s = std::min(rows, cols);
     auto up = [](long v) { return (v + 255) / 256 * 256; };
     OrthoWork o;
+    o.ldx = Iterate<F>::bytes(padded<F>(cols));
+    o.sx = o.ldx * rows;
+    o.lda = Iterate<F>::bytes(padded<F>(s));
+    o.sa = o.lda * s;
     o.part = 0;
     o.x[0] = up(batch * kParts * 8);
-    o.x[1] = o.x[0] + up(batch * rows * cols * w);
-    o.a = o.x[1] + up(batch * rows * cols * w);
-    o.b = o.a + up(batch * s * s * w);
-    o.total = o.b + up(batch * s * s * w);
+    o.x[1] = o.x[0] + up(batch * o.sx);
+    o.a = o.x[1] + up(batch * o.sx);
+    o.b = o.a + up(batch * o.sa);
+    o.total = o.b + up(batch * o.sa);
     return o;
 }
+OrthoWork ortho_work(int dtype, long batch, int rows, int cols) {
+    return dtype == GPX_F64 ? ortho_work_of<double>(batch, rows, cols) : ortho_work_of<mm::Split>(batch, rows, cols);
+}
 
-template <class W, class O, bool PKC, bool QKC> int launch(hipStream_t st, const OrthoArgs& g, int batch) {
-    const long tiles = ((g.I + 127L) / 128) * ((g.J + 127L) / 128);
-    ortho_mm_kernel<W, O, PKC, QKC><<<dim3((unsigned)tiles, (unsigned)batch), 256, 0, st>>>(g);
+// The tile of one product of split matrices, by the time it takes: rounds of workgroups over the 256 CUs, each of them K / 32
+// steps and an epilogue.  us per step and per epilogue, measured with S = 4096 and 1024 matrices: 256 (one workgroup of 8 waves
+// a CU) 2.3 / 20, 192 (one of 8) 1.65 / 10, 128 (two of 4; alone on its CU) 1.4 (0.85) / 8, 64 (two of 4, four LDS stages: a
+// grid that does not fill the chip waits for memory more than for the matrix cores) 0.55 (0.36) / 4.  Rounds decide: the 136
+// lower 256-tiles of a 4096 x 4096 Gram matrix take as long as all 256, its 253 lower 192-tiles 0.7 of that.
+enum TileChoice { TILE256, TILE192, TILE128, TILE64 };
+TileChoice choose_tile(bool sym, int I, int J, int K, int batch) {
+    struct { int b; double step, step_alone, rest; } t[4] = {{256, 2.3, 2.3, 20.0}, {192, 1.65, 1.65, 10.0}, {128, 1.4, 0.85, 8.0}, {64, 0.55, 0.36, 4.0}};
+    int best = 0;
+    double least = 1e300;
+    for (int c = 0; c < 4; ++c) {
+        const double it = (I + t[c].b - 1) / t[c].b, jt = (J + t[c].b - 1) / t[c].b;
+        const double tiles = (sym ? it * (it + 1) / 2 : it * jt) * batch, slots = t[c].b >= 192 ? 256.0 : 512.0;
+        const double step = tiles <= 256.0 ? t[c].step_alone : t[c].step;
+        const double cost = ceil(tiles / slots) * (step * ((K + 31) / 32) + t[c].rest);
+        if (cost < least) {
+            least = cost;
+            best = c;
+        }
+    }
+    return (TileChoice)best;
+}
+
+template <class F, class O, bool LAST, bool PKC, bool QKC, bool SYM> int launch(hipStream_t st, const OrthoArgs& g, int batch) {
+#define GO(B, R, C, S) go(std::integral_constant<int, B>{}, std::integral_constant<int, R>{}, std::integral_constant<int, C>{}, std::integral_constant<int, S>{})
+    auto go = [&](auto tile, auto wr, auto wc, auto stages) {
+        constexpr int B = decltype(tile)::value, WR = decltype(wr)::value, WC = decltype(wc)::value, ST = decltype(stages)::value;
+        const long it = (g.I + B - 1) / B, jt = (g.J + B - 1) / B;
+        const long tiles = SYM ? it * (it + 1) / 2 : it * jt;
+        ortho_mm_kernel<F, O, LAST, B, WR, WC, ST, PKC, QKC, SYM><<<dim3((unsigned)tiles, (unsigned)batch), WR * WC * 64, 0, st>>>(g);
+    };
+    if constexpr (mm::Stored<F>::split) {
+        const TileChoice c = choose_tile(SYM, g.I, g.J, g.K, batch);
+        if (c == TILE256) GO(256, 2, 4, 2);
+        else if (c == TILE192) GO(192, 2, 4, 2);
+        else if (c == TILE128) GO(128, 2, 2, 2);
+        else GO(64, 2, 2, 4);
+    } else GO(128, 2, 2, 2);
+#undef GO
     HIP_TRY(hipGetLastError());
     return GPX_OK;
 }
 
+// Largest |a s + b s^3 + c s^5| for 0 <= s <= top, a little above it: the ends and the zeros of the derivative
+double largest_value(double a, double b, double c, double top) {
+    auto p = [&](double s) { return fabs(s * (a + s * s * (b + c * s * s))); };
+    double most = p(top);
+    // a + 3 b u + 5 c u^2 = 0, u = s^2
+    double u[2] = {-1.0, -1.0};
+    if (c != 0.0) {
+        const double disc = 9.0 * b * b - 20.0 * a * c;
+        if (disc >= 0.0) {
+            u[0] = (-3.0 * b + sqrt(disc)) / (10.0 * c);
+            u[1] = (-3.0 * b - sqrt(disc)) / (10.0 * c);
+        }
+    } else if (b != 0.0) {
+        u[0] = -a / (3.0 * b);
+    }
+    for (double v : u)
+        if (v > 0.0 && v < top * top) most = std::max(most, p(sqrt(v)));
+    return most;
+}
+double largest_quadratic(double b, double c, double top) {   // largest |b u + c u^2|, 0 <= u <= top
+    double most = fabs(top * (b + c * top));
+    if (c != 0.0) {
+        const double u = -b / (2.0 * c);
+        if (u > 0.0 && u < top) most = std::max(most, fabs(u * (b + c * u)));
+    }
+    return most;
+}
+// the factors of every step's three products, powers of two of the split format included
+struct OrthoFactors { double start, gram[64], square[64], linear[64], unit[64], apply[64]; };
+int place(double bound);
+OrthoFactors ortho_factors(bool scaled, int steps, const double* coef) {
+    constexpr double slack = 1.01;   // rounding may carry a singular value past the bound of the exact iterate
+    OrthoFactors f;
+    double top = slack;              // of the singular values; |G|_F >= sigma_max
+    int ex = scaled ? place(top) : 0;
+    f.start = ldexp(1.0, ex);
+    for (int k = 0; k < steps; ++k) {
+        const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
+        top = std::max(top, 0x1p-400);
+        const double next = slack * largest_value(a, b, c, top);
+        const int ea = scaled ? place(slack * top * top) : 0;
+        const int eb = scaled ? place(slack * (fabs(a) + largest_quadratic(b, c, top * top))) : 0;
+        const int en = scaled && k + 1 < steps ? place(next) : 0;
+        f.gram[k] = ldexp(1.0, ea - 2 * ex);
+        f.square[k] = ldexp(c, eb - 2 * ea);
+        f.linear[k] = ldexp(b, eb - ea);
+        // a I goes into the square factor: its largest element is of the size of a anyway, and the product that follows
+        // reads X once instead of twice
+        f.unit[k] = ldexp(a, eb);
+        f.apply[k] = ldexp(1.0, en - ex - eb);
+        top = next;
+        ex = en;
+    }
+    return f;
+}
+// exponent of the power of two that places values of at most `bound` below 2^15
+int place(double bound) { return bound > 0.0 ? 14 - std::ilogb(bound) : 14; }
+
+// ---- small matrices: all steps in one workgroup -------------------------------------------------------------------------
+// X (short side S as rows, padded to 32; long side L padded to 32) and A stay in LDS in the split format, rows 32 bytes longer
+// than their values so that neighbouring rows do not share banks.  Per step: A = X X^T, one 16 x 16 tile per wave and turn;
+// A <- a I + b A + c A A from registers once every wave has read A; X <- A X by blocks of 16 columns, each read whole into
+// registers by the one wave that overwrites it.  What bounds it is latency: 15 short products behind barriers.
+constexpr int kSmallWaves = 16, kSmallSide = 128, kSmallLds = 160 * 1024 - 512;
+struct OrthoSmallArgs {
+    long ldg, stride_g, ldo, stride_o;   // elements
+    int rows, cols, steps;
+    double eps, scale;
+    float gram[64], square[64], linear[64], unit[64], apply[64];   // factors of every step, powers of two included
+};
+constexpr int small_row(int values) { return values * 4 + 32; }
+long small_lds(int rows, int cols) {
+    const int s = (std::min(rows, cols) + 31) / 32 * 32, l = (std::max(rows, cols) + 31) / 32 * 32;
+    return s <= kSmallSide && l <= (1 << 16) ? (long)s * (small_row(l) + small_row(s)) + (s == 32 ? kSmallWaves * 3 * 1024 : 0) : 1L << 40;
+}
+__device__ __forceinline__ mm::v4i small_frag_kc(const char* m, int ld, int row0, int k32, int lo, int lane) {
+    return *reinterpret_cast<const mm::v4i*>(m + (row0 + (lane & 15)) * ld + k32 * 128 + lo * 64 + (lane >> 4) * 16);
+}
+__device__ __forceinline__ mm::v4i small_frag_strided(const char* m, int ld, int col0, int k32, int lo, int lane) {
+    const int r = lane & 15, q = lane >> 4;
+    const char* p = m + (k32 * 32 + 8 * q + (r >> 2)) * ld + (col0 >> 5) * 128 + (col0 & 16) * 2 + lo * 64 + (r & 3) * 8;
+    typedef __attribute__((address_space(3))) mm::v4s lds4;
+    union { mm::v4s h[2]; mm::v4i v; } u;
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * ld));
+    return u.v;
+}
+// the three products of the split format in accumulators of their own: no matrix instruction waits for the one before it
+struct SmallAcc {
+    mm::v4f a = {}, b = {}, c = {};
+    __device__ __forceinline__ void add(mm::v4i qh, mm::v4i ql, mm::v4i ph, mm::v4i pl) {
+        a = mm::mma<_Float16>(ql, ph, a);
+        b = mm::mma<_Float16>(qh, pl, b);
+        c = mm::mma<_Float16>(qh, ph, c);
+    }
+    __device__ __forceinline__ mm::v4f sum() const { return (a + b) + c; }
+};
+__device__ __forceinline__ void small_store4(char* row, int j, mm::v4f v) {   // j a multiple of 4
+    typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+    v4h h, l;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        h[x] = (_Float16)v[x];
+        l[x] = (_Float16)(v[x] - (float)h[x]);
+    }
+    char* p = row + (j >> 5) * 128 + (j & 31) * 2;
+    *reinterpret_cast<v4h*>(p) = h;
+    *reinterpret_cast<v4h*>(p + 64) = l;
+}
+
+template <class T, int NB>   // NB: blocks of 32 of the short side
+__global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* G, T* O, const OrthoSmallArgs g) {
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    __shared__ double ws[kSmallWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+    const bool tall = g.rows > g.cols;
+    const int S = tall ? g.cols : g.rows, L = tall ? g.rows : g.cols;
+    constexpr int Sp = NB * 32, NT = NB * 2, TILES = NT * (NT + 1) / 2, TURNS = (TILES + kSmallWaves - 1) / kSmallWaves;
+    const int Lp = (L + 31) / 32 * 32;
+    const int ldx = small_row(Lp), lda = small_row(Sp);
+    char* X = lds;
+    char* A = lds + (long)Sp * ldx;
+    G += blockIdx.x * g.stride_g;
+    O += blockIdx.x * g.stride_o;
+    double s = 0.0;
+    each_run(g.rows, g.cols, threadIdx.x, kSmallWaves * 64, [&](int row, int c) {
+        T v[8];
+        load_run(G + row * g.ldg + c, g.cols - c, v);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) s = fma(as_double(v[x]), as_double(v[x]), s);
+    });
+#pragma unroll
+    for (int d = 32; d; d /= 2) s += __shfl_xor(s, d, 64);
+    if (lane == 0) ws[wave] = s;
+    for (int e = threadIdx.x; e < Sp * ldx / 16; e += kSmallWaves * 64) reinterpret_cast<mm::v4i*>(X)[e] = mm::v4i{0, 0, 0, 0};
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int w = 0; w < kSmallWaves; ++w) s += ws[w];
+    const double by = g.scale / (sqrt(s) + g.eps);
+    each_run(g.rows, g.cols, threadIdx.x, kSmallWaves * 64, [&](int row, int c) {
+        T v[8];
+        load_run(G + row * g.ldg + c, g.cols - c, v);
+        if (tall) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+                if (c + x < g.cols) Iterate<mm::Split>::store(X + (c + x) * ldx, row, (float)(as_double(v[x]) * by));
+        } else {
+            float w[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) w[x] = (float)(as_double(v[x]) * by);
+            Iterate<mm::Split>::store8(X + row * ldx, c, w);
+        }
+    });
+    __syncthreads();
+    const int kx = Lp / 32;
+    // this wave's tiles of the lower triangle
+    int ti[TURNS], tj[TURNS];
+#pragma unroll
+    for (int x = 0; x < TURNS; ++x) {
+        int t = wave + kSmallWaves * x, i = 0;
+        while (t > i) t -= ++i;
+        ti[x] = i * 16;
+        tj[x] = t * 16;
+    }
+    auto store_both = [&](int i0, int j0, mm::v4f c) {
+        small_store4(A + (i0 + r) * lda, j0 + 4 * q, c);
+        if (i0 != j0) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y) Iterate<mm::Split>::store(A + (j0 + 4 * q + y) * lda, i0 + r, c[y]);
+        }
+    };
+    for (int step = 0; step < g.steps; ++step) {
+        if constexpr (NB == 1) {
+            // three tiles: every wave takes each sixteenth block of k for all of them, the sums meet in LDS behind A
+            mm::v4f* meet = reinterpret_cast<mm::v4f*>(A + Sp * lda);
+            SmallAcc c[3];
+            for (int k = wave; k < kx; k += kSmallWaves) {
+                mm::v4i f[2][2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int lo = 0; lo < 2; ++lo) f[h][lo] = small_frag_kc(X, ldx, 16 * h, k, lo, lane);
+                c[0].add(f[0][0], f[0][1], f[0][0], f[0][1]);
+                c[1].add(f[0][0], f[0][1], f[1][0], f[1][1]);
+                c[2].add(f[1][0], f[1][1], f[1][0], f[1][1]);
+            }
+#pragma unroll
+            for (int x = 0; x < 3; ++x) meet[(wave * 3 + x) * 64 + lane] = c[x].sum();
+            __syncthreads();
+            if (wave < 3) {
+                mm::v4f c = meet[wave * 64 + lane];
+#pragma unroll
+                for (int w = 1; w < kSmallWaves; ++w) c += meet[(w * 3 + wave) * 64 + lane];
+                store_both(ti[0], tj[0], c * g.gram[step]);
+            }
+        } else {
+#pragma unroll
+            for (int x = 0; x < TURNS; ++x) {
+                if (wave + kSmallWaves * x >= TILES) break;
+                SmallAcc c;
+#pragma unroll 4
+                for (int k = 0; k < kx; ++k)
+                    c.add(small_frag_kc(X, ldx, tj[x], k, 0, lane), small_frag_kc(X, ldx, tj[x], k, 1, lane), small_frag_kc(X, ldx, ti[x], k, 0, lane),
+                          small_frag_kc(X, ldx, ti[x], k, 1, lane));
+                store_both(ti[x], tj[x], c.sum() * g.gram[step]);
+            }
+        }
+        __syncthreads();
+        mm::v4f b[TURNS];
+#pragma unroll
+        for (int x = 0; x < TURNS; ++x) {
+            if (wave + kSmallWaves * x >= TILES) break;
+            SmallAcc c;
+#pragma unroll
+            for (int k = 0; k < NB; ++k)
+                c.add(small_frag_kc(A, lda, tj[x], k, 0, lane), small_frag_kc(A, lda, tj[x], k, 1, lane), small_frag_kc(A, lda, ti[x], k, 0, lane),
+                      small_frag_kc(A, lda, ti[x], k, 1, lane));
+            b[x] = c.sum();
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const float a = Iterate<mm::Split>::load(A + (ti[x] + r) * lda, tj[x] + 4 * q + y);
+                b[x][y] = g.square[step] * b[x][y] + g.linear[step] * a + (ti[x] + r == tj[x] + 4 * q + y ? g.unit[step] : 0.0f);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < TURNS; ++x) {
+            if (wave + kSmallWaves * x >= TILES) break;
+            store_both(ti[x], tj[x], b[x]);
+        }
+        __syncthreads();
+        const bool last = step + 1 == g.steps;
+        mm::v4i next[NB][2];   // the block of the next turn is read while this one is multiplied
+        auto read_block = [&](int j0) {
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                next[k][0] = small_frag_strided(X, ldx, j0, k, 0, lane);
+                next[k][1] = small_frag_strided(X, ldx, j0, k, 1, lane);
+            }
+        };
+        if (wave * 16 < Lp) read_block(wave * 16);
+        for (int j0 = wave * 16; j0 < Lp; j0 += kSmallWaves * 16) {
+            mm::v4i qf[NB][2];
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                qf[k][0] = next[k][0];
+                qf[k][1] = next[k][1];
+            }
+            if (j0 + kSmallWaves * 16 < Lp) read_block(j0 + kSmallWaves * 16);
+#pragma unroll 2
+            for (int i0 = 0; i0 < Sp; i0 += 16) {
+                SmallAcc acc;
+#pragma unroll
+                for (int k = 0; k < NB; ++k)
+                    acc.add(qf[k][0], qf[k][1], small_frag_kc(A, lda, i0, k, 0, lane), small_frag_kc(A, lda, i0, k, 1, lane));
+                mm::v4f c = acc.sum();
+                c *= g.apply[step];
+                if (last) {
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const int i = i0 + r, j = j0 + 4 * q + y;
+                        if (i < S && j < L) O[tall ? j * g.ldo + i : i * g.ldo + j] = (T)c[y];
+                    }
+                } else {
+                    small_store4(X + (i0 + r) * ldx, j0 + 4 * q, c);
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
 // rows x cols row-major (the column-major cols x rows of the C interface)
-template <class T, class W>
-int ortho_typed(hipStream_t st, int dtype, int batch, int rows, int cols, const T* G, long ldg, long stride_g, int steps, const double* coef,
-                double eps, T* O, long ldo, long stride_o, char* work) {
-    const OrthoWork o = ortho_work(dtype, batch, rows, cols);
+template <class T, class F>
+int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long ldg, long stride_g, int steps, const double* coef, double eps,
+                T* O, long ldo, long stride_o, char* work) {
+    const OrthoFactors f = ortho_factors(mm::Stored<F>::split, steps, coef);
+    if constexpr (mm::Stored<F>::split) {
+        const long bytes = small_lds(rows, cols);
+        if (steps > 0 && bytes <= kSmallLds) {
+            OrthoSmallArgs g = {ldg, stride_g, ldo, stride_o, rows, cols, steps, eps, f.start, {}, {}, {}, {}, {}};
+            for (int k = 0; k < steps; ++k) {
+                g.gram[k] = (float)f.gram[k];
+                g.square[k] = (float)f.square[k];
+                g.linear[k] = (float)f.linear[k];
+                g.unit[k] = (float)f.unit[k];
+                g.apply[k] = (float)f.apply[k];
+            }
+            const int nb = (std::min(rows, cols) + 31) / 32;
+            if (nb == 1) ortho_small_kernel<T, 1><<<batch, kSmallWaves * 64, (unsigned)bytes, st>>>(G, O, g);
+            else if (nb == 2) ortho_small_kernel<T, 2><<<batch, kSmallWaves * 64, (unsigned)bytes, st>>>(G, O, g);
+            else if (nb == 3) ortho_small_kernel<T, 3><<<batch, kSmallWaves * 64, (unsigned)bytes, st>>>(G, O, g);
+            else ortho_small_kernel<T, 4><<<batch, kSmallWaves * 64, (unsigned)bytes, st>>>(G, O, g);
+            HIP_TRY(hipGetLastError());
+            return GPX_OK;
+        }
+    }
+    const OrthoWork o = ortho_work_of<F>(batch, rows, cols);
     double* part = reinterpret_cast<double*>(work + o.part);
-    ortho_norm_kernel<T><<<dim3(kParts, batch), 256, 0, st>>>(G, ldg, stride_g, rows, cols, part);
+    const long runs = (long)rows * ((padded<F>(cols) + 7) / 8);
+    const int parts = (int)std::min<long>((runs + 511) / 512, kParts);
+    ortho_norm_kernel<T><<<dim3(parts, batch), 256, 0, st>>>(G, ldg, stride_g, rows, cols, part);
     HIP_TRY(hipGetLastError());
-    const long total = (long)rows * cols;
-    const dim3 grid((unsigned)std::min<long>((total + 1023) / 1024, 2048), (unsigned)batch);
+    const dim3 grid((unsigned)std::min<long>((runs + 255) / 256, 2048), (unsigned)batch);
     if (steps == 0) {
-        ortho_scale_kernel<T, T><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, part, eps, O, ldo, stride_o);
+        ortho_normalize_kernel<T><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, part, parts, eps, O, ldo, stride_o);
         HIP_TRY(hipGetLastError());
         return GPX_OK;
     }
     char* x[2] = {work + o.x[0], work + o.x[1]};
     char *a = work + o.a, *b = work + o.b;
-    ortho_scale_kernel<T, W><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, part, eps, reinterpret_cast<W*>(x[0]), cols, total);
+    ortho_scale_kernel<T, F><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, padded<F>(cols), part, parts, eps, f.start, x[0], o.ldx, o.sx);
     HIP_TRY(hipGetLastError());
     const bool tall = rows > cols;
     const int s = std::min(rows, cols), l = std::max(rows, cols);
-    const long w = sizeof(W), ldx = cols * w, sx = total * w, lda = s * w, sa = (long)s * s * w;
     for (int k = 0; k < steps; ++k) {
-        const double ca = coef[3 * k], cb = coef[3 * k + 1], cc = coef[3 * k + 2];
         char *from = x[k & 1], *to = x[~k & 1];
-        OrthoArgs gram = {from, from, nullptr, a, ldx, ldx, 0, lda, sx, sx, 0, sa, s, s, l, 1.0, 0.0};
-        int rc = tall ? launch<W, W, false, false>(st, gram, batch) : launch<W, W, true, true>(st, gram, batch);
+        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, s, s, l, f.gram[k], 0.0, 0.0};
+        int rc = tall ? launch<F, F, false, false, false, true>(st, gram, batch) : launch<F, F, false, true, true, true>(st, gram, batch);
         if (rc) return rc;
-        OrthoArgs poly = {a, a, a, b, lda, lda, lda, lda, sa, sa, sa, sa, s, s, s, cc, cb};
-        if ((rc = launch<W, W, true, true>(st, poly, batch))) return rc;
+        const OrthoArgs poly = {a, a, a, b, o.lda, o.lda, o.lda, o.lda, o.sa, o.sa, o.sa, o.sa, s, s, s,
+                                f.square[k], f.linear[k], f.unit[k]};
+        if ((rc = launch<F, F, false, true, true, true>(st, poly, batch))) return rc;
         const bool last = k + 1 == steps;
-        const long ldd = last ? ldo * (long)sizeof(T) : ldx, sd = last ? stride_o * (long)sizeof(T) : sx;
+        const long ldd = last ? ldo * (long)sizeof(T) : o.ldx, sd = last ? stride_o * (long)sizeof(T) : o.sx;
         char* d = last ? reinterpret_cast<char*>(O) : to;
-        OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, ldx, lda, ldx, ldd, sx, sa, sx, sd, rows, cols, s, 1.0, ca}
-                               : OrthoArgs{b, from, from, d, lda, ldx, ldx, ldd, sa, sx, sx, sd, rows, cols, s, 1.0, ca};
-        if (tall) rc = last ? launch<W, T, true, true>(st, apply, batch) : launch<W, W, true, true>(st, apply, batch);
-        else rc = last ? launch<W, T, true, false>(st, apply, batch) : launch<W, W, true, false>(st, apply, batch);
+        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, rows, cols, s, f.apply[k], 0.0, 0.0}
+                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, rows, cols, s, f.apply[k], 0.0, 0.0};
+        if (tall) rc = last ? launch<F, T, true, true, true, false>(st, apply, batch) : launch<F, F, false, true, true, false>(st, apply, batch);
+        else rc = last ? launch<F, T, true, true, false, false>(st, apply, batch) : launch<F, F, false, true, false, false>(st, apply, batch);
         if (rc) return rc;
     }
     return GPX_OK;
@@ -153,7 +687,7 @@ bool sizes_ok(int dtype, int64_t batch, int64_t M, int64_t N) {
 
 extern "C" int gpx_orthogonalize_work(int dtype, int64_t batch, int64_t M, int64_t N, int64_t* work_bytes) {
     if (!work_bytes || !sizes_ok(dtype, batch, M, N)) return GPX_ERR_ARG;
-    *work_bytes = batch && M && N ? ortho_work(dtype, batch, N, M).total : 0;
+    *work_bytes = batch && M && N ? ortho_work(dtype, batch, (int)N, (int)M).total : 0;
     return GPX_OK;
 }
 
@@ -167,7 +701,7 @@ extern "C" int gpx_orthogonalize(int dtype, int64_t batch, int64_t M, int64_t N,
     if (!G || !O || !work) return GPX_ERR_ARG;
     const uintptr_t e = dtype == GPX_F64 ? 8 : dtype == GPX_F32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(G) % e || reinterpret_cast<uintptr_t>(O) % e || reinterpret_cast<uintptr_t>(work) % 16) return GPX_ERR_ARG;
-    if (work_bytes < ortho_work(dtype, batch, N, M).total) return GPX_ERR_ARG;
+    if (work_bytes < ortho_work(dtype, batch, (int)N, (int)M).total) return GPX_ERR_ARG;
     double table[3 * kMaxSteps];
     for (int k = 0; k < steps; ++k)
         for (int c = 0; c < 3; ++c) {
@@ -181,16 +715,16 @@ extern "C" int gpx_orthogonalize(int dtype, int64_t batch, int64_t M, int64_t N,
     const int b = (int)batch, r = (int)N, c = (int)M;
     switch (dtype) {
         case GPX_F64:
-            return ortho_typed<double, double>(st, dtype, b, r, c, static_cast<const double*>(G), ldg, stride_g, steps, table, eps,
+            return ortho_typed<double, double>(st, b, r, c, static_cast<const double*>(G), ldg, stride_g, steps, table, eps,
                                                static_cast<double*>(O), ldo, stride_o, w);
         case GPX_F32:
-            return ortho_typed<float, float>(st, dtype, b, r, c, static_cast<const float*>(G), ldg, stride_g, steps, table, eps,
+            return ortho_typed<float, mm::Split>(st, b, r, c, static_cast<const float*>(G), ldg, stride_g, steps, table, eps,
                                              static_cast<float*>(O), ldo, stride_o, w);
         case GPX_BF16:
-            return ortho_typed<__bf16, float>(st, dtype, b, r, c, static_cast<const __bf16*>(G), ldg, stride_g, steps, table, eps,
+            return ortho_typed<__bf16, mm::Split>(st, b, r, c, static_cast<const __bf16*>(G), ldg, stride_g, steps, table, eps,
                                               static_cast<__bf16*>(O), ldo, stride_o, w);
         default:
-            return ortho_typed<_Float16, float>(st, dtype, b, r, c, static_cast<const _Float16*>(G), ldg, stride_g, steps, table, eps,
+            return ortho_typed<_Float16, mm::Split>(st, b, r, c, static_cast<const _Float16*>(G), ldg, stride_g, steps, table, eps,
                                                 static_cast<_Float16*>(O), ldo, stride_o, w);
     }
 }
