@@ -7,13 +7,13 @@
 //
 // The offsets live on the device: the host never waits for them.  Every kernel clamps them to [0, T] and reads a
 // decreasing pair as an empty group, so no value of theirs leads outside the buffers.
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include "mm_tile.h"
 #include "../../include/gpx.h"
 
 namespace {
-
-using mm::v4f;
 
 struct GroupedArgs {
     const char* X; const char* W; char* Y;
@@ -22,7 +22,7 @@ struct GroupedArgs {
     long T;
     int groups, N, K;
     double alpha, beta;
-    int vec;   // Y's rows allow 4-element stores
+    int vec;   // Y's rows allow 16-byte stores
 };
 
 __device__ __forceinline__ long clamped(const int64_t* offsets, int g, long T) {
@@ -32,89 +32,131 @@ __device__ __forceinline__ long clamped(const int64_t* offsets, int g, long T) {
 
 struct RowTile { int group, rows; long row0; };   // rows of this tile; group < 0: no tile
 
-// The tile number `t` in the order of the groups, ceil(rows / BM) tiles each.  One wave looks at 64 groups at a time: the
-// tile counts, their running sum over the lanes, and the first lane whose sum passes t.
-template <int BM> __device__ RowTile find_row_tile(const int64_t* offsets, int groups, long T, long t) {
-    const int lane = threadIdx.x & 63;
-    RowTile out = {-1, 0, 0};
-    long before = 0;
-    for (int g0 = 0; g0 < groups; g0 += 64) {
-        const int g = g0 + lane;
-        long lo = 0, rows = 0;
+// One wave looks at 64 groups at a time: rows of group g0 + lane, in tiles of `unit` rows, and the running sum of the tiles.
+struct GroupScan {
+    long lo, rows, tiles, sum;
+    __device__ GroupScan(const int64_t* offsets, int groups, long T, int g0, unsigned unit) {
+        const int lane = threadIdx.x & 63, g = g0 + lane;
+        lo = rows = 0;
         if (g < groups) {
             lo = clamped(offsets, g, T);
             const long hi = clamped(offsets, g + 1, T);
             rows = hi > lo ? hi - lo : 0;
         }
-        const long tiles = (rows + BM - 1) / BM;
-        long sum = tiles;
+        sum = tiles = ((unsigned)rows + unit - 1) / unit;   // T < 2^31
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const long up = __shfl_up(sum, d, 64);
             if (lane >= d) sum += up;
         }
-        const unsigned long long past = __ballot(before + sum > t);
+    }
+};
+
+// row tile number t in the order of the groups; `first`: the scan of the first 64
+__device__ RowTile row_tile(const GroupScan& first, const int64_t* offsets, int groups, long T, long t, unsigned unit) {
+    long before = 0;
+    for (int g0 = 0; g0 < groups; g0 += 64) {
+        const GroupScan s = g0 ? GroupScan(offsets, groups, T, g0, unit) : first;
+        const unsigned long long past = __ballot(before + s.sum > t);
         if (past) {
             const int src = __builtin_ctzll(past);
-            const long mine = t - (before + sum - tiles);   // tile within the group
-            out.group = g0 + src;
-            const long m = __shfl(mine, src, 64);
-            const long r = __shfl(rows, src, 64) - m * BM;
-            out.rows = (int)(r < BM ? r : BM);
-            out.row0 = __shfl(lo, src, 64) + m * BM;
-            break;
+            const long m = t - before - __shfl(s.sum - s.tiles, src, 64);   // tile within the group
+            const long r = __shfl(s.rows, src, 64) - m * unit;
+            RowTile out;
+            out.group = __builtin_amdgcn_readfirstlane(g0 + src);
+            out.rows = __builtin_amdgcn_readfirstlane((int)(r < unit ? r : unit));
+            out.row0 = __shfl(s.lo, src, 64) + m * unit;
+            return out;
         }
-        before += __shfl(sum, 63, 64);
+        before += __shfl(s.sum, 63, 64);
     }
-    out.group = __builtin_amdgcn_readfirstlane(out.group);
-    out.rows = __builtin_amdgcn_readfirstlane(out.rows);
-    return out;
+    return {-1, 0, 0};
 }
 
-template <class O, class A, int CNT>
-__device__ __forceinline__ void put(char* row, int j, int N, const A* v, A alpha, A beta, bool vec) {
+// The order of the tiles: row tiles in the order of the groups, ceil(rows / BM) each, cut into bands of eight; a band's tiles
+// column by column.  That order is walked in chunks of CHUNK tiles, what the chip holds at a time, and since workgroups go
+// round the 8 XCDs, XCD x takes the x-th eighth of every chunk: its CUs share 8 row panels and a few column panels in their L2,
+// and all XCDs stay in one neighbourhood of X and W in the cache behind them.
+template <int BM, int CHUNK> __device__ RowTile find_tile(const int64_t* offsets, int groups, long T, int nt, int& col) {
+    const GroupScan first(offsets, groups, T, 0, BM);
+    long total = __shfl(first.sum, 63, 64);
+    for (int g0 = 64; g0 < groups; g0 += 64) total += __shfl(GroupScan(offsets, groups, T, g0, BM).sum, 63, 64);
+    const long all = total * nt;
+    const long start = (long)(blockIdx.x / CHUNK) * CHUNK;
+    const unsigned here = (unsigned)min((long)CHUNK, all - start), xcd = blockIdx.x & 7;
+    if (start >= all) return {-1, 0, 0};
+    const unsigned in_chunk = here * xcd / 8 + (blockIdx.x % CHUNK >> 3);
+    if (in_chunk >= here * (xcd + 1) / 8) return {-1, 0, 0};
+    constexpr int HIGH = 8;
+    const long o = start + in_chunk;
+    const unsigned band = (unsigned)(o / (HIGH * nt)), in = (unsigned)(o - (long)band * HIGH * nt);
+    const unsigned high = (unsigned)min((long)HIGH, total - (long)HIGH * band);
+    col = __builtin_amdgcn_readfirstlane((int)(in / high));
+    return row_tile(first, offsets, groups, T, (long)HIGH * band + in % high, BM);
+}
+
+// p[0..7] (those j + x < N) = alpha v + beta p in the type O; vec: the row allows 16-byte stores from multiples of 8 on
+template <class O> __device__ __forceinline__ void put8(char* row, int j, int N, const float (&v)[8], float alpha, float beta, bool vec) {
     O* p = reinterpret_cast<O*>(row) + j;
-    if (CNT == 4 && vec && j + 4 <= N) {
-        union { O e[4]; int w[sizeof(O)]; } u;
-        typedef int words __attribute__((ext_vector_type(sizeof(O) == 8 ? 4 : sizeof(O))));
-        if (beta != A(0)) {
+    union { O e[8]; mm::v4i w[sizeof(O) / 2]; } u;
+    const bool whole = vec && j + 8 <= N;
+    if (beta != 0.0f) {
+        if (whole) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) u.e[x] = (O)(alpha * v[x] + beta * (A)p[x]);
+            for (int x = 0; x < (int)sizeof(O) / 2; ++x) u.w[x] = reinterpret_cast<const mm::v4i*>(p)[x];
         } else {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) u.e[x] = (O)(alpha * v[x]);
+            for (int x = 0; x < 8; ++x) u.e[x] = j + x < N ? p[x] : (O)0.0f;
         }
-        words w;
 #pragma unroll
-        for (int x = 0; x < (int)sizeof(O); ++x) w[x] = u.w[x];
-        *reinterpret_cast<words*>(p) = w;
-        return;
+        for (int x = 0; x < 8; ++x) u.e[x] = (O)(alpha * v[x] + beta * (float)u.e[x]);
+    } else {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) u.e[x] = (O)(alpha * v[x]);
     }
+    if (whole) {
 #pragma unroll
-    for (int x = 0; x < CNT; ++x)
-        if (j + x < N) p[x] = (O)(beta != A(0) ? alpha * v[x] + beta * (A)p[x] : alpha * v[x]);
+        for (int x = 0; x < (int)sizeof(O) / 2; ++x) reinterpret_cast<mm::v4i*>(p)[x] = u.w[x];
+    } else {
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            if (j + x < N) p[x] = u.e[x];
+    }
 }
 
-template <class T, int BM, int BN, int WR, int WC, bool WKC, bool DIRECT>
-__global__ __launch_bounds__(WR * WC * 64, 2) void grouped_kernel(const GroupedArgs g) {
-    typedef mm::Tile<T, BM, BN, WR, WC, true, WKC> Tile;
+// the tile's result: rows x cols of it at `row0`, `ld` bytes apart
+template <class O, class Tile>
+__device__ __forceinline__ void store_tile(Tile& t, char* lds, char* row0, long ld, int rows, int cols, double alpha, double beta, bool vec) {
     typedef typename Tile::one A;
-    __shared__ __attribute__((aligned(128))) char lds[Tile::LDS];
-    const int nt = (g.N + BN - 1) / BN;
-    const RowTile rt = find_row_tile<BM>(g.offsets, g.groups, g.T, blockIdx.x / nt);
+    const A al = (A)alpha, be = (A)beta;
+    if constexpr (Tile::SWAP) {   // 16 neighbouring lanes store 16 neighbouring columns
+        t.each([&](int i, int j, const A* v, auto) {
+            if (i >= rows || j >= cols) return;
+            O* p = reinterpret_cast<O*>(row0 + i * ld) + j;
+            *p = (O)(be != A(0) ? al * v[0] + be * (A)*p : al * v[0]);
+        });
+    } else {
+        t.each_run(lds, rows, cols, [&](int i, int j, const float (&v)[8]) { put8<O>(row0 + i * ld, j, cols, v, al, be, vec); });
+    }
+}
+
+template <class Tile> constexpr int tile_lds() { return Tile::SWAP || Tile::LDS > Tile::SLAB ? Tile::LDS : Tile::SLAB; }
+
+template <class T, int BM, int BN, int WR, int WC, int ST, bool WKC, bool DIRECT>
+__global__ __launch_bounds__(WR * WC * 64, 2) void grouped_kernel(const GroupedArgs g) {
+    typedef mm::Tile<T, BM, BN, WR, WC, true, WKC, ST> Tile;
+    __shared__ __attribute__((aligned(128))) char lds[tile_lds<Tile>()];
+    int col = 0;
+    const RowTile rt = find_tile<BM, (BM * BN > 128 * 128 ? 256 : 512)>(g.offsets, g.groups, g.T, (g.N + BN - 1) / BN, col);
     if (rt.group < 0) return;
-    const int n0 = (int)(blockIdx.x % nt) * BN;
+    const int n0 = col * BN, cols = min(g.N - n0, BN);
     typename Tile::OpP p = {g.X + rt.row0 * g.ldx, g.ldx, rt.rows, g.K};
-    typename Tile::OpQ q = {g.W + rt.group * g.stride_w + (WKC ? n0 * g.ldw : n0 * (long)sizeof(T)), g.ldw, min(g.N - n0, BN), g.K};
+    typename Tile::OpQ q = {g.W + rt.group * g.stride_w + (WKC ? n0 * g.ldw : n0 * (long)sizeof(T)), g.ldw, cols, g.K};
     Tile t;
     t.clear();
     if (DIRECT) t.run_direct(lds, p, q, g.K);
     else t.run_staged(lds, p, q, g.K);
-    char* y = g.Y + rt.row0 * g.ldy;
-    const A alpha = (A)g.alpha, beta = (A)g.beta;
-    t.each([&](int i, int j, const A* v, auto cnt) {
-        if (i < rt.rows) put<T, A, decltype(cnt)::value>(y + i * g.ldy, n0 + j, g.N, v, alpha, beta, g.vec);
-    });
+    store_tile<T>(t, lds, g.Y + rt.row0 * g.ldy + n0 * (long)sizeof(T), g.ldy, rt.rows, cols, g.alpha, g.beta, g.vec);
 }
 
 struct GroupedDwArgs {
@@ -123,85 +165,215 @@ struct GroupedDwArgs {
     long ldx, ldz, ldc, stride_c;   // bytes
     long T;
     int M, N;   // columns of X (contiguous in C) and of Z
+    int groups;
     double alpha, beta;
     int vec;
+    char* slabs;     // SPLIT: the sum over every part of `part_rows` rows, N x M each, in the accumulators' type
+    int part_rows, parts;
 };
+
+// SPLIT: few tiles and many rows.  The rows of every group are cut into parts, a workgroup sums one part into a slab of its own,
+// and grouped_dw_join_kernel adds the slabs of a group in their order: the same bits in every run.
+template <class T, class O, int B, int WR, int WC, int ST, bool DIRECT, bool SPLIT>
+__global__ __launch_bounds__(WR * WC * 64, 2) void grouped_dw_kernel(const GroupedDwArgs g) {
+    typedef mm::Tile<T, B, B, WR, WC, false, false, ST> Tile;
+    typedef typename Tile::one A;
+    __shared__ __attribute__((aligned(128))) char lds[tile_lds<Tile>()];
+    const int mt = (g.M + B - 1) / B;
+    const int n0 = (int)(blockIdx.x / mt) * B, m0 = (int)(blockIdx.x % mt) * B;
+    long lo;
+    int rows;
+    if (SPLIT) {
+        const RowTile part = row_tile(GroupScan(g.offsets, g.groups, g.T, 0, g.part_rows), g.offsets, g.groups, g.T, blockIdx.y, g.part_rows);
+        if (part.group < 0) return;
+        lo = part.row0;
+        rows = part.rows;
+    } else {
+        lo = clamped(g.offsets, blockIdx.y, g.T);
+        const long hi = clamped(g.offsets, blockIdx.y + 1, g.T);
+        rows = (int)(hi > lo ? hi - lo : 0);
+    }
+    typename Tile::OpP p = {g.Z + lo * g.ldz + n0 * (long)sizeof(T), g.ldz, min(g.N - n0, B), rows};
+    typename Tile::OpQ q = {g.X + lo * g.ldx + m0 * (long)sizeof(T), g.ldx, min(g.M - m0, B), rows};
+    Tile t;
+    t.clear();
+    if (DIRECT) t.run_direct(lds, p, q, rows);
+    else t.run_staged(lds, p, q, rows);
+    if (SPLIT) {
+        const long ld = (long)g.M * sizeof(A);
+        store_tile<A>(t, lds, g.slabs + (blockIdx.y * (long)g.N + n0) * ld + m0 * (long)sizeof(A), ld, p.rows, q.rows, 1.0, 0.0, g.M % 4 == 0);
+    } else {
+        store_tile<O>(t, lds, g.C + blockIdx.y * g.stride_c + n0 * g.ldc + m0 * (long)sizeof(O), g.ldc, p.rows, q.rows, g.alpha, g.beta, g.vec);
+    }
+}
+
+template <class A, class O>
+__global__ __launch_bounds__(256) void grouped_dw_join_kernel(const GroupedDwArgs g) {
+    const int group = blockIdx.y;
+    // parts before this group and in it
+    long first = 0, mine = 0;
+    for (int g0 = 0; g0 <= group; g0 += 64) {
+        const GroupScan s(g.offsets, g.groups, g.T, g0, g.part_rows);
+        const int last = min(group - g0, 63);
+        first += __shfl(s.sum - (g0 + 63 >= group ? s.tiles : 0), last, 64);
+        mine = __shfl(s.tiles, last, 64);
+    }
+    mine = min(mine, max(0L, g.parts - first));   // a wrong table may name more parts than there are slabs
+    const long size = (long)g.N * g.M;
+    const A* slab = reinterpret_cast<const A*>(g.slabs) + first * size;
+    const A al = (A)g.alpha, be = (A)g.beta;
+    for (long e = blockIdx.x * 256L + threadIdx.x; e < size; e += gridDim.x * 256L) {
+        A s = A(0);
+        for (long part = 0; part < mine; ++part) s += slab[part * size + e];
+        O* c = reinterpret_cast<O*>(g.C + group * g.stride_c + e / g.M * g.ldc) + e % g.M;
+        *c = (O)(be != A(0) ? al * s + be * (A)*c : al * s);
+    }
+}
 
 // rows in whole, aligned 16-byte chunks: what a direct-to-LDS load needs
 bool whole_chunks(const void* p, long ld_bytes, long stride_bytes, long extent, long elem) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld_bytes % 16 == 0 && stride_bytes % 16 == 0 && extent * elem % 16 == 0;
 }
 
-template <class T, class O, int BM, int BN, int WR, int WC, bool DIRECT>
-__global__ __launch_bounds__(WR * WC * 64, 2) void grouped_dw_kernel(const GroupedDwArgs g) {
-    typedef mm::Tile<T, BM, BN, WR, WC, false, false> Tile;
-    typedef typename Tile::one A;
-    __shared__ __attribute__((aligned(128))) char lds[Tile::LDS];
-    const int mt = (g.M + BN - 1) / BN;
-    const int group = blockIdx.y;
-    const int n0 = (int)(blockIdx.x / mt) * BM, m0 = (int)(blockIdx.x % mt) * BN;
-    const long lo = clamped(g.offsets, group, g.T), hi = clamped(g.offsets, group + 1, g.T);
-    const int rows = (int)(hi > lo ? hi - lo : 0);
-    typename Tile::OpP p = {g.Z + lo * g.ldz + n0 * (long)sizeof(T), g.ldz, min(g.N - n0, BM), rows};
-    typename Tile::OpQ q = {g.X + lo * g.ldx + m0 * (long)sizeof(T), g.ldx, min(g.M - m0, BN), rows};
-    Tile t;
-    t.clear();
-    if (DIRECT) t.run_direct(lds, p, q, rows);
-    else t.run_staged(lds, p, q, rows);
-    char* c = g.C + group * g.stride_c + n0 * g.ldc;
-    const A alpha = (A)g.alpha, beta = (A)g.beta;
-    t.each([&](int i, int j, const A* v, auto cnt) {
-        if (n0 + i < g.N) put<O, A, decltype(cnt)::value>(c + i * g.ldc, m0 + j, g.M, v, alpha, beta, g.vec);
-    });
-}
+template <int V> using Int = std::integral_constant<int, V>;
 
 // A row-tile count that is never less than sum of ceil(rows / BM)
 long row_tiles(long T, int groups, int BM) { return T / BM + (groups < T ? groups : T); }
 
-template <class T, int BM, int BN, int WR, int WC> int grouped_launch(hipStream_t st, bool w_kc, bool direct, const GroupedArgs& g) {
-    const long tiles = row_tiles(g.T, g.groups, BM) * ((g.N + BN - 1) / BN);
-    if (tiles >= 1L << 31) return GPX_ERR_UNSUPPORTED;
-    auto go = [&](auto kc, auto dir) {
-        grouped_kernel<T, BM, BN, WR, WC, decltype(kc)::value, decltype(dir)::value><<<(unsigned)tiles, WR * WC * 64, 0, st>>>(g);
-    };
-    if (w_kc && direct) go(std::true_type{}, std::true_type{});
-    else if (w_kc) go(std::true_type{}, std::false_type{});
-    else if (direct) go(std::false_type{}, std::true_type{});
-    else go(std::false_type{}, std::false_type{});
-    HIP_TRY(hipGetLastError());
-    return GPX_OK;
+// Which tile: the one whose rounds over the 256 CUs take the least time, by the time of a K step (128 bytes of k) with the
+// chip full and with one workgroup on a CU, and of prologue and epilogue.  us, measured on a full chip:
+struct TileCost { int bm, bn, slots; double step, alone, rest; };
+constexpr TileCost kCost16[] = {
+    {256, 256, 256, 1.50, 1.50, 14.0},   // one workgroup of 8 waves a CU: 1.23-1.26 PFLOP/s on 8 x 4096 x 4096 x 7168
+    {128, 128, 512, 0.95, 0.52, 3.0},    // two of 4 waves: 1.07
+    {64, 64, 512, 0.38, 0.25, 2.3},      // two of 4 waves, four LDS stages: 0.63
+    {32, 128, 512, 0.43, 0.30, 2.0},     // a few rows a group, W in 256-byte runs (n contiguous): the read of W bounds it
+    {32, 64, 768, 0.36, 0.25, 2.0}};     // the same, k contiguous: 5.0 TB/s on 32 x 2816 x 2048, 6 TB/s where W is cached
+constexpr TileCost kCost32[] = {{128, 128, 512, 3.30, 2.40, 3.0}, {64, 64, 256, 0.52, 0.52, 1.0}, {32, 64, 256, 0.32, 0.32, 1.0}};   // 4-byte floats
+constexpr TileCost kCost64[] = {{128, 128, 512, 3.90, 2.20, 3.0}, {64, 64, 256, 0.51, 0.51, 1.0}, {32, 64, 256, 0.31, 0.31, 1.0}};   // doubles
+double tile_time(const TileCost& c, double tiles, double steps) {
+    const double full = floor(tiles / c.slots), left = tiles - full * c.slots;
+    return full * (c.step * steps + c.rest) + (left > 256.0 ? c.step * steps + c.rest : left > 0.0 ? c.alone * steps + c.rest : 0.0);
 }
-// 16-bit products: 256 x 256 tiles (one workgroup of 8 waves per CU, 128 KB of LDS) once they fill the chip, else 128 x 128
-// (two workgroups of 4 waves per CU).  bf16, 8 x (4096 x 4096 x 7168): 1.17-1.23 PFLOP/s against 1.02-1.05; 8 groups of one
-// row, N = 1024, K = 512: 17.5 us against 11.5.
-bool tile256(long row_tiles256, long N) { return row_tiles256 * ((N + 255) / 256) >= 256; }
 
 template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArgs& g) {
     // rows of X (k contiguous) and of W in 16-byte chunks, lane offsets of one K step within the buffer resource
     const long wn = w_kc ? g.K : g.N;   // W's contiguous extent
     const bool direct = whole_chunks(g.X, g.ldx, 0, g.K, sizeof(T)) && whole_chunks(g.W, g.ldw, g.stride_w, wn, sizeof(T)) &&
                         256 * g.ldx < (long)mm::kRange && 256 * g.ldw < (long)mm::kRange;
-    if constexpr (sizeof(T) == 2)
-        if (tile256(g.T / 256 + g.groups / 2, g.N)) return grouped_launch<T, 256, 256, 2, 4>(st, w_kc, direct, g);
-    return grouped_launch<T, 128, 128, 2, 2>(st, w_kc, direct, g);
-}
-
-template <class T, class O, int BM, int BN, int WR, int WC> int grouped_dw_launch(hipStream_t st, bool direct, const GroupedDwArgs& g, int groups) {
-    const long tiles = (long)((g.N + BM - 1) / BM) * ((g.M + BN - 1) / BN);
-    if (tiles >= 1L << 31) return GPX_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)tiles, (unsigned)groups);
-    if (direct) grouped_dw_kernel<T, O, BM, BN, WR, WC, true><<<grid, WR * WC * 64, 0, st>>>(g);
-    else grouped_dw_kernel<T, O, BM, BN, WR, WC, false><<<grid, WR * WC * 64, 0, st>>>(g);
+    const double busy = (double)std::min<long>(g.groups, g.T), steps = (double)((g.K * (long)sizeof(T) + 127) / 128);
+    auto time_of = [&](const TileCost& c) {   // half a row tile of every group is empty on average
+        const double mt = std::max(busy, g.T / (double)c.bm + 0.5 * busy);
+        return tile_time(c, mt * ((g.N + c.bn - 1) / c.bn), steps);
+    };
+    int rc = GPX_OK;
+    auto go = [&](auto bm, auto bn, auto wr, auto wc, auto stages) {
+        constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WR = decltype(wr)::value, WC = decltype(wc)::value, ST = decltype(stages)::value;
+        const long tiles = row_tiles(g.T, g.groups, BM) * ((g.N + BN - 1) / BN);
+        if (tiles >= (1L << 31) - 512) {
+            rc = GPX_ERR_UNSUPPORTED;
+            return;
+        }
+        const unsigned grid = (unsigned)((tiles + 511) / 512 * 512);   // whole chunks
+        if (w_kc && direct) grouped_kernel<T, BM, BN, WR, WC, ST, true, true><<<grid, WR * WC * 64, 0, st>>>(g);
+        else if (direct) grouped_kernel<T, BM, BN, WR, WC, ST, false, true><<<grid, WR * WC * 64, 0, st>>>(g);
+        else if (w_kc) grouped_kernel<T, BM, BN, WR, WC, 2, true, false><<<grid, WR * WC * 64, 0, st>>>(g);
+        else grouped_kernel<T, BM, BN, WR, WC, 2, false, false><<<grid, WR * WC * 64, 0, st>>>(g);
+    };
+    auto best_of = [&](const TileCost* c, int n, int not_this) {
+        int best = 0;
+        for (int i = 1; i < n; ++i)
+            if (i != not_this && time_of(c[i]) < time_of(c[best])) best = i;
+        return best;
+    };
+    if constexpr (sizeof(T) == 2) {
+        switch (best_of(kCost16, 5, w_kc ? 3 : 4)) {
+            case 0: go(Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{}); break;
+            case 1: go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}); break;
+            case 2: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<4>{}); break;
+            case 3: go(Int<32>{}, Int<128>{}, Int<1>{}, Int<4>{}, Int<4>{}); break;
+            default: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<4>{});
+        }
+    } else {
+        switch (best_of(sizeof(T) == 4 ? kCost32 : kCost64, 3, -1)) {
+            case 0: go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}); break;
+            case 1: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{}); break;
+            default: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<4>{});
+        }
+    }
     HIP_TRY(hipGetLastError());
-    return GPX_OK;
+    return rc;
 }
 
-template <class T, class O> int grouped_dw_typed(hipStream_t st, const GroupedDwArgs& g, int groups) {
+// The weight gradient's tile and the rows of a part (0: not split), from sizes alone: the workspace follows from it.
+struct DwPlan { int tile, part_rows; long parts; };
+DwPlan dw_plan(int elem, long groups, long T, long M, long N) {
+    const TileCost* c = elem == 2 ? kCost16 : elem == 4 ? kCost32 : kCost64;
+    const int sizes = elem == 2 ? 3 : 2;
+    const double busy = (double)std::max<long>(1, std::min(groups, T)), per = 128.0 / elem, steps = std::max(1.0, ceil(T / busy / per));
+    auto tiles = [&](int i) { return (double)((N + c[i].bn - 1) / c[i].bn) * ((M + c[i].bm - 1) / c[i].bm); };
+    DwPlan best = {0, 0, 0};
+    double least = 1e300;
+    for (int i = 0; i < sizes; ++i) {
+        const double t = tile_time(c[i], tiles(i) * groups, steps);
+        if (t < least) {
+            least = t;
+            best = {i, 0, 0};
+        }
+    }
+    // Split: parts of at least 8 steps, as many as give the chip one round; the slabs are written and read once (4 TB/s) and
+    // the second kernel costs 4 us more.
+    for (int i = 0; i < sizes; ++i) {
+        const double round = std::max(256.0, (double)c[i].slots) / tiles(i);
+        const long rows = std::max<long>((long)(8 * per), ((long)ceil(T / std::max(1.0, round - 0.5 * busy)) + 63) / 64 * 64);
+        if (rows * busy > 0.75 * T) continue;
+        const long parts = T / rows + std::min(groups, T);
+        const double each = std::max(c[i].alone, c[i].step / std::max(1.0, c[i].slots / 256.0));
+        const double t = ceil(tiles(i) * (T / (double)rows + 0.5 * busy) / 256.0) * (each * rows / per + c[i].rest) +
+                         4.0 + 2.0 * parts * (double)(M * N) * std::max(4, elem) / 4e6;
+        if (t < 0.8 * least && rows < (1L << 30) && parts <= 65535) {
+            least = t;
+            best = {i, (int)rows, parts};
+        }
+    }
+    return best;
+}
+long dw_work_bytes(const DwPlan& p, int elem, long M, long N) { return p.part_rows ? p.parts * M * N * std::max(4, elem) : 0; }
+
+template <class T, class O> int grouped_dw_typed(hipStream_t st, const GroupedDwArgs& g, const DwPlan& plan) {
     const bool direct = whole_chunks(g.X, g.ldx, 0, g.M, sizeof(T)) && whole_chunks(g.Z, g.ldz, 0, g.N, sizeof(T)) &&
                         64 * g.ldx < (long)mm::kRange && 64 * g.ldz < (long)mm::kRange;
-    if constexpr (sizeof(T) == 2)
-        if (tile256((long)groups * ((g.N + 255) / 256), g.M)) return grouped_dw_launch<T, O, 256, 256, 2, 4>(st, direct, g, groups);
-    return grouped_dw_launch<T, O, 128, 128, 2, 2>(st, direct, g, groups);
+    int rc = GPX_OK;
+    auto go = [&](auto bm, auto wr, auto wc, auto stages) {
+        constexpr int B = decltype(bm)::value, WR = decltype(wr)::value, WC = decltype(wc)::value, ST = decltype(stages)::value;
+        const long tiles = (long)((g.N + B - 1) / B) * ((g.M + B - 1) / B);
+        if (tiles >= 1L << 31) {
+            rc = GPX_ERR_UNSUPPORTED;
+            return;
+        }
+        if (plan.part_rows) {
+            const dim3 grid((unsigned)tiles, (unsigned)plan.parts);
+            if (direct) grouped_dw_kernel<T, O, B, WR, WC, ST, true, true><<<grid, WR * WC * 64, 0, st>>>(g);
+            else grouped_dw_kernel<T, O, B, WR, WC, 2, false, true><<<grid, WR * WC * 64, 0, st>>>(g);
+            const long size = (long)g.M * g.N;
+            grouped_dw_join_kernel<typename mm::Acc<T>::one, O>
+                <<<dim3((unsigned)std::min<long>((size + 255) / 256, 2048), (unsigned)g.groups), 256, 0, st>>>(g);
+        } else {
+            const dim3 grid((unsigned)tiles, (unsigned)g.groups);
+            if (direct) grouped_dw_kernel<T, O, B, WR, WC, ST, true, false><<<grid, WR * WC * 64, 0, st>>>(g);
+            else grouped_dw_kernel<T, O, B, WR, WC, 2, false, false><<<grid, WR * WC * 64, 0, st>>>(g);
+        }
+    };
+    if constexpr (sizeof(T) == 2) {
+        if (plan.tile == 0) go(Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{});
+        else if (plan.tile == 1) go(Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{});
+        else go(Int<64>{}, Int<2>{}, Int<2>{}, Int<4>{});
+    } else {
+        if (plan.tile == 0) go(Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{});
+        else go(Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{});
+    }
+    HIP_TRY(hipGetLastError());
+    return rc;
 }
 
 constexpr long kMaxExtent = (1L << 31) - 1024;   // row, column and k numbers within one product are 32-bit
@@ -209,9 +381,8 @@ constexpr int kMaxGroups = 65535;
 
 int elem_bytes(int dtype) { return dtype == GPX_F64 ? 8 : dtype == GPX_F32 ? 4 : dtype == GPX_BF16 || dtype == GPX_F16 ? 2 : 0; }
 bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes != 0; }
-bool rows4(const void* p, long ld_bytes, long stride_bytes, int elem) {   // 4-element vector stores
-    const uintptr_t a = (uintptr_t)(elem == 8 ? 16 : 4 * elem);
-    return reinterpret_cast<uintptr_t>(p) % a == 0 && ld_bytes % (long)a == 0 && stride_bytes % (long)a == 0;
+bool aligned_rows(const void* p, long ld_bytes, long stride_bytes) {   // 16-byte stores
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld_bytes % 16 == 0 && stride_bytes % 16 == 0;
 }
 
 }  // namespace
@@ -229,7 +400,7 @@ extern "C" int gpx_grouped_gemm(int dtype, int w_kc, int64_t groups, int64_t T, 
     StreamDevice dev(static_cast<hipStream_t>(hip_stream));
     if (dev.status) return dev.status;
     GroupedArgs g = {static_cast<const char*>(X), static_cast<const char*>(W), static_cast<char*>(Y), offsets, ldx * e, ldw * e,
-                     stride_w * e, ldy * e, T, (int)groups, (int)N, (int)K, alpha, beta, rows4(Y, ldy * e, 0, e)};
+                     stride_w * e, ldy * e, T, (int)groups, (int)N, (int)K, alpha, beta, aligned_rows(Y, ldy * e, 0)};
     const hipStream_t st = static_cast<hipStream_t>(hip_stream);
     switch (dtype) {
         case GPX_F64: return grouped_typed<double>(st, w_kc != 0, g);
@@ -251,22 +422,26 @@ extern "C" int gpx_grouped_gemm_dw(int dtype, int c_dtype, int64_t groups, int64
     if (groups > 1 && stride_c < (N - 1) * ldc + M) return GPX_ERR_ARG;   // results of two groups would overlap
     if (!C || !offsets || (T > 0 && (!X || !Z))) return GPX_ERR_ARG;
     if (misaligned(X, e) || misaligned(Z, e) || misaligned(C, ec) || misaligned(offsets, 8)) return GPX_ERR_ARG;
+    const DwPlan plan = dw_plan(e, groups, T, M, N);
+    if (plan.part_rows && (!work || misaligned(work, 16) || work_bytes < dw_work_bytes(plan, e, M, N))) return GPX_ERR_ARG;
     StreamDevice dev(static_cast<hipStream_t>(hip_stream));
     if (dev.status) return dev.status;
-    GroupedDwArgs g = {static_cast<const char*>(X), static_cast<const char*>(Z), static_cast<char*>(C), offsets, ldx * e, ldz * e,
-                       ldc * ec, stride_c * ec, T, (int)M, (int)N, alpha, beta, rows4(C, ldc * ec, stride_c * ec, ec)};
+    const GroupedDwArgs g = {static_cast<const char*>(X), static_cast<const char*>(Z), static_cast<char*>(C), offsets, ldx * e, ldz * e, ldc * ec,
+                             stride_c * ec, T, (int)M, (int)N, (int)groups, alpha, beta, aligned_rows(C, ldc * ec, stride_c * ec),
+                             static_cast<char*>(work), plan.part_rows, (int)plan.parts};
     const hipStream_t st = static_cast<hipStream_t>(hip_stream);
-    const int n = (int)groups;
     switch (dtype) {
-        case GPX_F64: return grouped_dw_typed<double, double>(st, g, n);
-        case GPX_F32: return grouped_dw_typed<float, float>(st, g, n);
-        case GPX_BF16: return c_dtype == GPX_F32 ? grouped_dw_typed<__bf16, float>(st, g, n) : grouped_dw_typed<__bf16, __bf16>(st, g, n);
-        default: return c_dtype == GPX_F32 ? grouped_dw_typed<_Float16, float>(st, g, n) : grouped_dw_typed<_Float16, _Float16>(st, g, n);
+        case GPX_F64: return grouped_dw_typed<double, double>(st, g, plan);
+        case GPX_F32: return grouped_dw_typed<float, float>(st, g, plan);
+        case GPX_BF16: return c_dtype == GPX_F32 ? grouped_dw_typed<__bf16, float>(st, g, plan) : grouped_dw_typed<__bf16, __bf16>(st, g, plan);
+        default: return c_dtype == GPX_F32 ? grouped_dw_typed<_Float16, float>(st, g, plan) : grouped_dw_typed<_Float16, _Float16>(st, g, plan);
     }
 }
 
 extern "C" int gpx_grouped_gemm_dw_work(int dtype, int64_t groups, int64_t T, int64_t M, int64_t N, int64_t* work_bytes) {
-    if (!elem_bytes(dtype) || !work_bytes || groups < 0 || T < 0 || M < 0 || N < 0) return GPX_ERR_ARG;
-    *work_bytes = 0;
+    const int e = elem_bytes(dtype);
+    if (!e || !work_bytes || groups < 0 || groups > kMaxGroups || T < 0 || M < 0 || N < 0 || T > kMaxExtent || M > kMaxExtent || N > kMaxExtent)
+        return GPX_ERR_ARG;
+    *work_bytes = groups && T && M && N ? dw_work_bytes(dw_plan(e, groups, T, M, N), e, M, N) : 0;
     return GPX_OK;
 }

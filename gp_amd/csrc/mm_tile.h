@@ -36,6 +36,12 @@ template <class T> __device__ __forceinline__ int strided_swizzle(int k) {
     return (k & 3) | ((k >> 3) & 1) << 2;      // 32-byte blocks: rows k..k+3 of the k groups 8q
 }
 
+// of the block numbers of a row of `cols` elements: the permutation must stay within the row
+template <class T> constexpr int swizzle_mask(int cols) {
+    return sizeof(T) == 2 ? (cols / 16 % 8 == 0 ? 7 : cols / 16 % 4 == 0 ? 3 : cols / 16 % 2 == 0 ? 1 : 0)
+                          : (cols / 16 % 4 == 0 ? 3 : cols / 16 % 2 == 0 ? 1 : 0);
+}
+
 template <class T, int ROWS, bool KC>
 __device__ __forceinline__ v4i frag(const char* s, int row0, int kk, int lane) {
     const int r = lane & 15, q = lane >> 4;
@@ -43,7 +49,7 @@ __device__ __forceinline__ v4i frag(const char* s, int row0, int kk, int lane) {
         const int row = row0 + r;
         return *reinterpret_cast<const v4i*>(s + row * 128 + (((kk * 4 + q) ^ (row & 7)) << 4));
     } else if constexpr (sizeof(T) == 2) {
-        constexpr int mask = ROWS / 16 < 8 ? ROWS / 16 - 1 : 7;
+        constexpr int mask = swizzle_mask<T>(ROWS);
         const int k = kk * 32 + 8 * q + (r >> 2);
         const int b = (row0 >> 4) ^ (strided_swizzle<T>(k) & mask);
         const char* p = s + k * (ROWS * 2) + b * 32 + (r & 3) * 8;
@@ -53,7 +59,7 @@ __device__ __forceinline__ v4i frag(const char* s, int row0, int kk, int lane) {
         u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * ROWS * 2));
         return u.v;
     } else {
-        constexpr int E = chunk_elems<T>(), mask = ROWS / 16 < 4 ? ROWS / 16 - 1 : 3;
+        constexpr int E = chunk_elems<T>(), mask = swizzle_mask<T>(ROWS);
         const int k = kk * 4 * E + E * q;
         const int b = (row0 >> 4) ^ (strided_swizzle<T>(k) & mask);
         const T* p = reinterpret_cast<const T*>(s) + k * ROWS + b * 16 + r;
@@ -72,6 +78,7 @@ template <int ROWS, bool KC>
 __device__ __forceinline__ v4i frag_split(const char* s, int row0, int lo, int lane) {
     if constexpr (KC) return frag<_Float16, ROWS, true>(s, row0, lo, lane);
     const int r = lane & 15, q = lane >> 4;
+    static_assert(swizzle_mask<_Float16>(2 * ROWS) == 7, "whole permutations");
     const int k = 8 * q + (r >> 2);
     const int b = ((row0 >> 5) * 4 + ((row0 >> 4) & 1) + 2 * lo) ^ strided_swizzle<_Float16>(k);
     const char* p = s + k * (ROWS * 4) + b * 32 + (r & 3) * 8;
@@ -144,7 +151,7 @@ template <class F, int ROWS, bool KC, int NT> struct Operand {
         } else {
             constexpr int PER = COLS / E;              // chunks per k
             constexpr int HB = 16 / E;                 // chunks per block of 16 columns
-            constexpr int mask = COLS / 16 < 8 ? COLS / 16 - 1 : 7;
+            constexpr int mask = swizzle_mask<T>(COLS);
             k = c / PER;
             const int slot = c % PER;
             row = ((slot / HB) ^ (strided_swizzle<T>(k) & mask)) * 16 + slot % HB * E;
@@ -158,6 +165,19 @@ template <class F, int ROWS, bool KC, int NT> struct Operand {
             k += k0;
             if (KC) r[it] = load_chunk<T>(base + row * ld + (long)k * sizeof(T), row < rows ? K - k : 0);
             else r[it] = load_chunk<T>(base + k * ld + (long)row * sizeof(T), k < K ? rows - row : 0);
+        }
+    }
+    // The same for a step that has more than a step of k behind it: no tests.  Rows that do not exist read the last one
+    // (their results are dropped); with k strided a run may end up to 15 bytes behind its row, in the rows of the next step.
+    __device__ __forceinline__ void load_inside(v4i (&r)[NL], int k0) const {
+#pragma unroll
+        for (int it = 0; it < NL; ++it) {
+            int row, k;
+            place(it * NT + (int)threadIdx.x, row, k);
+            row = min(row, rows - 1);
+            k += k0;
+            const char* p = KC ? base + row * ld + (long)k * sizeof(T) : base + k * ld + (long)row * sizeof(T);
+            __builtin_memcpy(&r[it], p, 16);
         }
     }
     // ---- straight from memory into LDS: 16-byte aligned rows whose contiguous extent is a multiple of E elements, so that
@@ -215,7 +235,13 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
 #pragma unroll
             for (int j = 0; j < TJ; ++j) acc[i][j] = vec{};
     }
-    __device__ __forceinline__ void multiply(const char* s) {
+    // whether any of this wave's rows and columns exist: a ragged last tile costs the matrix cores only the wave rows it has
+    __device__ __forceinline__ bool has_rows(int rows_p, int rows_q) const {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        return wave / WC * (BM / WR) < rows_p && wave % WC * (BN / WC) < rows_q;   // (split, k strided: twice the rows, never less)
+    }
+    // halves: 1 if the second 64 bytes of k are all zeros (the end of K)
+    __device__ __forceinline__ void multiply(const char* s, int halves = 2) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const int i0 = wave / WC * (BM / WR), j0 = wave % WC * (BN / WC);
         if constexpr (Stored<F>::split) {
@@ -240,6 +266,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
         }
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
+            if (kk >= halves) break;
             v4i fp[TI], fq[TJ];
 #pragma unroll
             for (int i = 0; i < TI; ++i) fp[i] = frag<T, BM, PKC>(s, i0 + 16 * i, kk, lane);
@@ -257,18 +284,24 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
         v4i rp[OpP::NL], rq[OpQ::NL];
         const int steps = (K + OpP::BK - 1) / OpP::BK;
         if (steps == 0) return;
-        p.load(rp, 0);
-        q.load(rq, 0);
+        const bool busy = has_rows(p.rows, q.rows);
+        auto load = [&](int s) {
+            if ((s + 2) * OpP::BK <= K) {
+                p.load_inside(rp, s * OpP::BK);
+                q.load_inside(rq, s * OpP::BK);
+            } else {
+                p.load(rp, s * OpP::BK);
+                q.load(rq, s * OpP::BK);
+            }
+        };
+        load(0);
         for (int s = 0; s < steps; ++s) {
             char* st = lds + (s & 1) * STAGE;
             p.stash(st, rp);
             q.stash(st + OpP::BYTES, rq);
-            if (s + 1 < steps) {
-                p.load(rp, (s + 1) * OpP::BK);
-                q.load(rq, (s + 1) * OpP::BK);
-            }
+            if (s + 1 < steps) load(s + 1);
             __syncthreads();   // also: nobody reads the other stage any more when the next step writes it
-            multiply(st);
+            if (busy) multiply(st);
         }
     }
     // K loop on direct loads, STAGES LDS stages: while step s is multiplied, steps s + 1 .. s + STAGES - 1 are on their way
@@ -287,6 +320,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
             p.issue(at + stage * STAGE, lp, s);
             q.issue(at + stage * STAGE + OpP::BYTES, lq, s);
         };
+        const bool busy = has_rows(p.rows, q.rows);
         for (int s = 0; s < STAGES - 1 && s < steps; ++s) issue(s, s);
         int stage = 0, into = STAGES - 1;   // of step s, of step s + STAGES - 1
         for (int s = 0; s < steps; ++s) {
@@ -294,7 +328,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
             if (STAGES > 2 && s + STAGES - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(AHEAD) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (s + STAGES - 1 < steps) issue(s + STAGES - 1, into);
-            multiply(lds + stage * STAGE);
+            if (busy) multiply(lds + stage * STAGE, s >= full && rest * 2 <= BK ? 1 : 2);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             into = into + 1 == STAGES ? 0 : into + 1;
         }
@@ -310,6 +344,26 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
         for (int i = 0; i < TI; ++i)
 #pragma unroll
             for (int j = 0; j < TJ; ++j) *reinterpret_cast<v4f*>(slab + (16 * i + r) * SLAB_LD + j0 + 16 * j + 4 * q) = acc[i][j];
+    }
+    // Epilogue in whole runs: f(i, j, v) for every run of 8 columns j.. of row i, i < rows, j < cols; 16-bit operands
+    template <class Put> __device__ __forceinline__ void each_run(char* lds, int rows, int cols, Put&& f) const {
+        static_assert(!SWAP, "accumulators along j");
+        float* slab = reinterpret_cast<float*>(lds);
+        for (int pass = 0; pass < WR; ++pass) {
+            const int ib = pass * SLAB_ROWS;
+            if (ib >= rows) return;
+            __syncthreads();
+            to_slab(slab, pass);
+            __syncthreads();
+            for (int e = threadIdx.x; e < SLAB_ROWS * (BN / 8); e += NT) {
+                const int il = e / (BN / 8), j = e % (BN / 8) * 8;
+                if (ib + il >= rows || j >= cols) continue;
+                union { v4f w[2]; float v[8]; } u;
+                u.w[0] = *reinterpret_cast<const v4f*>(slab + il * SLAB_LD + j);
+                u.w[1] = *reinterpret_cast<const v4f*>(slab + il * SLAB_LD + j + 4);
+                f(ib + il, j, u.v);
+            }
+        }
     }
     // f(i, j, value pointer, count): count consecutive columns j.. of row i of the tile
     template <class Put> __device__ __forceinline__ void each(Put&& f) {

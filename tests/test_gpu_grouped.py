@@ -117,6 +117,42 @@ def test_grouped_gemm_dw(dtype, out32, shape, frame):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("sizes,n,k", [([9000], 24, 40), ([1, 6000, 0, 2049, 700], 65, 130), ([0, 0, 5000, 0], 130, 17), ([64] * 70 + [8192], 16, 16),
+                                       ([20000, 3], 200, 264)], ids=str)
+def test_grouped_gemm_dw_over_many_rows(dtype, sizes, n, k):
+    """Few results from many rows: the rows are cut into parts whose sums are added afterwards."""
+    lib = _lib()
+    rows = sum(sizes)
+    x, dy = framed(data(1, dtype, rows, k), 3, 1)[1], framed(data(2, dtype, rows, n), 8, 16)[1]
+    off = table(sizes)
+    for alpha, beta in ((1.0, 0.0), (-0.5, 2.0)):
+        old = data(3, dtype, len(sizes), n, k)
+        flat, out = framed(old, 3, 1)
+        lib.grouped_gemm_dw(x, dy, off, out, alpha=alpha, beta=beta)
+        want, tol = oracle.grouped_dw(x, dy, off.tolist(), old, alpha, beta)
+        check(out, want, tol, (alpha, beta))
+        assert untouched(flat, out)
+        again = old.clone()
+        lib.grouped_gemm_dw(x, dy, off, again, alpha=alpha, beta=beta)
+        assert torch.equal(again, out)
+    if dtype in (torch.bfloat16, torch.float16):
+        c = lib.grouped_gemm_dw(x, dy, off, torch.empty(len(sizes), n, k, device="cuda"))
+        check(c, *oracle.grouped_dw(x, dy, off.tolist(), torch.zeros_like(c)))
+
+
+def test_wrong_tables_with_many_rows():
+    """Tables whose groups overlap name more rows than there are: the result is wrong, nothing outside it is touched."""
+    lib = _lib()
+    rows, n, k = 9000, 24, 40
+    x, dy = data(1, torch.float32, rows, k), data(2, torch.float32, rows, n)
+    for offsets in ([0, rows, 0, rows, 0, rows, 0, rows], [rows, -5, 1 << 40, 3, rows, 0, 1, 2]):
+        flat, out = framed(torch.zeros(7, n, k, device="cuda"), 8, 16)
+        lib.grouped_gemm_dw(x, dy, torch.tensor(offsets, device="cuda"), out)
+        assert untouched(flat, out)
+        assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_neighbouring_groups_do_not_mix(dtype):
     """NaN in one group's rows stays in that group's results, for row counts on both sides of a tile's edge."""
     lib = _lib()
