@@ -274,7 +274,7 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
             rc = GPX_ERR_UNSUPPORTED;
             return;
         }
-        const unsigned grid = (unsigned)((tiles + 511) / 512 * 512);   // whole chunks
+        const unsigned grid = (unsigned)((tiles + 7) / 8 * 8);   // as many for every XCD
         if (w_kc && direct) grouped_kernel<T, BM, BN, WR, WC, ST, true, true><<<grid, WR * WC * 64, 0, st>>>(g);
         else if (direct) grouped_kernel<T, BM, BN, WR, WC, ST, false, true><<<grid, WR * WC * 64, 0, st>>>(g);
         else if (w_kc) grouped_kernel<T, BM, BN, WR, WC, 2, true, false><<<grid, WR * WC * 64, 0, st>>>(g);

@@ -336,6 +336,8 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
     // The accumulators of wave row `pass` (BM / WR rows of the tile) as floats in LDS, rows of SLAB_LD: what an epilogue that
     // reads and writes whole 16-byte runs needs.  Between barriers of the caller.
     static constexpr int SLAB_ROWS = BM / WR, SLAB_LD = BN + 4, SLAB = SLAB_ROWS * SLAB_LD * 4;
+    // groups of four columns permuted by the row, so that a column of eight-row runs does not meet in one bank
+    __device__ static __forceinline__ int slab_at(int row, int col) { return row * SLAB_LD + (col ^ (row >> 3 & 7) << 2); }
     __device__ __forceinline__ void to_slab(float* slab, int pass) const {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
         if (wave / WC != pass) return;
@@ -343,7 +345,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
 #pragma unroll
         for (int i = 0; i < TI; ++i)
 #pragma unroll
-            for (int j = 0; j < TJ; ++j) *reinterpret_cast<v4f*>(slab + (16 * i + r) * SLAB_LD + j0 + 16 * j + 4 * q) = acc[i][j];
+            for (int j = 0; j < TJ; ++j) *reinterpret_cast<v4f*>(slab + slab_at(16 * i + r, j0 + 16 * j + 4 * q)) = acc[i][j];
     }
     // Epilogue in whole runs: f(i, j, v) for every run of 8 columns j.. of row i, i < rows, j < cols; 16-bit operands
     template <class Put> __device__ __forceinline__ void each_run(char* lds, int rows, int cols, Put&& f) const {
@@ -359,8 +361,8 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
                 const int il = e / (BN / 8), j = e % (BN / 8) * 8;
                 if (ib + il >= rows || j >= cols) continue;
                 union { v4f w[2]; float v[8]; } u;
-                u.w[0] = *reinterpret_cast<const v4f*>(slab + il * SLAB_LD + j);
-                u.w[1] = *reinterpret_cast<const v4f*>(slab + il * SLAB_LD + j + 4);
+                u.w[0] = *reinterpret_cast<const v4f*>(slab + slab_at(il, j));
+                u.w[1] = *reinterpret_cast<const v4f*>(slab + slab_at(il, j + 4));
                 f(ib + il, j, u.v);
             }
         }

@@ -22,6 +22,7 @@ template <class Body> __device__ __forceinline__ void each_run(int rows, int col
     const int n8 = (cols + 7) / 8;
     long r = first / n8, dr = step / n8;
     int c = (int)(first % n8), dc = (int)(step % n8);
+#pragma unroll 4
     while (r < rows) {
         f((int)r, c * 8);
         r += dr;
@@ -76,6 +77,19 @@ __device__ __forceinline__ double norm_of(const double* part, int parts) {
     for (int d = 32; d; d /= 2) s += __shfl_xor(s, d, 64);
     return sqrt(s);
 }
+
+// A positive factor of any size as mantissa and exponent: floats times it without overflow on the way, by the exact power of
+// two first and one rounded product
+struct Factor {
+    double all;
+    float mantissa;
+    int exponent;
+    __device__ explicit Factor(double v) : all(v) {
+        exponent = isfinite(v) && v > 0.0 ? ilogb(v) : 0;
+        mantissa = (float)ldexp(v, -exponent);
+    }
+    __device__ __forceinline__ float times(float v) const { return ldexpf(v, exponent) * mantissa; }
+};
 
 // steps == 0: the normalised matrix itself.  G and X may be the same buffer.
 template <class T>
@@ -144,7 +158,7 @@ template <class T, class F>
 __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ G, long ldg, long stride_g, int rows, int cols, int pcols,
                                                           const double* __restrict__ part, int parts, double eps, double scale, char* __restrict__ X,
                                                           long ldx, long stride_x) {
-    const double by = scale / (norm_of(part + blockIdx.y * kParts, parts) + eps);
+    const Factor by(scale / (norm_of(part + blockIdx.y * kParts, parts) + eps));
     each_run(rows, pcols, blockIdx.x * 256L + threadIdx.x, gridDim.x * 256L, [&](int r, int c) {
         T v[8];
         load_run(G + blockIdx.y * stride_g + r * ldg + c, cols - c, v);
@@ -152,12 +166,12 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ 
         if constexpr (mm::Stored<F>::split) {
             float w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = (float)(as_double(v[e]) * by);
+            for (int e = 0; e < 8; ++e) w[e] = by.times((float)v[e]);
             Iterate<F>::store8(x, c, w);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (c + e < pcols) Iterate<F>::store(x, c + e, as_double(v[e]) * by);
+                if (c + e < pcols) Iterate<F>::store(x, c + e, as_double(v[e]) * by.all);
         }
     });
 }
@@ -167,7 +181,7 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ 
 struct OrthoArgs {
     const char* P; const char* Q; const char* E; char* D;
     long ldp, ldq, lde, ldd, sp, sq, se, sd;   // bytes
-    int I, J, K;
+    int I, J, K, batch;
     double c1, c2, c3;
 };
 template <class F, class O, bool LAST, int B, int WR, int WC, int ST, bool PKC, bool QKC, bool SYM>
@@ -178,43 +192,71 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
     constexpr int WE = mm::Stored<F>::WIDE;
     constexpr int LDS = mm::Stored<F>::split && Tile::SLAB > Tile::LDS ? Tile::SLAB : Tile::LDS;
     __shared__ __attribute__((aligned(128))) char lds[LDS];
-    const int jt = (g.J + B - 1) / B;
-    int ti, tj;
-    if (SYM) {   // number in the lower triangle, row by row
-        ti = (int)((sqrtf(8.0f * blockIdx.x + 1.0f) - 1.0f) * 0.5f);
-        while ((ti + 1) * (ti + 2) / 2 <= (int)blockIdx.x) ++ti;
-        while (ti * (ti + 1) / 2 > (int)blockIdx.x) --ti;
-        tj = blockIdx.x - ti * (ti + 1) / 2;
+    // Bands of eight tile rows, column by column, matrix after matrix; XCD x takes the x-th eighth of every chunk of
+    // workgroups that the chip holds at a time, so that its CUs share eight row panels and a few column panels in their L2.
+    constexpr int CHUNK = B > 128 ? 256 : 512;
+    const int it = (g.I + B - 1) / B, jt = (g.J + B - 1) / B;
+    const unsigned tiles = SYM ? it * (it + 1) / 2 : it * jt, all = tiles * g.batch, start = blockIdx.x / CHUNK * CHUNK;
+    if (start >= all) return;
+    const unsigned here = min((unsigned)CHUNK, all - start), xcd = blockIdx.x & 7;
+    const unsigned nth = here * xcd / 8 + (blockIdx.x % CHUNK >> 3);
+    if (nth >= here * (xcd + 1) / 8) return;
+    const int mat = (start + nth) / tiles;
+    int in = (start + nth) % tiles, ti, tj;
+    if (SYM) {   // band b: 8 b whole columns, then the triangle on the diagonal, row by row
+        int band = 0, high = min(8, it), size = high * (high + 1) / 2;
+        while (in >= size) {
+            in -= size;
+            ++band;
+            high = min(8, it - 8 * band);
+            size = 8 * band * high + high * (high + 1) / 2;
+        }
+        if (in < 8 * band * high) {
+            ti = 8 * band + in % high;
+            tj = in / high;
+        } else {
+            int r = 0;
+            in -= 8 * band * high;
+            while (in > r) in -= ++r;
+            ti = 8 * band + r;
+            tj = 8 * band + in;
+        }
     } else {
-        ti = blockIdx.x / jt;
-        tj = blockIdx.x % jt;
+        const int band = in / (8 * jt), high = min(8, it - 8 * band);
+        in -= band * 8 * jt;
+        ti = 8 * band + in % high;
+        tj = in / high;
     }
     const int i0 = ti * B, j0 = tj * B;
     const int Jp = (g.J + Iterate<F>::PAD - 1) / Iterate<F>::PAD * Iterate<F>::PAD, Ip = (g.I + Iterate<F>::PAD - 1) / Iterate<F>::PAD * Iterate<F>::PAD;
-    typename Tile::OpP p = {g.P + blockIdx.y * g.sp + (PKC ? i0 * g.ldp : i0 * (long)W), g.ldp, PKC ? min(g.I - i0, B) : min(Ip - i0, B) * WE, g.K};
-    typename Tile::OpQ q = {g.Q + blockIdx.y * g.sq + (QKC ? j0 * g.ldq : j0 * (long)W), g.ldq, QKC ? min(g.J - j0, B) : min(Jp - j0, B) * WE, g.K};
+    typename Tile::OpP p = {g.P + mat * g.sp + (PKC ? i0 * g.ldp : i0 * (long)W), g.ldp, PKC ? min(g.I - i0, B) : min(Ip - i0, B) * WE, g.K};
+    typename Tile::OpQ q = {g.Q + mat * g.sq + (QKC ? j0 * g.ldq : j0 * (long)W), g.ldq, QKC ? min(g.J - j0, B) : min(Jp - j0, B) * WE, g.K};
     Tile t;
     t.clear();
     t.run_direct(lds, p, q, g.K);
     const one c1 = (one)g.c1, c2 = (one)g.c2, c3 = (one)g.c3;
-    const char* E = g.E + blockIdx.y * g.se;
-    char* D = g.D + blockIdx.y * g.sd;
+    const char* E = g.E + mat * g.se;
+    char* D = g.D + mat * g.sd;
     if constexpr (mm::Stored<F>::split) {
         // Through LDS, one wave row of the tile at a time, so that planes are read and written in runs of 16 bytes, the mirrored
         // tile too (single elements from the accumulators: 90 us for a 256 x 256 tile, most of it the mirrored stores).
         float* slab = reinterpret_cast<float*>(lds);
-        constexpr int NT = WR * WC * 64, R = Tile::SLAB_ROWS, LD = Tile::SLAB_LD;
+        constexpr int NT = WR * WC * 64, R = Tile::SLAB_ROWS;
         for (int pass = 0; pass < WR; ++pass) {
             const int ib = i0 + pass * R;
             __syncthreads();
             t.to_slab(slab, pass);
             __syncthreads();
             for (int e = threadIdx.x; e < R * (B / 8); e += NT) {
-                const int i = ib + e / (B / 8), jl = e % (B / 8) * 8, j = j0 + jl;
+                const int il = e / (B / 8), i = ib + il, jl = e % (B / 8) * 8, j = j0 + jl;
                 if (i >= g.I || j >= Jp) continue;
                 float v[8];
+                const mm::v4f lo = *reinterpret_cast<const mm::v4f*>(slab + Tile::slab_at(il, jl)), hi = *reinterpret_cast<const mm::v4f*>(slab + Tile::slab_at(il, jl + 4));
 #pragma unroll
-                for (int x = 0; x < 8; ++x) v[x] = c1 * slab[(i - ib) * LD + jl + x];
+                for (int x = 0; x < 4; ++x) {
+                    v[x] = c1 * lo[x];
+                    v[4 + x] = c1 * hi[x];
+                }
                 if (c2 != 0.0f) Iterate<F>::add8(E + i * g.lde, j, c2, v);
                 if (SYM && ti == tj) {
 #pragma unroll
@@ -238,12 +280,14 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
                 }
             }
             if (SYM && ti != tj) {   // D(j, i): E is symmetric to the bit, so both triangles are
-                for (int e = threadIdx.x; e < B * (R / 8); e += NT) {
-                    const int jl = e / (R / 8), j = j0 + jl, il = e % (R / 8) * 8, i = ib + il;
+                // eight lanes along i (128 bytes of a row of D, both planes twice), eight along j
+                for (int e = threadIdx.x; e < B * ((R + 63) / 64 * 8); e += NT) {
+                    const int jl = (e >> 3) % B, j = j0 + jl, il = ((e & 7) + (e >> 3) / B * 8) * 8, i = ib + il;
+                    if (R % 64 != 0 && il >= R) continue;
                     if (j >= g.J || i >= Ip) continue;
                     float v[8];
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) v[x] = c1 * slab[(il + x) * LD + jl];
+                    for (int x = 0; x < 8; ++x) v[x] = c1 * slab[Tile::slab_at(il + x, jl)];
                     if (c2 != 0.0f) Iterate<F>::add8(E + j * g.lde, i, c2, v);
                     Iterate<F>::store8(D + j * g.ldd, i, v);
                 }
@@ -276,13 +320,18 @@ struct OrthoWork {   // offsets and strides in bytes; rows of the iterates padde
     long part, x[2], a, b, total;
     long ldx, sx, lda, sa;
 };
+// Rows of a power of two of bytes would meet in few memory channels: the K step of a tile reads 128 bytes of every row.
+template <class F> long row_bytes(int cols) {
+    const long b = Iterate<F>::bytes(padded<F>(cols));
+    return b % 1024 == 0 ? b + 128 : b;
+}
 template <class F> OrthoWork ortho_work_of(long batch, int rows, int cols) {
     const int s = std::min(rows, cols);
     auto up = [](long v) { return (v + 255) / 256 * 256; };
     OrthoWork o;
-    o.ldx = Iterate<F>::bytes(padded<F>(cols));
+    o.ldx = row_bytes<F>(cols);
     o.sx = o.ldx * rows;
-    o.lda = Iterate<F>::bytes(padded<F>(s));
+    o.lda = row_bytes<F>(s);
     o.sa = o.lda * s;
     o.part = 0;
     o.x[0] = up(batch * kParts * 8);
@@ -321,11 +370,16 @@ TileChoice choose_tile(bool sym, int I, int J, int K, int batch) {
 
 template <class F, class O, bool LAST, bool PKC, bool QKC, bool SYM> int launch(hipStream_t st, const OrthoArgs& g, int batch) {
 #define GO(B, R, C, S) go(std::integral_constant<int, B>{}, std::integral_constant<int, R>{}, std::integral_constant<int, C>{}, std::integral_constant<int, S>{})
+    int rc = GPX_OK;
     auto go = [&](auto tile, auto wr, auto wc, auto stages) {
         constexpr int B = decltype(tile)::value, WR = decltype(wr)::value, WC = decltype(wc)::value, ST = decltype(stages)::value;
         const long it = (g.I + B - 1) / B, jt = (g.J + B - 1) / B;
-        const long tiles = SYM ? it * (it + 1) / 2 : it * jt;
-        ortho_mm_kernel<F, O, LAST, B, WR, WC, ST, PKC, QKC, SYM><<<dim3((unsigned)tiles, (unsigned)batch), WR * WC * 64, 0, st>>>(g);
+        const long grid = ((SYM ? it * (it + 1) / 2 : it * jt) * batch + 7) / 8 * 8;   // as many for every XCD
+        if (grid >= 1L << 31) {
+            rc = GPX_ERR_UNSUPPORTED;
+            return;
+        }
+        ortho_mm_kernel<F, O, LAST, B, WR, WC, ST, PKC, QKC, SYM><<<(unsigned)grid, WR * WC * 64, 0, st>>>(g);
     };
     if constexpr (mm::Stored<F>::split) {
         const TileChoice c = choose_tile(SYM, g.I, g.J, g.K, batch);
@@ -333,10 +387,14 @@ template <class F, class O, bool LAST, bool PKC, bool QKC, bool SYM> int launch(
         else if (c == TILE192) GO(192, 2, 4, 2);
         else if (c == TILE128) GO(128, 2, 2, 2);
         else GO(64, 2, 2, 4);
-    } else GO(128, 2, 2, 2);
+    } else {   // doubles: 64 x 64 tiles cost 4 % on a full chip and are three to four times as many; 32 x 32 where these are few
+        const long it = (g.I + 63) / 64, jt = (g.J + 63) / 64;
+        if ((SYM ? it * (it + 1) / 2 : it * jt) * batch >= 192) GO(64, 2, 2, 2);
+        else GO(32, 2, 2, 4);
+    }
 #undef GO
     HIP_TRY(hipGetLastError());
-    return GPX_OK;
+    return rc;
 }
 
 // Largest |a s + b s^3 + c s^5| for 0 <= s <= top, a little above it: the ends and the zeros of the derivative
@@ -410,9 +468,13 @@ struct OrthoSmallArgs {
     float gram[64], square[64], linear[64], unit[64], apply[64];   // factors of every step, powers of two included
 };
 constexpr int small_row(int values) { return values * 4 + 32; }
+// Bytes of LDS, or 0 where the matrix does not fit or one workgroup would need longer than the many of the general path:
+// 0.9 us + 1.5 us per 10^6 of S S (2 L + S) a step (128 x 128: 10 us) against 13 us there, most of it three launches.
 long small_lds(int rows, int cols) {
-    const int s = (std::min(rows, cols) + 31) / 32 * 32, l = (std::max(rows, cols) + 31) / 32 * 32;
-    return s <= kSmallSide && l <= (1 << 16) ? (long)s * (small_row(l) + small_row(s)) + (s == 32 ? kSmallWaves * 3 * 1024 : 0) : 1L << 40;
+    const long s = (std::min(rows, cols) + 31) / 32 * 32, l = (std::max(rows, cols) + 31) / 32 * 32;
+    if (s > kSmallSide || l > (1 << 16) || s * s * (2 * l + s) > 6500000) return 0;
+    const long bytes = s * (small_row((int)l) + small_row((int)s)) + (s == 32 ? kSmallWaves * 3 * 1024 : 0);
+    return bytes <= kSmallLds ? bytes : 0;
 }
 __device__ __forceinline__ mm::v4i small_frag_kc(const char* m, int ld, int row0, int k32, int lo, int lane) {
     return *reinterpret_cast<const mm::v4i*>(m + (row0 + (lane & 15)) * ld + k32 * 128 + lo * 64 + (lane >> 4) * 16);
@@ -478,18 +540,18 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
     s = 0.0;
 #pragma unroll
     for (int w = 0; w < kSmallWaves; ++w) s += ws[w];
-    const double by = g.scale / (sqrt(s) + g.eps);
+    const Factor by(g.scale / (sqrt(s) + g.eps));
     each_run(g.rows, g.cols, threadIdx.x, kSmallWaves * 64, [&](int row, int c) {
         T v[8];
         load_run(G + row * g.ldg + c, g.cols - c, v);
         if (tall) {
 #pragma unroll
             for (int x = 0; x < 8; ++x)
-                if (c + x < g.cols) Iterate<mm::Split>::store(X + (c + x) * ldx, row, (float)(as_double(v[x]) * by));
+                if (c + x < g.cols) Iterate<mm::Split>::store(X + (c + x) * ldx, row, by.times((float)v[x]));
         } else {
             float w[8];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) w[x] = (float)(as_double(v[x]) * by);
+            for (int x = 0; x < 8; ++x) w[x] = by.times((float)v[x]);
             Iterate<mm::Split>::store8(X + row * ldx, c, w);
         }
     });
@@ -619,7 +681,7 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
     const OrthoFactors f = ortho_factors(mm::Stored<F>::split, steps, coef);
     if constexpr (mm::Stored<F>::split) {
         const long bytes = small_lds(rows, cols);
-        if (steps > 0 && bytes <= kSmallLds) {
+        if (steps > 0 && bytes) {
             OrthoSmallArgs g = {ldg, stride_g, ldo, stride_o, rows, cols, steps, eps, f.start, {}, {}, {}, {}, {}};
             for (int k = 0; k < steps; ++k) {
                 g.gram[k] = (float)f.gram[k];
@@ -657,17 +719,17 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
     const int s = std::min(rows, cols), l = std::max(rows, cols);
     for (int k = 0; k < steps; ++k) {
         char *from = x[k & 1], *to = x[~k & 1];
-        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, s, s, l, f.gram[k], 0.0, 0.0};
+        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, s, s, l, batch, f.gram[k], 0.0, 0.0};
         int rc = tall ? launch<F, F, false, false, false, true>(st, gram, batch) : launch<F, F, false, true, true, true>(st, gram, batch);
         if (rc) return rc;
-        const OrthoArgs poly = {a, a, a, b, o.lda, o.lda, o.lda, o.lda, o.sa, o.sa, o.sa, o.sa, s, s, s,
+        const OrthoArgs poly = {a, a, a, b, o.lda, o.lda, o.lda, o.lda, o.sa, o.sa, o.sa, o.sa, s, s, s, batch,
                                 f.square[k], f.linear[k], f.unit[k]};
         if ((rc = launch<F, F, false, true, true, true>(st, poly, batch))) return rc;
         const bool last = k + 1 == steps;
         const long ldd = last ? ldo * (long)sizeof(T) : o.ldx, sd = last ? stride_o * (long)sizeof(T) : o.sx;
         char* d = last ? reinterpret_cast<char*>(O) : to;
-        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, rows, cols, s, f.apply[k], 0.0, 0.0}
-                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, rows, cols, s, f.apply[k], 0.0, 0.0};
+        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, rows, cols, s, batch, f.apply[k], 0.0, 0.0}
+                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, rows, cols, s, batch, f.apply[k], 0.0, 0.0};
         if (tall) rc = last ? launch<F, T, true, true, true, false>(st, apply, batch) : launch<F, F, false, true, true, false>(st, apply, batch);
         else rc = last ? launch<F, T, true, true, false, false>(st, apply, batch) : launch<F, F, false, true, false, false>(st, apply, batch);
         if (rc) return rc;
