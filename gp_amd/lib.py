@@ -346,58 +346,66 @@ lib.gpx_grouped_gemm_dw_work.argtypes = [_i, _i64, _i64, _i64, _i64, C.POINTER(_
 lib.gpx_orthogonalize.argtypes = [_i, _i64, _i64, _i64, _vp, _i64, _i64, _i, _vp, _d, _vp, _i64, _i64, _vp, _i64, _vp]
 lib.gpx_orthogonalize_work.argtypes = [_i, _i64, _i64, _i64, C.POINTER(_i64)]
 
-_dtype_codes = {}
+_torch = None
+_codes = {}
+
+
+def _load_torch():
+    global _torch, _raw_stream
+    import torch
+    _codes.update({torch.float64: F64, torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+    # the handle of torch's current stream of a device; the public way builds a Stream object for it (1 us of a 6 us call)
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _torch = torch
 
 
 def _dtype(t, what):
-    if not _dtype_codes:
-        import torch
-        _dtype_codes.update({torch.float64: F64, torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
-    code = _dtype_codes.get(t.dtype)
+    if _torch is None:
+        _load_torch()
+    code = _codes.get(t.dtype)
     if code is None:
         raise ValueError(f"{what}: float64, float32, bfloat16 or float16, not {t.dtype}")
     return code
 
 
-def _rows(t, dims, what):
-    """(stride between matrices, stride between rows) of a tensor of `dims` dimensions with contiguous rows."""
-    if t.dim() != dims:
-        raise ValueError(f"{what}: {dims} dimensions, not {t.dim()}")
-    cols, count = t.shape[-1], t.shape[-2]
-    if cols > 1 and t.stride(-1) != 1:
+def _rows(shape, stride, what):
+    """Stride between rows of a tensor whose last dimension is contiguous."""
+    cols, rows = shape[-1], shape[-2]
+    if cols > 1 and stride[-1] != 1:
         raise ValueError(f"{what}: the last dimension has to be contiguous")
-    ld = t.stride(-2) if count > 1 else max(cols, 1)
+    ld = stride[-2] if rows > 1 else max(cols, 1)
     if ld < cols:
         raise ValueError(f"{what}: rows overlap (stride {ld} for {cols} elements)")
-    return (t.stride(0) if dims == 3 and t.shape[0] > 1 else 0), ld
+    return ld
 
 
-def _one_device(*tensors):
-    dev = tensors[0].device
-    if dev.type != "cuda":
-        raise ValueError(f"tensors on the GPU are wanted, not on {dev}")
-    for t in tensors[1:]:
-        if t.device != dev:
-            raise ValueError(f"all tensors on one device are wanted: {dev} and {t.device}")
-    return dev.index
+def _one_device(first, *others):
+    index = first.get_device()
+    if index < 0 or not first.is_cuda:
+        raise ValueError(f"tensors on the GPU are wanted, not on {first.device}")
+    for t in others:
+        if t.get_device() != index:
+            raise ValueError(f"all tensors on one device are wanted: {first.device} and {t.device}")
+    return index
 
 
 def _launch(fn, what, index, *args):
     """fn(..., stream) on torch's current stream of device `index`; the null stream belongs to the current device."""
-    import torch
-    stream = torch.cuda.current_stream(index).cuda_stream
-    if stream or index == torch.cuda.current_device():
-        check(fn(*args, stream), what)
+    stream = _raw_stream(index)
+    if stream or index == _torch.cuda.current_device():
+        status = fn(*args, stream)
     else:
-        with torch.cuda.device(index):
-            check(fn(*args, stream), what)
+        with _torch.cuda.device(index):
+            status = fn(*args, stream)
+    if status:
+        check(status, what)
 
 
 def _offsets(offsets, groups):
-    if str(offsets.dtype) != "torch.int64" or offsets.dim() != 1 or not offsets.is_contiguous():
+    if offsets.dtype is not _torch.int64 or offsets.dim() != 1 or not offsets.is_contiguous():
         raise ValueError("offsets: a contiguous vector of int64 is wanted")
-    if offsets.shape[0] != groups + 1:
-        raise ValueError(f"offsets: {groups + 1} values for {groups} groups, not {offsets.shape[0]}")
+    if offsets.numel() != groups + 1:
+        raise ValueError(f"offsets: {groups + 1} values for {groups} groups, not {offsets.numel()}")
 
 
 def _work(query, like, *args):
@@ -406,8 +414,7 @@ def _work(query, like, *args):
     check(query(*args, C.byref(n)), "workspace query")
     if n.value == 0:
         return None, 0
-    w = like.new_empty(-(-n.value // like.element_size()))
-    return w, n.value
+    return like.new_empty(-(-n.value // like.element_size())), n.value
 
 
 def grouped_gemm(x, w, offsets, out, w_kc=True, alpha=1.0, beta=0.0):
@@ -415,67 +422,71 @@ def grouped_gemm(x, w, offsets, out, w_kc=True, alpha=1.0, beta=0.0):
 
     x (T, K), out (T, N); w (G, N, K) for w_kc, else (G, K, N); offsets (G + 1,) int64 on the device.  The gradient of x is
     grouped_gemm(dy, w, offsets, dx, w_kc=not w_kc); that of w is grouped_gemm_dw."""
-    index = _one_device(x, w, offsets, out)
     code = _dtype(x, "x")
-    if w.dtype != x.dtype or out.dtype != x.dtype:
+    index = _one_device(x, w, offsets, out)
+    if w.dtype is not x.dtype or out.dtype is not x.dtype:
         raise ValueError("x, w and out have to be of one type")
-    (_, ldx), (_, ldy) = _rows(x, 2, "x"), _rows(out, 2, "out")
-    stride_w, ldw = _rows(w, 3, "w")
-    groups, n, k = w.shape if w_kc else (w.shape[0], w.shape[2], w.shape[1])
-    rows = x.shape[0]
-    if x.shape[1] != k or tuple(out.shape) != (rows, n):
-        raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, w {tuple(w.shape)}, out {tuple(out.shape)}")
+    sx, sw, so = x.shape, w.shape, out.shape
+    if len(sx) != 2 or len(sw) != 3 or len(so) != 2:
+        raise ValueError(f"dimensions do not fit: x {tuple(sx)}, w {tuple(sw)}, out {tuple(so)}")
+    groups, n, k = sw if w_kc else (sw[0], sw[2], sw[1])
+    rows = sx[0]
+    if sx[1] != k or so[0] != rows or so[1] != n:
+        raise ValueError(f"shapes do not fit: x {tuple(sx)}, w {tuple(sw)}, out {tuple(so)}")
+    tw = w.stride()
+    ldx, ldw, ldy = _rows(sx, x.stride(), "x"), _rows(sw, tw, "w"), _rows(so, out.stride(), "out")
     _offsets(offsets, groups)
-    _launch(lib.gpx_grouped_gemm, "grouped_gemm", index, code, int(w_kc), groups, rows, n, k, alpha, x.data_ptr(), ldx, w.data_ptr(),
-            ldw, stride_w, offsets.data_ptr(), beta, out.data_ptr(), ldy)
+    _launch(lib.gpx_grouped_gemm, "grouped_gemm", index, code, w_kc, groups, rows, n, k, alpha, x.data_ptr(), ldx, w.data_ptr(),
+            ldw, tw[0] if groups > 1 else 0, offsets.data_ptr(), beta, out.data_ptr(), ldy)
     return out
 
 
 def grouped_gemm_dw(x, dy, offsets, out, alpha=1.0, beta=0.0):
     """out[g] = alpha * dy_g^T x_g + beta * out[g] over the rows of every group: x (T, K), dy (T, N), out (G, N, K) of their type,
     or float32 for 16-bit rows.  For weights in the (G, K, N) layout exchange x and dy."""
-    index = _one_device(x, dy, offsets, out)
     code, code_out = _dtype(x, "x"), _dtype(out, "out")
-    if dy.dtype != x.dtype:
+    index = _one_device(x, dy, offsets, out)
+    if dy.dtype is not x.dtype:
         raise ValueError("x and dy have to be of one type")
     if code_out != code and not (code_out == F32 and code in (BF16, F16)):
         raise ValueError(f"out: {x.dtype}, or float32 for 16-bit rows, not {out.dtype}")
-    (_, ldx), (_, ldz) = _rows(x, 2, "x"), _rows(dy, 2, "dy")
-    stride_c, ldc = _rows(out, 3, "out")
-    groups, n, k = out.shape
-    rows = x.shape[0]
-    if x.shape[1] != k or tuple(dy.shape) != (rows, n):
-        raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, dy {tuple(dy.shape)}, out {tuple(out.shape)}")
+    sx, sz, so = x.shape, dy.shape, out.shape
+    if len(sx) != 2 or len(sz) != 2 or len(so) != 3 or sx[1] != so[2] or sz[0] != sx[0] or sz[1] != so[1]:
+        raise ValueError(f"shapes do not fit: x {tuple(sx)}, dy {tuple(sz)}, out {tuple(so)}")
+    groups, n, k = so
+    rows = sx[0]
+    tc = out.stride()
+    ldx, ldz, ldc = _rows(sx, x.stride(), "x"), _rows(sz, dy.stride(), "dy"), _rows(so, tc, "out")
     _offsets(offsets, groups)
     work, size = _work(lib.gpx_grouped_gemm_dw_work, x, code, groups, rows, k, n)
     _launch(lib.gpx_grouped_gemm_dw, "grouped_gemm_dw", index, code, code_out, groups, rows, k, n, alpha, x.data_ptr(), ldx,
-            dy.data_ptr(), ldz, offsets.data_ptr(), beta, out.data_ptr(), ldc, stride_c, work.data_ptr() if size else None, size)
+            dy.data_ptr(), ldz, offsets.data_ptr(), beta, out.data_ptr(), ldc, tc[0] if groups > 1 else 0,
+            work.data_ptr() if size else None, size)
     return out
 
 
 def orthogonalize(g, out, steps=5, coef=None, eps=1e-7):
     """The Newton-Schulz update of g (M, N) or (B, M, N) into out (of g's shape and type; g itself is allowed): g / (|g|_F + eps),
     then `steps` times x <- a x + (b A + c A A) x with A = x x^T.  coef: (a, b, c), or one such triple for every step."""
-    index = _one_device(g, out)
     code = _dtype(g, "g")
-    if out.dtype != g.dtype or out.shape != g.shape:
+    index = _one_device(g, out)
+    shape = g.shape
+    if out.dtype is not g.dtype or out.shape != shape:
         raise ValueError("out has to be of g's shape and type")
-    if g.dim() == 2:
-        g3, out3 = g.unsqueeze(0), out.unsqueeze(0)
-    else:
-        g3, out3 = g, out
-    (stride_g, ldg), (stride_o, ldo) = _rows(g3, 3, "g"), _rows(out3, 3, "out")
-    batch, rows, cols = g3.shape
+    if len(shape) != 2 and len(shape) != 3:
+        raise ValueError(f"g: 2 or 3 dimensions, not {len(shape)}")
+    tg, to = g.stride(), out.stride()
+    ldg, ldo = _rows(shape, tg, "g"), _rows(shape, to, "out")
+    batch, rows, cols = shape if len(shape) == 3 else (1, *shape)
     table = None
     if coef is not None:
         table = _c(coef)
         if table.shape == (3,):
-            table = np.tile(table, steps)
+            table = np.tile(table, max(steps, 0))
         elif table.shape != (steps, 3):
             raise ValueError("coef: three values, or three for every step")
-        table = np.ascontiguousarray(table)
     work, size = _work(lib.gpx_orthogonalize_work, g, code, batch, cols, rows)
-    _launch(lib.gpx_orthogonalize, "orthogonalize", index, code, batch, cols, rows, g.data_ptr(), ldg, stride_g, steps,
-            table.ctypes.data if table is not None and steps else None, eps, out.data_ptr(), ldo, stride_o,
+    _launch(lib.gpx_orthogonalize, "orthogonalize", index, code, batch, cols, rows, g.data_ptr(), ldg, tg[0] if batch > 1 else 0, steps,
+            table.ctypes.data if table is not None and steps > 0 else None, eps, out.data_ptr(), ldo, to[0] if batch > 1 else 0,
             work.data_ptr() if size else None, size)
     return out
