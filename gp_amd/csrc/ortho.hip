@@ -113,6 +113,14 @@ __global__ __launch_bounds__(256) void ortho_normalize_kernel(const T* G, long l
 // every iterate from the coefficients and places the largest possible element at 2^15: nothing overflows, and the smallest
 // step of the second plane is 2^-39 of that bound.
 template <class F> struct Iterate;
+// v = h + l.  The compiler may form a converted product in one rounding and the product itself in two; h has to be one value
+// for both planes (told apart at ties, the planes would disagree by a step of the first one).
+__device__ __forceinline__ void split(float v, _Float16& h, _Float16& l) {
+    unsigned bits = __builtin_bit_cast(unsigned short, (_Float16)v);
+    asm("" : "+v"(bits));
+    h = __builtin_bit_cast(_Float16, (unsigned short)bits);
+    l = (_Float16)(v - (float)h);
+}
 template <> struct Iterate<double> {
     static constexpr int PAD = 2;
     __device__ static void store(char* row, int j, double v) { reinterpret_cast<double*>(row)[j] = v; }
@@ -124,9 +132,7 @@ template <> struct Iterate<mm::Split> {
     __device__ static long at(int j) { return (long)(j >> 5) * 64 + (j & 31); }
     __device__ static void store(char* row, int j, float v) {
         _Float16* p = reinterpret_cast<_Float16*>(row) + at(j);
-        const _Float16 h = (_Float16)v;
-        p[0] = h;
-        p[32] = (_Float16)(v - (float)h);
+        split(v, p[0], p[32]);
     }
     __device__ static float load(const char* row, int j) {
         const _Float16* p = reinterpret_cast<const _Float16*>(row) + at(j);
@@ -138,8 +144,10 @@ template <> struct Iterate<mm::Split> {
         mm::v8h h, l;
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-            h[x] = (_Float16)v[x];
-            l[x] = (_Float16)(v[x] - (float)h[x]);
+            _Float16 a, b;
+            split(v[x], a, b);
+            h[x] = a;
+            l[x] = b;
         }
         _Float16* p = reinterpret_cast<_Float16*>(row) + at(j);
         *reinterpret_cast<mm::v8h*>(p) = h;
@@ -503,8 +511,10 @@ __device__ __forceinline__ void small_store4(char* row, int j, mm::v4f v) {   //
     v4h h, l;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-        h[x] = (_Float16)v[x];
-        l[x] = (_Float16)(v[x] - (float)h[x]);
+        _Float16 a, b;
+        split(v[x], a, b);
+        h[x] = a;
+        l[x] = b;
     }
     char* p = row + (j >> 5) * 128 + (j & 31) * 2;
     *reinterpret_cast<v4h*>(p) = h;

@@ -57,6 +57,19 @@ def test_steps_and_coefficients(dtype, steps, coef):
     check(lib.orthogonalize(g, torch.empty_like(g), steps=steps, coef=coef), g, steps=steps, coef=coef)
 
 
+@pytest.mark.parametrize("size", [(100, 128), (100, 3000), (700, 600)], ids=str)
+def test_every_element_keeps_22_bits(size):
+    """(1, 0, 0) leaves the normalised matrix: no element may lose more than the last of its 22 bits on the way, twice a step
+    (once into the planes, once out of the product with the planes of I), or 2^-36 of the largest possible value."""
+    lib = _lib()
+    g = data(1, torch.float32, *size)
+    for steps in (1, 3):
+        want = g.double() / (torch.linalg.norm(g.double()) + 1e-7)
+        out = lib.orthogonalize(g, torch.empty_like(g), steps=steps, coef=(1.0, 0.0, 0.0))
+        off = (out.double() - want).abs() - (steps + 1) * 2.0 ** -21 * want.abs() - 2.0 ** -36
+        assert float(off.max()) <= 0.0
+
+
 def test_cubic_steps_reach_the_polar_factor():
     """(1.5, -0.5, 0) converges to U V^T: the rows of the result are orthonormal."""
     lib = _lib()
