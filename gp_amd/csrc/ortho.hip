@@ -184,13 +184,13 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ 
     });
 }
 
-// D = c1 P Q^T + c2 E + c3 I over a batch, E and D in the format F, or (LAST) D in the type O of the result.
+// D = c1 P Q^T + c2 E over a batch, E and D in the format F, or (LAST) D in the type O of the result.
 // SYM: D is symmetric; tiles on and below the diagonal are computed, and those below it stored on both sides.
 struct OrthoArgs {
     const char* P; const char* Q; const char* E; char* D;
     long ldp, ldq, lde, ldd, sp, sq, se, sd;   // bytes
     int I, J, K, batch;
-    double c1, c2, c3;
+    double c1, c2;
 };
 template <class F, class O, bool LAST, int B, int WR, int WC, int ST, bool PKC, bool QKC, bool SYM>
 __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2) void ortho_mm_kernel(const OrthoArgs g) {
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
     Tile t;
     t.clear();
     t.run_direct(lds, p, q, g.K);
-    const one c1 = (one)g.c1, c2 = (one)g.c2, c3 = (one)g.c3;
+    const one c1 = (one)g.c1, c2 = (one)g.c2;
     const char* E = g.E + mat * g.se;
     char* D = g.D + mat * g.sd;
     if constexpr (mm::Stored<F>::split) {
@@ -266,10 +266,6 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
                     v[4 + x] = c1 * hi[x];
                 }
                 if (c2 != 0.0f) Iterate<F>::add8(E + i * g.lde, j, c2, v);
-                if (SYM && ti == tj) {
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) v[x] += j + x == i ? c3 : 0.0f;
-                }
                 if constexpr (LAST) {
                     O* d = reinterpret_cast<O*>(D + i * g.ldd) + j;
                     typedef O o8 __attribute__((ext_vector_type(8)));
@@ -308,7 +304,6 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
             if (i >= g.I || j >= (LAST ? g.J : Jp)) return;
             one d = c1 * v[0];
             if (c2 != one(0) && j < g.J) d += c2 * Iterate<F>::load(E + i * g.lde, j);
-            if (SYM && i == j) d += c3;
             if constexpr (LAST) {
                 reinterpret_cast<O*>(D + i * g.ldd)[j] = (O)d;
             } else {
@@ -433,7 +428,7 @@ double largest_quadratic(double b, double c, double top) {   // largest |b u + c
     return most;
 }
 // the factors of every step's three products, powers of two of the split format included
-struct OrthoFactors { double start, gram[64], square[64], linear[64], unit[64], apply[64]; };
+struct OrthoFactors { double start, gram[64], square[64], linear[64], apply[64], keep[64]; };
 int place(double bound);
 OrthoFactors ortho_factors(bool scaled, int steps, const double* coef) {
     constexpr double slack = 1.01;   // rounding may carry a singular value past the bound of the exact iterate
@@ -446,15 +441,15 @@ OrthoFactors ortho_factors(bool scaled, int steps, const double* coef) {
         top = std::max(top, 0x1p-400);
         const double next = slack * largest_value(a, b, c, top);
         const int ea = scaled ? place(slack * top * top) : 0;
-        const int eb = scaled ? place(slack * (fabs(a) + largest_quadratic(b, c, top * top))) : 0;
+        const int eb = scaled ? place(slack * largest_quadratic(b, c, top * top)) : 0;
         const int en = scaled && k + 1 < steps ? place(next) : 0;
         f.gram[k] = ldexp(1.0, ea - 2 * ex);
         f.square[k] = ldexp(c, eb - 2 * ea);
         f.linear[k] = ldexp(b, eb - ea);
-        // a I goes into the square factor: its largest element is of the size of a anyway, and the product that follows
-        // reads X once instead of twice
-        f.unit[k] = ldexp(a, eb);
         f.apply[k] = ldexp(1.0, en - ex - eb);
+        // a X is added to the finished sum: inside it, as a I in the square factor, every later addition of the sum would round
+        // relative to a X (first steps, 4096 x 4096: error 4.2e-7 instead of 4e-8)
+        f.keep[k] = ldexp(a, en - ex);
         top = next;
         ex = en;
     }
@@ -466,14 +461,14 @@ int place(double bound) { return bound > 0.0 ? 14 - std::ilogb(bound) : 14; }
 // ---- small matrices: all steps in one workgroup -------------------------------------------------------------------------
 // X (short side S as rows, padded to 32; long side L padded to 32) and A stay in LDS in the split format, rows 32 bytes longer
 // than their values so that neighbouring rows do not share banks.  Per step: A = X X^T, one 16 x 16 tile per wave and turn;
-// A <- a I + b A + c A A from registers once every wave has read A; X <- A X by blocks of 16 columns, each read whole into
+// A <- b A + c A A from registers once every wave has read A; X <- a X + A X by blocks of 16 columns, each read whole into
 // registers by the one wave that overwrites it.  What bounds it is latency: 15 short products behind barriers.
 constexpr int kSmallWaves = 16, kSmallSide = 128, kSmallLds = 160 * 1024 - 512;
 struct OrthoSmallArgs {
     long ldg, stride_g, ldo, stride_o;   // elements
     int rows, cols, steps;
     double eps, scale;
-    float gram[64], square[64], linear[64], unit[64], apply[64];   // factors of every step, powers of two included
+    float gram[64], square[64], linear[64], apply[64], keep[64];   // factors of every step, powers of two included
 };
 constexpr int small_row(int values) { return values * 4 + 32; }
 // Bytes of LDS, or 0 where the matrix does not fit or one workgroup would need longer than the many of the general path:
@@ -519,6 +514,16 @@ __device__ __forceinline__ void small_store4(char* row, int j, mm::v4f v) {   //
     char* p = row + (j >> 5) * 128 + (j & 31) * 2;
     *reinterpret_cast<v4h*>(p) = h;
     *reinterpret_cast<v4h*>(p + 64) = l;
+}
+
+__device__ __forceinline__ mm::v4f small_load4(const char* row, int j) {
+    typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+    const char* p = row + (j >> 5) * 128 + (j & 31) * 2;
+    const v4h h = *reinterpret_cast<const v4h*>(p), l = *reinterpret_cast<const v4h*>(p + 64);
+    mm::v4f v;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) v[x] = (float)h[x] + (float)l[x];
+    return v;
 }
 
 template <class T, int NB>   // NB: blocks of 32 of the short side
@@ -633,7 +638,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
                 const float a = Iterate<mm::Split>::load(A + (ti[x] + r) * lda, tj[x] + 4 * q + y);
-                b[x][y] = g.square[step] * b[x][y] + g.linear[step] * a + (ti[x] + r == tj[x] + 4 * q + y ? g.unit[step] : 0.0f);
+                b[x][y] = g.square[step] * b[x][y] + g.linear[step] * a;
             }
         }
         __syncthreads();
@@ -667,8 +672,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
 #pragma unroll
                 for (int k = 0; k < NB; ++k)
                     acc.add(qf[k][0], qf[k][1], small_frag_kc(A, lda, i0, k, 0, lane), small_frag_kc(A, lda, i0, k, 1, lane));
-                mm::v4f c = acc.sum();
-                c *= g.apply[step];
+                mm::v4f c = acc.sum() * g.apply[step] + small_load4(X + (i0 + r) * ldx, j0 + 4 * q) * g.keep[step];
                 if (last) {
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
@@ -697,8 +701,8 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
                 g.gram[k] = (float)f.gram[k];
                 g.square[k] = (float)f.square[k];
                 g.linear[k] = (float)f.linear[k];
-                g.unit[k] = (float)f.unit[k];
                 g.apply[k] = (float)f.apply[k];
+                g.keep[k] = (float)f.keep[k];
             }
             const int nb = (std::min(rows, cols) + 31) / 32;
             if (nb == 1) ortho_small_kernel<T, 1><<<batch, kSmallWaves * 64, (unsigned)bytes, st>>>(G, O, g);
@@ -729,17 +733,17 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
     const int s = std::min(rows, cols), l = std::max(rows, cols);
     for (int k = 0; k < steps; ++k) {
         char *from = x[k & 1], *to = x[~k & 1];
-        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, s, s, l, batch, f.gram[k], 0.0, 0.0};
+        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, s, s, l, batch, f.gram[k], 0.0};
         int rc = tall ? launch<F, F, false, false, false, true>(st, gram, batch) : launch<F, F, false, true, true, true>(st, gram, batch);
         if (rc) return rc;
         const OrthoArgs poly = {a, a, a, b, o.lda, o.lda, o.lda, o.lda, o.sa, o.sa, o.sa, o.sa, s, s, s, batch,
-                                f.square[k], f.linear[k], f.unit[k]};
+                                f.square[k], f.linear[k]};
         if ((rc = launch<F, F, false, true, true, true>(st, poly, batch))) return rc;
         const bool last = k + 1 == steps;
         const long ldd = last ? ldo * (long)sizeof(T) : o.ldx, sd = last ? stride_o * (long)sizeof(T) : o.sx;
         char* d = last ? reinterpret_cast<char*>(O) : to;
-        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, rows, cols, s, batch, f.apply[k], 0.0, 0.0}
-                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, rows, cols, s, batch, f.apply[k], 0.0, 0.0};
+        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k]}
+                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k]};
         if (tall) rc = last ? launch<F, T, true, true, true, false>(st, apply, batch) : launch<F, F, false, true, true, false>(st, apply, batch);
         else rc = last ? launch<F, T, true, true, false, false>(st, apply, batch) : launch<F, F, false, true, false, false>(st, apply, batch);
         if (rc) return rc;
