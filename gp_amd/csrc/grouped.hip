@@ -95,31 +95,31 @@ template <int BM, int CHUNK> __device__ RowTile find_tile(const int64_t* offsets
     return row_tile(first, offsets, groups, T, (long)HIGH * band + in % high, BM);
 }
 
-// p[0..7] (those j + x < N) = alpha v + beta p in the type O; vec: the row allows 16-byte stores from multiples of 8 on
-template <class O> __device__ __forceinline__ void put8(char* row, int j, int N, const float (&v)[8], float alpha, float beta, bool vec) {
+// p[0..R) (those j + x < N) = alpha v + beta p in the type O, R of them 16 bytes; vec: the row allows 16-byte stores from
+// multiples of R on
+template <class O, int R> __device__ __forceinline__ void put_run(char* row, int j, int N, const float (&v)[R], float alpha, float beta, bool vec) {
+    static_assert(R * sizeof(O) == 16, "16 bytes");
     O* p = reinterpret_cast<O*>(row) + j;
-    union { O e[8]; mm::v4i w[sizeof(O) / 2]; } u;
-    const bool whole = vec && j + 8 <= N;
+    union { O e[R]; mm::v4i w; } u;
+    const bool whole = vec && j + R <= N;
     if (beta != 0.0f) {
         if (whole) {
-#pragma unroll
-            for (int x = 0; x < (int)sizeof(O) / 2; ++x) u.w[x] = reinterpret_cast<const mm::v4i*>(p)[x];
+            u.w = *reinterpret_cast<const mm::v4i*>(p);
         } else {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) u.e[x] = j + x < N ? p[x] : (O)0.0f;
+            for (int x = 0; x < R; ++x) u.e[x] = j + x < N ? p[x] : (O)0.0f;
         }
 #pragma unroll
-        for (int x = 0; x < 8; ++x) u.e[x] = (O)(alpha * v[x] + beta * (float)u.e[x]);
+        for (int x = 0; x < R; ++x) u.e[x] = (O)(alpha * v[x] + beta * (float)u.e[x]);
     } else {
 #pragma unroll
-        for (int x = 0; x < 8; ++x) u.e[x] = (O)(alpha * v[x]);
+        for (int x = 0; x < R; ++x) u.e[x] = (O)(alpha * v[x]);
     }
     if (whole) {
-#pragma unroll
-        for (int x = 0; x < (int)sizeof(O) / 2; ++x) reinterpret_cast<mm::v4i*>(p)[x] = u.w[x];
+        *reinterpret_cast<mm::v4i*>(p) = u.w;
     } else {
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
+        for (int x = 0; x < R; ++x)
             if (j + x < N) p[x] = u.e[x];
     }
 }
@@ -136,7 +136,8 @@ __device__ __forceinline__ void store_tile(Tile& t, char* lds, char* row0, long 
             *p = (O)(be != A(0) ? al * v[0] + be * (A)*p : al * v[0]);
         });
     } else {
-        t.each_run(lds, rows, cols, [&](int i, int j, const float (&v)[8]) { put8<O>(row0 + i * ld, j, cols, v, al, be, vec); });
+        constexpr int R = 16 / (int)sizeof(O);
+        t.template each_run<R>(lds, rows, cols, [&](int i, int j, const float (&v)[R]) { put_run<O, R>(row0 + i * ld, j, cols, v, al, be, vec); });
     }
 }
 
@@ -172,6 +173,20 @@ struct GroupedDwArgs {
     int part_rows, parts;
 };
 
+// Up to 64 groups are taken by their rows, most first (equal ones in their order), so that what runs last on a nearly empty
+// chip is short: 8 groups of 4096 to 12288 rows, m = 1024 in double: 2.13 -> 2.02 ms; 16 of 256 to 768, bf16: 174 -> 171 us.
+__device__ int nth_group(const int64_t* offsets, int groups, long T, int n) {
+    if (groups > 64) return n;
+    const GroupScan s(offsets, groups, T, 0, 1);
+    const int mine = (int)s.rows, lane = threadIdx.x & 63;
+    int rank = 0;
+    for (int h = 0; h < groups; ++h) {
+        const int r = __builtin_amdgcn_readlane(mine, h);
+        rank += r > mine || (r == mine && h < lane);
+    }
+    return __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(lane < groups && rank == n)));
+}
+
 // SPLIT: few tiles and many rows.  The rows of every group are cut into parts, a workgroup sums one part into a slab of its own,
 // and grouped_dw_join_kernel adds the slabs of a group in their order: the same bits in every run.
 template <class T, class O, int B, int WR, int WC, int ST, bool DIRECT, bool SPLIT>
@@ -182,15 +197,16 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void grouped_dw_kernel(const Group
     const int mt = (g.M + B - 1) / B;
     const int n0 = (int)(blockIdx.x / mt) * B, m0 = (int)(blockIdx.x % mt) * B;
     long lo;
-    int rows;
+    int rows, group = 0;
     if (SPLIT) {
         const RowTile part = row_tile(GroupScan(g.offsets, g.groups, g.T, 0, g.part_rows), g.offsets, g.groups, g.T, blockIdx.y, g.part_rows);
         if (part.group < 0) return;
         lo = part.row0;
         rows = part.rows;
     } else {
-        lo = clamped(g.offsets, blockIdx.y, g.T);
-        const long hi = clamped(g.offsets, blockIdx.y + 1, g.T);
+        group = nth_group(g.offsets, g.groups, g.T, blockIdx.y);
+        lo = clamped(g.offsets, group, g.T);
+        const long hi = clamped(g.offsets, group + 1, g.T);
         rows = (int)(hi > lo ? hi - lo : 0);
     }
     typename Tile::OpP p = {g.Z + lo * g.ldz + n0 * (long)sizeof(T), g.ldz, min(g.N - n0, B), rows};
@@ -203,7 +219,7 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void grouped_dw_kernel(const Group
         const long ld = (long)g.M * sizeof(A);
         store_tile<A>(t, lds, g.slabs + (blockIdx.y * (long)g.N + n0) * ld + m0 * (long)sizeof(A), ld, p.rows, q.rows, 1.0, 0.0, g.M % 4 == 0);
     } else {
-        store_tile<O>(t, lds, g.C + blockIdx.y * g.stride_c + n0 * g.ldc + m0 * (long)sizeof(O), g.ldc, p.rows, q.rows, g.alpha, g.beta, g.vec);
+        store_tile<O>(t, lds, g.C + group * g.stride_c + n0 * g.ldc + m0 * (long)sizeof(O), g.ldc, p.rows, q.rows, g.alpha, g.beta, g.vec);
     }
 }
 
@@ -244,8 +260,8 @@ long row_tiles(long T, int groups, int BM) { return T / BM + (groups < T ? group
 // chip full and with one workgroup on a CU, and of prologue and epilogue.  us, measured on a full chip:
 struct TileCost { int bm, bn, slots; double step, alone, rest; };
 constexpr TileCost kCost16[] = {
-    {256, 256, 256, 1.50, 1.50, 14.0},   // one workgroup of 8 waves a CU: 1.23-1.26 PFLOP/s on 8 x 4096 x 4096 x 7168
-    {128, 128, 512, 0.95, 0.52, 3.0},    // two of 4 waves: 1.07
+    {256, 256, 256, 1.50, 1.50, 14.0},   // one workgroup of 8 waves a CU: 1.17-1.25 PFLOP/s on 8 x 4096 x 4096 x 7168
+    {128, 128, 512, 1.05, 0.52, 5.0},    // two of 4 waves: 1.00-1.07
     {64, 64, 512, 0.38, 0.25, 2.3},      // two of 4 waves, four LDS stages: 0.63
     {32, 128, 512, 0.43, 0.30, 2.0},     // a few rows a group, W in 256-byte runs (n contiguous): the read of W bounds it
     {32, 64, 768, 0.36, 0.25, 2.0}};     // the same, k contiguous: 5.0 TB/s on 32 x 2816 x 2048, 6 TB/s where W is cached
@@ -307,7 +323,8 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
 
 // The weight gradient's tile and the rows of a part (0: not split), from sizes alone: the workspace follows from it.
 struct DwPlan { int tile, part_rows; long parts; };
-DwPlan dw_plan(int elem, long groups, long T, long M, long N) {
+// (Whether it is split and into what does not depend on the results' type, so that the workspace does not either.)
+DwPlan dw_plan(int elem, int c_elem, long groups, long T, long M, long N) {
     const TileCost* c = elem == 2 ? kCost16 : elem == 4 ? kCost32 : kCost64;
     const int sizes = elem == 2 ? 3 : 2;
     const double busy = (double)std::max<long>(1, std::min(groups, T)), per = 128.0 / elem, steps = std::max(1.0, ceil(T / busy / per));
@@ -315,7 +332,10 @@ DwPlan dw_plan(int elem, long groups, long T, long M, long N) {
     DwPlan best = {0, 0, 0};
     double least = 1e300;
     for (int i = 0; i < sizes; ++i) {
-        const double t = tile_time(c[i], tiles(i) * groups, steps);
+        // Groups of unequal rows leave the large tiles of floats and doubles unevenly over the CUs where each gets a few:
+        // 512 tiles of 128 in double, groups of 4096 to 12288 rows: 2.39 ms, as 2048 tiles of 64: 2.02; equal groups: 1.97 and 2.06.
+        const double uneven = elem > 2 && i == 0 && groups > 1 && tiles(i) * groups < 4.0 * c[i].slots ? 1.2 : 1.0;
+        const double t = uneven * tile_time(c[i], tiles(i) * groups, steps);
         if (t < least) {
             least = t;
             best = {i, 0, 0};
@@ -335,6 +355,17 @@ DwPlan dw_plan(int elem, long groups, long T, long M, long N) {
             least = t;
             best = {i, (int)rows, parts};
         }
+    }
+    // 16-bit rows, one pass: the stores of a round weigh more than its steps where the groups are short.  us a round besides the
+    // steps, 16- and 32-bit results: 256-tiles 9 / 16, 128-tiles 3 / 10 (16 groups of 512 rows, 2816 x 2048: 125 / 165 and 119 / 193)
+    if (elem == 2 && !best.part_rows) {
+        const double wide = c_elem == 4 ? 7.0 : 0.0;
+        TileCost t256 = c[0], t128 = c[1];
+        t256.rest = 9.0 + wide;
+        t128.step = 0.95;
+        t128.rest = 3.0 + wide;
+        const double a = tile_time(t256, tiles(0) * groups, steps), b = tile_time(t128, tiles(1) * groups, steps);
+        if (best.tile < 2 || std::min(a, b) < least) best.tile = a < b ? 0 : 1;
     }
     return best;
 }
@@ -422,7 +453,7 @@ extern "C" int gpx_grouped_gemm_dw(int dtype, int c_dtype, int64_t groups, int64
     if (groups > 1 && stride_c < (N - 1) * ldc + M) return GPX_ERR_ARG;   // results of two groups would overlap
     if (!C || !offsets || (T > 0 && (!X || !Z))) return GPX_ERR_ARG;
     if (misaligned(X, e) || misaligned(Z, e) || misaligned(C, ec) || misaligned(offsets, 8)) return GPX_ERR_ARG;
-    const DwPlan plan = dw_plan(e, groups, T, M, N);
+    const DwPlan plan = dw_plan(e, ec, groups, T, M, N);
     if (plan.part_rows && (!work || misaligned(work, 16) || work_bytes < dw_work_bytes(plan, e, M, N))) return GPX_ERR_ARG;
     StreamDevice dev(static_cast<hipStream_t>(hip_stream));
     if (dev.status) return dev.status;
@@ -442,6 +473,6 @@ extern "C" int gpx_grouped_gemm_dw_work(int dtype, int64_t groups, int64_t T, in
     const int e = elem_bytes(dtype);
     if (!e || !work_bytes || groups < 0 || groups > kMaxGroups || T < 0 || M < 0 || N < 0 || T > kMaxExtent || M > kMaxExtent || N > kMaxExtent)
         return GPX_ERR_ARG;
-    *work_bytes = groups && T && M && N ? dw_work_bytes(dw_plan(e, groups, T, M, N), e, M, N) : 0;
+    *work_bytes = groups && T && M && N ? dw_work_bytes(dw_plan(e, e, groups, T, M, N), e, M, N) : 0;
     return GPX_OK;
 }

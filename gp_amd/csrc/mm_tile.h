@@ -347,9 +347,10 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
 #pragma unroll
             for (int j = 0; j < TJ; ++j) *reinterpret_cast<v4f*>(slab + slab_at(16 * i + r, j0 + 16 * j + 4 * q)) = acc[i][j];
     }
-    // Epilogue in whole runs: f(i, j, v) for every run of 8 columns j.. of row i, i < rows, j < cols; 16-bit operands
-    template <class Put> __device__ __forceinline__ void each_run(char* lds, int rows, int cols, Put&& f) const {
-        static_assert(!SWAP, "accumulators along j");
+    // Epilogue in whole runs: f(i, j, v) for every run of RUN columns j.. of row i, i < rows, j < cols (16-bit operands).  RUN
+    // elements of the result are 16 bytes, so that neighbouring lanes store neighbouring 16 bytes.
+    template <int RUN, class Put> __device__ __forceinline__ void each_run(char* lds, int rows, int cols, Put&& f) const {
+        static_assert(!SWAP && (RUN == 4 || RUN == 8), "accumulators along j");
         float* slab = reinterpret_cast<float*>(lds);
         for (int pass = 0; pass < WR; ++pass) {
             const int ib = pass * SLAB_ROWS;
@@ -357,12 +358,12 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
             __syncthreads();
             to_slab(slab, pass);
             __syncthreads();
-            for (int e = threadIdx.x; e < SLAB_ROWS * (BN / 8); e += NT) {
-                const int il = e / (BN / 8), j = e % (BN / 8) * 8;
+            for (int e = threadIdx.x; e < SLAB_ROWS * (BN / RUN); e += NT) {
+                const int il = e / (BN / RUN), j = e % (BN / RUN) * RUN;
                 if (ib + il >= rows || j >= cols) continue;
-                union { v4f w[2]; float v[8]; } u;
-                u.w[0] = *reinterpret_cast<const v4f*>(slab + slab_at(il, j));
-                u.w[1] = *reinterpret_cast<const v4f*>(slab + slab_at(il, j + 4));
+                union { v4f w[RUN / 4]; float v[RUN]; } u;
+#pragma unroll
+                for (int x = 0; x < RUN / 4; ++x) u.w[x] = *reinterpret_cast<const v4f*>(slab + slab_at(il, j + 4 * x));
                 f(ib + il, j, u.v);
             }
         }
