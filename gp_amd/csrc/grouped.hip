@@ -77,7 +77,7 @@ __device__ RowTile row_tile(const GroupScan& first, const int64_t* offsets, int 
 // column by column.  That order is walked in chunks of CHUNK tiles, what the chip holds at a time, and since workgroups go
 // round the 8 XCDs, XCD x takes the x-th eighth of every chunk: its CUs share 8 row panels and a few column panels in their L2,
 // and all XCDs stay in one neighbourhood of X and W in the cache behind them.
-template <int BM, int CHUNK> __device__ RowTile find_tile(const int64_t* offsets, int groups, long T, int nt, int& col) {
+template <int BM, int CHUNK, int HIGH = 8> __device__ RowTile find_tile(const int64_t* offsets, int groups, long T, int nt, int& col) {
     const GroupScan first(offsets, groups, T, 0, BM);
     long total = __shfl(first.sum, 63, 64);
     for (int g0 = 64; g0 < groups; g0 += 64) total += __shfl(GroupScan(offsets, groups, T, g0, BM).sum, 63, 64);
@@ -87,7 +87,6 @@ template <int BM, int CHUNK> __device__ RowTile find_tile(const int64_t* offsets
     if (start >= all) return {-1, 0, 0};
     const unsigned in_chunk = here * xcd / 8 + (blockIdx.x % CHUNK >> 3);
     if (in_chunk >= here * (xcd + 1) / 8) return {-1, 0, 0};
-    constexpr int HIGH = 8;
     const long o = start + in_chunk;
     const unsigned band = (unsigned)(o / (HIGH * nt)), in = (unsigned)(o - (long)band * HIGH * nt);
     const unsigned high = (unsigned)min((long)HIGH, total - (long)HIGH * band);
@@ -141,6 +140,8 @@ __device__ __forceinline__ void store_tile(Tile& t, char* lds, char* row0, long 
     }
 }
 
+constexpr int kShortSub = 8;
+
 template <class Tile> constexpr int tile_lds() { return Tile::SWAP || Tile::LDS > Tile::SLAB ? Tile::LDS : Tile::SLAB; }
 
 template <class T, int BM, int BN, int WR, int WC, int ST, bool WKC, bool DIRECT>
@@ -158,6 +159,106 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void grouped_kernel(const GroupedA
     if (DIRECT) t.run_direct(lds, p, q, g.K);
     else t.run_staged(lds, p, q, g.K);
     store_tile<T>(t, lds, g.Y + rt.row0 * g.ldy + n0 * (long)sizeof(T), g.ldy, rt.rows, cols, g.alpha, g.beta, g.vec);
+}
+
+// Short k (at most 512 bytes of it: inputs of a few dozen dimensions) in floats and doubles, where the result is most of the
+// traffic: one workgroup takes its 64 columns of W into registers for all of k (as fragments, once through LDS) and walks
+// SUB tiles of 32 rows.  Per tile one wait and one barrier: the rows of the next tile arrive while this one is multiplied,
+// and the stores of this one leave while the next is.  Four workgroups a CU (32 KB of LDS each): the products of one cover
+// the waits of the others.  The columns of one group of rows go side by side over the chip (whole rows of the result at a
+// time: 232 -> 192 us at d = 20, N = 2048 in double, 5.7 TB/s).  65536 rows, d = 50, N = 1024 in double, 12 groups: 178 us (floors: 97
+// for the products, 85 for the result); as single 128-tiles 204, with W in LDS and so two workgroups a CU 193.
+template <class T, bool WKC>
+__global__ __launch_bounds__(256, 4) void grouped_short_kernel(const GroupedArgs g) {
+    constexpr int BM = 32, BN = 64, SUB = kShortSub, MOST = 4;   // MOST: K steps
+    typedef mm::Tile<T, BM, BN, 2, 2, true, WKC> Tile;
+    typedef typename Tile::OpP OpP;
+    typedef typename Tile::OpQ OpQ;
+    constexpr int TI = Tile::TI, TJ = Tile::TJ;
+    static_assert(2 * OpP::BYTES <= OpQ::BYTES, "the rows of two tiles take the place of W");
+    __shared__ __attribute__((aligned(128))) char lds[MOST * OpQ::BYTES];
+    int col = 0;
+    const RowTile rt = find_tile<BM * SUB, 1024, 1>(g.offsets, g.groups, g.T, (g.N + BN - 1) / BN, col);
+    if (rt.group < 0) return;
+    const int n0 = col * BN, cols = min(g.N - n0, BN);
+    const int steps = (g.K + OpP::BK - 1) / OpP::BK, last = g.K - (steps - 1) * OpP::BK;
+    const int halves = last * 2 <= OpP::BK ? 1 : 2;   // of the last step
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i0 = wave / 2 * (BM / 2), j0 = wave % 2 * (BN / 2);
+    const unsigned at = (unsigned)reinterpret_cast<unsigned long long>((__attribute__((address_space(3))) char*)lds);
+    const OpQ q = {g.W + rt.group * g.stride_w + (WKC ? n0 * g.ldw : n0 * (long)sizeof(T)), g.ldw, cols, g.K};
+    for (int s = 0; s < steps; ++s) q.issue(at + s * OpQ::BYTES, q.lanes(s + 1 < steps ? OpQ::BK : last), s);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    mm::v4i w[MOST][2][TJ];
+#pragma unroll
+    for (int s = 0; s < MOST; ++s) {
+        if (s >= steps) break;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) w[s][kk][j] = mm::frag<T, BN, WKC>(lds + s * OpQ::BYTES, j0 + 16 * j, kk, lane);
+    }
+    const int tiles = (rt.rows + BM - 1) / BM;
+    auto fetch = [&](int t) {
+        const OpP p = {g.X + (rt.row0 + t * BM) * g.ldx, g.ldx, min(rt.rows - t * BM, BM), g.K};
+        for (int s = 0; s < steps; ++s) p.issue(at + ((t & 1) * MOST + s) * OpP::BYTES, p.lanes(s + 1 < steps ? OpP::BK : last), s);
+    };
+    constexpr int STORES = TI * TJ * 4;   // of this wave, of a whole tile
+    bool counted = false;                 // the stores behind the last fetch are exactly these
+    const typename Tile::one alpha = (typename Tile::one)g.alpha;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // W is in every wave's registers
+    fetch(0);
+    if (tiles > 1) fetch(1);
+    for (int t = 0; t < tiles; ++t) {
+        const int rows = min(rt.rows - t * BM, BM);
+        // Tile t is here.  Vector memory operations retire in order: the stores of tile t - 1 and the fetch of tile t + 1, issued
+        // behind the fetch that is waited for, may stay on their way.
+        if (!counted) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else if (steps == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(STORES + OpP::NL) : "memory");
+        else if (steps == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(STORES + 2 * OpP::NL) : "memory");
+        else if (steps == 3) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(STORES + 3 * OpP::NL) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(STORES + 4 * OpP::NL) : "memory");
+        Tile m;
+        m.clear();
+#pragma unroll
+        for (int s = 0; s < MOST; ++s) {
+            if (s >= steps) break;
+            const char* sp = lds + ((t & 1) * MOST + s) * OpP::BYTES;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                if (kk == 1 && s + 1 == steps && halves == 1) break;
+#pragma unroll
+                for (int i = 0; i < TI; ++i) {
+                    const mm::v4i p = mm::frag<T, BM, true>(sp, i0 + 16 * i, kk, lane);
+#pragma unroll
+                    for (int j = 0; j < TJ; ++j) m.acc[i][j] = mm::mma<T>(p, w[s][kk][j], m.acc[i][j]);
+                }
+            }
+        }
+        char* y = g.Y + (rt.row0 + t * BM) * g.ldy + n0 * (long)sizeof(T);
+        const bool whole = rows == BM && cols == BN && g.beta == 0.0;
+        if (whole) {
+            // one store instruction per element of a fragment, written out so that their number is known; past the L2, which
+            // the result would only sweep
+            const unsigned long long to = reinterpret_cast<unsigned long long>(y);
+            unsigned long long base = (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)to) |
+                                      (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(to >> 32)) << 32;
+            mm::settle(base);
+            m.each([=](int i, int j, const typename Tile::one* v, auto) {
+                const unsigned long long at_y = base;
+                const unsigned off = (unsigned)(i * g.ldy) + j * (unsigned)sizeof(T);
+                const typename Tile::one o = alpha * v[0];   // (also what the matrix instruction's result has to pass before a store)
+                if constexpr (sizeof(T) == 8) asm volatile("global_store_dwordx2 %0, %1, %2 nt" ::"v"(off), "v"(o), "s"(at_y) : "memory");
+                else asm volatile("global_store_dword %0, %1, %2 nt" ::"v"(off), "v"(o), "s"(at_y) : "memory");
+            });
+        } else {
+            store_tile<T>(m, lds, y, g.ldy, rows, cols, g.alpha, g.beta, g.vec);
+        }
+        counted = whole && t + 2 < tiles;
+        if (t + 2 < tiles) {
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // nobody reads tile t any more
+            fetch(t + 2);
+        }
+    }
 }
 
 struct GroupedDwArgs {
@@ -310,6 +411,12 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
             case 3: go(Int<32>{}, Int<128>{}, Int<1>{}, Int<4>{}, Int<4>{}); break;
             default: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<4>{});
         }
+    } else if (const long units = row_tiles(g.T, g.groups, 32 * kShortSub) * ((g.N + 63) / 64);
+               direct && g.K * (long)sizeof(T) <= 512 && 32 * g.ldy < (long)mm::kRange && g.K > 0 && units >= 512 && units < (1L << 31) - 512) {
+        // (fewer workgroups than slots on the chip: no better than single tiles)
+        const unsigned grid = (unsigned)((units + 7) / 8 * 8);
+        if (w_kc) grouped_short_kernel<T, true><<<grid, 256, 0, st>>>(g);
+        else grouped_short_kernel<T, false><<<grid, 256, 0, st>>>(g);
     } else {
         switch (best_of(sizeof(T) == 4 ? kCost32 : kCost64, 3, -1)) {
             case 0: go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}); break;

@@ -126,6 +126,11 @@ template <class T> __device__ __forceinline__ v4i load_chunk(const char* p, int 
     return v;
 }
 
+// Scalar registers that a vector instruction may have written (readfirstlane) must be five wait states old before a memory
+// instruction reads them.  The compiler sees to that for its own instructions, not for those in inline assembly: the value
+// passes through this between the two.
+template <class S> __device__ __forceinline__ void settle(S& s) { asm volatile("s_nop 4" : "+s"(s)); }
+
 constexpr unsigned kRange = 0x7fff0000u;     // bytes that the lane offsets of one K step may span (checked by the host)
 constexpr unsigned kOutside = 0x7fff8000u;   // an offset behind them
 
@@ -197,8 +202,9 @@ template <class F, int ROWS, bool KC, int NT> struct Operand {
     }
     __device__ __forceinline__ void issue(unsigned lds_addr, const Lanes& l, int step) const {
         const unsigned long long a = reinterpret_cast<unsigned long long>(base) + (unsigned long long)step * (KC ? 128 : BK * ld);
-        const v4i rsrc = {__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff)),
-                          (int)kRange, 0x00027000};
+        v4i rsrc = {__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff)),
+                    (int)kRange, 0x00027000};
+        settle(rsrc);
         const unsigned wave_addr = __builtin_amdgcn_readfirstlane(lds_addr + (threadIdx.x >> 6) * 1024);
 #pragma unroll
         for (int it = 0; it < NL; ++it)   // lane l of the wave writes the 16 bytes at M0 + 16 l
@@ -241,7 +247,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
         return wave / WC * (BM / WR) < rows_p && wave % WC * (BN / WC) < rows_q;   // (split, k strided: twice the rows, never less)
     }
     // halves: 1 if the second 64 bytes of k are all zeros (the end of K)
-    __device__ __forceinline__ void multiply(const char* s, int halves = 2) {
+    __device__ __forceinline__ void multiply(const char* sp, const char* sq, int halves = 2) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const int i0 = wave / WC * (BM / WR), j0 = wave % WC * (BN / WC);
         if constexpr (Stored<F>::split) {
@@ -249,12 +255,12 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
             v4i qh[TJ], ql[TJ];
 #pragma unroll
             for (int j = 0; j < TJ; ++j) {
-                qh[j] = frag_split<BN, QKC>(s + OpP::BYTES, j0 + 16 * j, 0, lane);
-                ql[j] = frag_split<BN, QKC>(s + OpP::BYTES, j0 + 16 * j, 1, lane);
+                qh[j] = frag_split<BN, QKC>(sq, j0 + 16 * j, 0, lane);
+                ql[j] = frag_split<BN, QKC>(sq, j0 + 16 * j, 1, lane);
             }
 #pragma unroll
             for (int i = 0; i < TI; ++i) {
-                const v4i ph = frag_split<BM, PKC>(s, i0 + 16 * i, 0, lane), pl = frag_split<BM, PKC>(s, i0 + 16 * i, 1, lane);
+                const v4i ph = frag_split<BM, PKC>(sp, i0 + 16 * i, 0, lane), pl = frag_split<BM, PKC>(sp, i0 + 16 * i, 1, lane);
 #pragma unroll
                 for (int j = 0; j < TJ; ++j) acc[i][j] = mma<T>(ql[j], ph, acc[i][j]);
 #pragma unroll
@@ -269,9 +275,9 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
             if (kk >= halves) break;
             v4i fp[TI], fq[TJ];
 #pragma unroll
-            for (int i = 0; i < TI; ++i) fp[i] = frag<T, BM, PKC>(s, i0 + 16 * i, kk, lane);
+            for (int i = 0; i < TI; ++i) fp[i] = frag<T, BM, PKC>(sp, i0 + 16 * i, kk, lane);
 #pragma unroll
-            for (int j = 0; j < TJ; ++j) fq[j] = frag<T, BN, QKC>(s + OpP::BYTES, j0 + 16 * j, kk, lane);
+            for (int j = 0; j < TJ; ++j) fq[j] = frag<T, BN, QKC>(sq, j0 + 16 * j, kk, lane);
 #pragma unroll
             for (int i = 0; i < TI; ++i)
 #pragma unroll
@@ -301,7 +307,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
             q.stash(st + OpP::BYTES, rq);
             if (s + 1 < steps) load(s + 1);
             __syncthreads();   // also: nobody reads the other stage any more when the next step writes it
-            if (busy) multiply(st);
+            if (busy) multiply(st, st + OpP::BYTES);
         }
     }
     // K loop on direct loads, STAGES LDS stages: while step s is multiplied, steps s + 1 .. s + STAGES - 1 are on their way
@@ -328,7 +334,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
             if (STAGES > 2 && s + STAGES - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(AHEAD) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (s + STAGES - 1 < steps) issue(s + STAGES - 1, into);
-            if (busy) multiply(lds + stage * STAGE, s >= full && rest * 2 <= BK ? 1 : 2);
+            if (busy) multiply(lds + stage * STAGE, lds + stage * STAGE + OpP::BYTES, s >= full && rest * 2 <= BK ? 1 : 2);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             into = into + 1 == STAGES ? 0 : into + 1;
         }
