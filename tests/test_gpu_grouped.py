@@ -116,6 +116,47 @@ def test_grouped_gemm_dw(dtype, out32, shape, frame):
         assert untouched(flat, out)
 
 
+RAGGED = [int(v) for v in np.random.RandomState(3).randint(0, 170, 70)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("w_kc", [True, False], ids=["kc", "nc"])
+@pytest.mark.parametrize("sizes,n,k", [(RAGGED, 2104, 72), ([9000, 0, 7001, 3999], 1304, 64), ([5000, 300], 264, 520), ([700] * 9, 2056, 136),
+                                       ([200] * 40, 520, 264)], ids=["g70", "g4", "g2", "g9", "g40"])
+def test_grouped_gemm_on_a_full_chip(dtype, w_kc, sizes, n, k):
+    """More tiles than the chip holds at a time, in every tile size and order, more than 64 groups."""
+    lib = _lib()
+    first, tail = 3, 9
+    rows = first + sum(sizes) + tail
+    x, w = data(1, dtype, rows, k), data(2, dtype, len(sizes), *((n, k) if w_kc else (k, n)))
+    off = table(sizes, first)
+    flat, out = framed(torch.full((rows, n), 5.0, dtype=dtype, device="cuda"), 8, 16)
+    lib.grouped_gemm(x, w, off, out, w_kc=w_kc)
+    want, tol = oracle.grouped(x, w, off.tolist(), torch.full((rows, n), 5.0, dtype=dtype, device="cuda"), w_kc)
+    check(out, want, tol)
+    assert untouched(flat, out)
+    c = lib.grouped_gemm_dw(x, out, off, torch.empty(len(sizes), n, k, dtype=dtype, device="cuda"), alpha=0.25)
+    check(c, *oracle.grouped_dw(x, out, off.tolist(), torch.zeros_like(c), alpha=0.25))
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32], ids=str)
+@pytest.mark.parametrize("w_kc", [True, False], ids=["kc", "nc"])
+@pytest.mark.parametrize("sizes,n,k", [([20000, 0, 31, 15000, 4997], 256, 50), ([33, 40000], 1000, 8), ([30001, 9000], 264, 64), ([40000, 1], 320, 32),
+                                       ([513] * 80, 256, 20)], ids=str)
+def test_short_k(dtype, w_kc, sizes, n, k):
+    """k of at most 512 bytes and many rows: inputs of a few dozen dimensions."""
+    lib = _lib()
+    k += k if dtype == torch.float32 else 0
+    rows = 2 + sum(sizes) + 7
+    x, w = framed(data(1, dtype, rows, k), 8, 16)[1], data(2, dtype, len(sizes), *((n, k) if w_kc else (k, n)))
+    off, old = table(sizes, 2), data(3, dtype, rows, n)
+    for alpha, beta in ((1.0, 0.0), (-0.5, 2.0)):
+        flat, out = framed(old, 8, 16)
+        lib.grouped_gemm(x, w, off, out, w_kc=w_kc, alpha=alpha, beta=beta)
+        check(out, *oracle.grouped(x, w, off.tolist(), old, w_kc, alpha, beta), what=(alpha, beta))
+        assert torch.equal(out[:2], old[:2]) and torch.equal(out[rows - 7:], old[rows - 7:]) and untouched(flat, out)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("sizes,n,k", [([9000], 24, 40), ([1, 6000, 0, 2049, 700], 65, 130), ([0, 0, 5000, 0], 130, 17), ([64] * 70 + [8192], 16, 16),
                                        ([20000, 3], 200, 264)], ids=str)
