@@ -136,6 +136,9 @@ constexpr unsigned kOutside = 0x7fff8000u;   // an offset behind them
 
 // what a type is stored as, and the values of k in a step
 template <class T> struct Stored { typedef T type; static constexpr int BK = step_k<T>(), WIDE = 1; static constexpr bool split = false; };
+// the first plane alone, as an ordinary 16-bit matrix: products of values rounded to 11 bits
+struct Rounded {};
+template <> struct Stored<Rounded> : Stored<_Float16> {};
 template <> struct Stored<Split> { typedef _Float16 type; static constexpr int BK = 32, WIDE = 2; static constexpr bool split = true; };
 
 template <class F, int ROWS, bool KC, int NT> struct Operand {

@@ -107,11 +107,16 @@ __global__ __launch_bounds__(256) void ortho_normalize_kernel(const T* G, long l
 }
 
 // ---- the iterates ------------------------------------------------------------------------------------------------
-// Double matrices stay in double.  All others are iterated in the split format, two f16 planes under one power of two per
+// Double matrices stay in double.  Floats and f16 are iterated in the split format, two f16 planes under one power of two per
 // matrix and step: 22 bits of every value, the accumulators and all sums in 32.  One f16 product is 16 times the rate of a
 // product of floats here, the three that the split needs leave a factor of five.  The host bounds the singular values of
 // every iterate from the coefficients and places the largest possible element at 2^15: nothing overflows, and the smallest
 // step of the second plane is 2^-39 of that bound.
+// bf16: X is kept as the same two planes, but apart, and the products take the first one only, values rounded to 11 bits, one
+// matrix product instead of three and half the bytes.  That rounding is an eighth of the one that the bf16 matrix itself has
+// behind it, and the result is rounded to 8 bits; a X, where X's own bits count, is formed from both planes.
+// 16 matrices of 1024 x 2816: 2.61 -> 1.45 ms; off from 64 bits by 2.1e-3, of which 1.7e-3 is the rounding of the result; half a step
+// of the input moves the result by 4e-3 (by 4e-2 where the singular values span five orders of magnitude: 1.8e-3 here).
 template <class F> struct Iterate;
 // v = h + l.  The compiler may form a converted product in one rounding and the product itself in two; h has to be one value
 // for both planes (told apart at ties, the planes would disagree by a step of the first one).
@@ -122,13 +127,13 @@ __device__ __forceinline__ void split(float v, _Float16& h, _Float16& l) {
     l = (_Float16)(v - (float)h);
 }
 template <> struct Iterate<double> {
-    static constexpr int PAD = 2;
+    static constexpr int PAD = 2, PLANES = 1;
     __device__ static void store(char* row, int j, double v) { reinterpret_cast<double*>(row)[j] = v; }
     __device__ static double load(const char* row, int j) { return reinterpret_cast<const double*>(row)[j]; }
     static long bytes(long cols) { return cols * 8; }
 };
 template <> struct Iterate<mm::Split> {
-    static constexpr int PAD = 32;
+    static constexpr int PAD = 32, PLANES = 1;
     __device__ static long at(int j) { return (long)(j >> 5) * 64 + (j & 31); }
     __device__ static void store(char* row, int j, float v) {
         _Float16* p = reinterpret_cast<_Float16*>(row) + at(j);
@@ -140,7 +145,7 @@ template <> struct Iterate<mm::Split> {
     }
     static long bytes(long cols) { return cols * 4; }
     // eight neighbours from column j on, j a multiple of 8
-    __device__ static void store8(char* row, int j, const float (&v)[8]) {
+    __device__ static void store8(char* row, long, int j, const float (&v)[8]) {
         mm::v8h h, l;
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
@@ -153,9 +158,33 @@ template <> struct Iterate<mm::Split> {
         *reinterpret_cast<mm::v8h*>(p) = h;
         *reinterpret_cast<mm::v8h*>(p + 32) = l;
     }
-    __device__ static void add8(const char* row, int j, float by, float (&v)[8]) {   // v += by * row
+    __device__ static void add8(const char* row, long, int j, float by, float (&v)[8]) {   // v += by * row
         const _Float16* p = reinterpret_cast<const _Float16*>(row) + at(j);
         const mm::v8h h = *reinterpret_cast<const mm::v8h*>(p), l = *reinterpret_cast<const mm::v8h*>(p + 32);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] += by * ((float)h[x] + (float)l[x]);
+    }
+};
+template <> struct Iterate<mm::Rounded> {
+    static constexpr int PAD = 8, PLANES = 2;
+    static long bytes(long cols) { return cols * 2; }
+    // lo: bytes from the first plane to the second, 0 where there is none (the square factors)
+    __device__ static void store8(char* row, long lo, int j, const float (&v)[8]) {
+        mm::v8h h, l;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            _Float16 a, b;
+            split(v[x], a, b);
+            h[x] = a;
+            l[x] = b;
+        }
+        *reinterpret_cast<mm::v8h*>(row + j * 2) = h;
+        if (lo) *reinterpret_cast<mm::v8h*>(row + lo + j * 2) = l;
+    }
+    __device__ static void add8(const char* row, long lo, int j, float by, float (&v)[8]) {
+        const mm::v8h h = *reinterpret_cast<const mm::v8h*>(row + j * 2);
+        mm::v8h l = {};
+        if (lo) l = *reinterpret_cast<const mm::v8h*>(row + lo + j * 2);
 #pragma unroll
         for (int x = 0; x < 8; ++x) v[x] += by * ((float)h[x] + (float)l[x]);
     }
@@ -165,17 +194,17 @@ template <class F> int padded(int cols) { return (cols + Iterate<F>::PAD - 1) / 
 template <class T, class F>
 __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ G, long ldg, long stride_g, int rows, int cols, int pcols,
                                                           const double* __restrict__ part, int parts, double eps, double scale, char* __restrict__ X,
-                                                          long ldx, long stride_x) {
+                                                          long ldx, long stride_x, long lo) {
     const Factor by(scale / (norm_of(part + blockIdx.y * kParts, parts) + eps));
     each_run(rows, pcols, blockIdx.x * 256L + threadIdx.x, gridDim.x * 256L, [&](int r, int c) {
         T v[8];
         load_run(G + blockIdx.y * stride_g + r * ldg + c, cols - c, v);
         char* x = X + blockIdx.y * stride_x + r * ldx;
-        if constexpr (mm::Stored<F>::split) {
+        if constexpr (!__is_same(F, double)) {
             float w[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = by.times((float)v[e]);
-            Iterate<F>::store8(x, c, w);
+            Iterate<F>::store8(x, lo, c, w);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -189,6 +218,7 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ 
 struct OrthoArgs {
     const char* P; const char* Q; const char* E; char* D;
     long ldp, ldq, lde, ldd, sp, sq, se, sd;   // bytes
+    long loe, lod;                             // from the first plane of E and D to the second, where there is one
     int I, J, K, batch;
     double c1, c2;
 };
@@ -198,7 +228,7 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
     typedef typename Tile::one one;
     constexpr int W = mm::Stored<F>::WIDE * (int)sizeof(typename Tile::T);   // bytes per value
     constexpr int WE = mm::Stored<F>::WIDE;
-    constexpr int LDS = mm::Stored<F>::split && Tile::SLAB > Tile::LDS ? Tile::SLAB : Tile::LDS;
+    constexpr int LDS = !Tile::SWAP && Tile::SLAB > Tile::LDS ? Tile::SLAB : Tile::LDS;
     __shared__ __attribute__((aligned(128))) char lds[LDS];
     // Bands of eight tile rows, column by column, matrix after matrix; XCD x takes the x-th eighth of every chunk of
     // workgroups that the chip holds at a time, so that its CUs share eight row panels and a few column panels in their L2.
@@ -245,7 +275,7 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
     const one c1 = (one)g.c1, c2 = (one)g.c2;
     const char* E = g.E + mat * g.se;
     char* D = g.D + mat * g.sd;
-    if constexpr (mm::Stored<F>::split) {
+    if constexpr (!Tile::SWAP) {
         // Through LDS, one wave row of the tile at a time, so that planes are read and written in runs of 16 bytes, the mirrored
         // tile too (single elements from the accumulators: 90 us for a 256 x 256 tile, most of it the mirrored stores).
         float* slab = reinterpret_cast<float*>(lds);
@@ -265,7 +295,7 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
                     v[x] = c1 * lo[x];
                     v[4 + x] = c1 * hi[x];
                 }
-                if (c2 != 0.0f) Iterate<F>::add8(E + i * g.lde, j, c2, v);
+                if (c2 != 0.0f) Iterate<F>::add8(E + i * g.lde, g.loe, j, c2, v);
                 if constexpr (LAST) {
                     O* d = reinterpret_cast<O*>(D + i * g.ldd) + j;
                     typedef O o8 __attribute__((ext_vector_type(8)));
@@ -280,7 +310,7 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
                             if (j + x < g.J) d[x] = (O)v[x];
                     }
                 } else {
-                    Iterate<F>::store8(D + i * g.ldd, j, v);
+                    Iterate<F>::store8(D + i * g.ldd, g.lod, j, v);
                 }
             }
             if (SYM && ti != tj) {   // D(j, i): E is symmetric to the bit, so both triangles are
@@ -292,8 +322,8 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
                     float v[8];
 #pragma unroll
                     for (int x = 0; x < 8; ++x) v[x] = c1 * slab[Tile::slab_at(il + x, jl)];
-                    if (c2 != 0.0f) Iterate<F>::add8(E + j * g.lde, i, c2, v);
-                    Iterate<F>::store8(D + j * g.ldd, i, v);
+                    if (c2 != 0.0f) Iterate<F>::add8(E + j * g.lde, g.loe, i, c2, v);
+                    Iterate<F>::store8(D + j * g.ldd, g.lod, i, v);
                 }
             }
         }
@@ -321,7 +351,7 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
 
 struct OrthoWork {   // offsets and strides in bytes; rows of the iterates padded to whole blocks
     long part, x[2], a, b, total;
-    long ldx, sx, lda, sa;
+    long ldx, sx, lda, sa, lo;   // lo: from the first plane of X to the second
 };
 // Rows of a power of two of bytes would meet in few memory channels: the K step of a tile reads 128 bytes of every row.
 template <class F> long row_bytes(int cols) {
@@ -338,14 +368,17 @@ template <class F> OrthoWork ortho_work_of(long batch, int rows, int cols) {
     o.sa = o.lda * s;
     o.part = 0;
     o.x[0] = up(batch * kParts * 8);
-    o.x[1] = o.x[0] + up(batch * o.sx);
-    o.a = o.x[1] + up(batch * o.sx);
+    o.lo = Iterate<F>::PLANES == 2 ? up(batch * o.sx) : 0;
+    o.x[1] = o.x[0] + Iterate<F>::PLANES * up(batch * o.sx);
+    o.a = o.x[1] + Iterate<F>::PLANES * up(batch * o.sx);
     o.b = o.a + up(batch * o.sa);
     o.total = o.b + up(batch * o.sa);
     return o;
 }
 OrthoWork ortho_work(int dtype, long batch, int rows, int cols) {
-    return dtype == GPX_F64 ? ortho_work_of<double>(batch, rows, cols) : ortho_work_of<mm::Split>(batch, rows, cols);
+    return dtype == GPX_F64    ? ortho_work_of<double>(batch, rows, cols)
+           : dtype == GPX_BF16 ? ortho_work_of<mm::Rounded>(batch, rows, cols)
+                               : ortho_work_of<mm::Split>(batch, rows, cols);
 }
 
 // The tile of one product of split matrices, by the time it takes: rounds of workgroups over the 256 CUs, each of them K / 32
@@ -353,16 +386,20 @@ OrthoWork ortho_work(int dtype, long batch, int rows, int cols) {
 // a CU) 2.3 / 20, 192 (one of 8) 1.65 / 10, 128 (two of 4; alone on its CU) 1.4 (0.85) / 8, 64 (two of 4, four LDS stages: a
 // grid that does not fill the chip waits for memory more than for the matrix cores) 0.55 (0.36) / 4.  Rounds decide: the 136
 // lower 256-tiles of a 4096 x 4096 Gram matrix take as long as all 256, its 253 lower 192-tiles 0.7 of that.
-enum TileChoice { TILE256, TILE192, TILE128, TILE64 };
-TileChoice choose_tile(bool sym, int I, int J, int K, int batch) {
-    struct { int b; double step, step_alone, rest; } t[4] = {{256, 2.3, 2.3, 20.0}, {192, 1.65, 1.65, 10.0}, {128, 1.4, 0.85, 8.0}, {64, 0.55, 0.36, 4.0}};
+// Products of rounded values: K / 64 steps of 1.5 / 14, 0.95 (0.52) / 5, 0.38 (0.25) / 3, no 192.
+enum TileChoice { TILE256, TILE128, TILE64, TILE192 };
+TileChoice choose_tile(bool split, bool sym, int I, int J, int K, int batch) {
+    struct Cost { int b; double step, step_alone, rest; };
+    static const Cost of_split[4] = {{256, 2.3, 2.3, 20.0}, {128, 1.4, 0.85, 8.0}, {64, 0.55, 0.36, 4.0}, {192, 1.65, 1.65, 10.0}};
+    static const Cost of_rounded[3] = {{256, 1.5, 1.5, 14.0}, {128, 0.95, 0.52, 5.0}, {64, 0.38, 0.25, 3.0}};
+    const Cost* t = split ? of_split : of_rounded;
     int best = 0;
     double least = 1e300;
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < (split ? 4 : 3); ++c) {
         const double it = (I + t[c].b - 1) / t[c].b, jt = (J + t[c].b - 1) / t[c].b;
         const double tiles = (sym ? it * (it + 1) / 2 : it * jt) * batch, slots = t[c].b >= 192 ? 256.0 : 512.0;
         const double step = tiles <= 256.0 ? t[c].step_alone : t[c].step;
-        const double cost = ceil(tiles / slots) * (step * ((K + 31) / 32) + t[c].rest);
+        const double cost = ceil(tiles / slots) * (step * (split ? (K + 31) / 32 : (K + 63) / 64) + t[c].rest);
         if (cost < least) {
             least = cost;
             best = c;
@@ -384,12 +421,12 @@ template <class F, class O, bool LAST, bool PKC, bool QKC, bool SYM> int launch(
         }
         ortho_mm_kernel<F, O, LAST, B, WR, WC, ST, PKC, QKC, SYM><<<(unsigned)grid, WR * WC * 64, 0, st>>>(g);
     };
-    if constexpr (mm::Stored<F>::split) {
-        const TileChoice c = choose_tile(SYM, g.I, g.J, g.K, batch);
+    if constexpr (!__is_same(F, double)) {
+        const TileChoice c = choose_tile(mm::Stored<F>::split, SYM, g.I, g.J, g.K, batch);
         if (c == TILE256) GO(256, 2, 4, 2);
-        else if (c == TILE192) GO(192, 2, 4, 2);
         else if (c == TILE128) GO(128, 2, 2, 2);
-        else GO(64, 2, 2, 4);
+        else if (c == TILE64) GO(64, 2, 2, 4);
+        else if constexpr (mm::Stored<F>::split) GO(192, 2, 4, 2);
     } else {   // doubles: 64 x 64 tiles cost 4 % on a full chip and are three to four times as many; 32 x 32 where these are few
         const long it = (g.I + 63) / 64, jt = (g.J + 63) / 64;
         if ((SYM ? it * (it + 1) / 2 : it * jt) * batch >= 192) GO(64, 2, 2, 2);
@@ -430,16 +467,16 @@ double largest_quadratic(double b, double c, double top) {   // largest |b u + c
 // the factors of every step's three products, powers of two of the split format included
 struct OrthoFactors { double start, gram[64], square[64], linear[64], apply[64], keep[64]; };
 int place(double bound);
-OrthoFactors ortho_factors(bool scaled, int steps, const double* coef) {
+bool ortho_factors(bool scaled, int steps, const double* coef, OrthoFactors& f) {   // false: the iterates may leave 2^100
     constexpr double slack = 1.01;   // rounding may carry a singular value past the bound of the exact iterate
-    OrthoFactors f;
     double top = slack;              // of the singular values; |G|_F >= sigma_max
     int ex = scaled ? place(top) : 0;
     f.start = ldexp(1.0, ex);
     for (int k = 0; k < steps; ++k) {
         const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
-        top = std::max(top, 0x1p-400);
+        top = std::max(top, 0x1p-100);
         const double next = slack * largest_value(a, b, c, top);
+        if (scaled && !(std::max(next, top * largest_quadratic(b, c, top * top)) < 0x1p100)) return false;
         const int ea = scaled ? place(slack * top * top) : 0;
         const int eb = scaled ? place(slack * largest_quadratic(b, c, top * top)) : 0;
         const int en = scaled && k + 1 < steps ? place(next) : 0;
@@ -453,7 +490,7 @@ OrthoFactors ortho_factors(bool scaled, int steps, const double* coef) {
         top = next;
         ex = en;
     }
-    return f;
+    return true;
 }
 // exponent of the power of two that places values of at most `bound` below 2^15
 int place(double bound) { return bound > 0.0 ? 14 - std::ilogb(bound) : 14; }
@@ -567,7 +604,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
             float w[8];
 #pragma unroll
             for (int x = 0; x < 8; ++x) w[x] = by.times((float)v[x]);
-            Iterate<mm::Split>::store8(X + row * ldx, c, w);
+            Iterate<mm::Split>::store8(X + row * ldx, 0, c, w);
         }
     });
     __syncthreads();
@@ -692,11 +729,12 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
 template <class T, class F>
 int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long ldg, long stride_g, int steps, const double* coef, double eps,
                 T* O, long ldo, long stride_o, char* work) {
-    const OrthoFactors f = ortho_factors(mm::Stored<F>::split, steps, coef);
-    if constexpr (mm::Stored<F>::split) {
+    OrthoFactors f;
+    if (!ortho_factors(!__is_same(F, double), steps, coef, f)) return GPX_ERR_ARG;
+    if constexpr (!__is_same(F, double)) {
         const long bytes = small_lds(rows, cols);
         if (steps > 0 && bytes) {
-            OrthoSmallArgs g = {ldg, stride_g, ldo, stride_o, rows, cols, steps, eps, f.start, {}, {}, {}, {}, {}};
+            OrthoSmallArgs g = {ldg, stride_g, ldo, stride_o, rows, cols, steps, eps, f.start, {}, {}, {}, {}, {}};   // split planes for bf16 too
             for (int k = 0; k < steps; ++k) {
                 g.gram[k] = (float)f.gram[k];
                 g.square[k] = (float)f.square[k];
@@ -727,23 +765,23 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
     }
     char* x[2] = {work + o.x[0], work + o.x[1]};
     char *a = work + o.a, *b = work + o.b;
-    ortho_scale_kernel<T, F><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, padded<F>(cols), part, parts, eps, f.start, x[0], o.ldx, o.sx);
+    ortho_scale_kernel<T, F><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, padded<F>(cols), part, parts, eps, f.start, x[0], o.ldx, o.sx, o.lo);
     HIP_TRY(hipGetLastError());
     const bool tall = rows > cols;
     const int s = std::min(rows, cols), l = std::max(rows, cols);
     for (int k = 0; k < steps; ++k) {
         char *from = x[k & 1], *to = x[~k & 1];
-        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, s, s, l, batch, f.gram[k], 0.0};
+        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, 0, 0, s, s, l, batch, f.gram[k], 0.0};
         int rc = tall ? launch<F, F, false, false, false, true>(st, gram, batch) : launch<F, F, false, true, true, true>(st, gram, batch);
         if (rc) return rc;
-        const OrthoArgs poly = {a, a, a, b, o.lda, o.lda, o.lda, o.lda, o.sa, o.sa, o.sa, o.sa, s, s, s, batch,
+        const OrthoArgs poly = {a, a, a, b, o.lda, o.lda, o.lda, o.lda, o.sa, o.sa, o.sa, o.sa, 0, 0, s, s, s, batch,
                                 f.square[k], f.linear[k]};
         if ((rc = launch<F, F, false, true, true, true>(st, poly, batch))) return rc;
         const bool last = k + 1 == steps;
         const long ldd = last ? ldo * (long)sizeof(T) : o.ldx, sd = last ? stride_o * (long)sizeof(T) : o.sx;
         char* d = last ? reinterpret_cast<char*>(O) : to;
-        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k]}
-                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k]};
+        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, o.lo, o.lo, rows, cols, s, batch, f.apply[k], f.keep[k]}
+                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, o.lo, o.lo, rows, cols, s, batch, f.apply[k], f.keep[k]};
         if (tall) rc = last ? launch<F, T, true, true, true, false>(st, apply, batch) : launch<F, F, false, true, true, false>(st, apply, batch);
         else rc = last ? launch<F, T, true, true, false, false>(st, apply, batch) : launch<F, F, false, true, false, false>(st, apply, batch);
         if (rc) return rc;
@@ -797,7 +835,7 @@ extern "C" int gpx_orthogonalize(int dtype, int64_t batch, int64_t M, int64_t N,
             return ortho_typed<float, mm::Split>(st, b, r, c, static_cast<const float*>(G), ldg, stride_g, steps, table, eps,
                                              static_cast<float*>(O), ldo, stride_o, w);
         case GPX_BF16:
-            return ortho_typed<__bf16, mm::Split>(st, b, r, c, static_cast<const __bf16*>(G), ldg, stride_g, steps, table, eps,
+            return ortho_typed<__bf16, mm::Rounded>(st, b, r, c, static_cast<const __bf16*>(G), ldg, stride_g, steps, table, eps,
                                               static_cast<__bf16*>(O), ldo, stride_o, w);
         default:
             return ortho_typed<_Float16, mm::Split>(st, b, r, c, static_cast<const _Float16*>(G), ldg, stride_g, steps, table, eps,

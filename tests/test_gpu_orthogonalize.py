@@ -70,6 +70,22 @@ def test_every_element_keeps_22_bits(size):
         assert float(off.max()) <= 0.0
 
 
+@pytest.mark.parametrize("size", [(256, 256), (300, 1000), (700, 200)], ids=str)
+@pytest.mark.parametrize("spread", [0.0, 3.0, 6.0])
+def test_bfloat16_is_as_good_as_its_input(size, spread):
+    """Products of operands rounded to 11 bits: no further from the result of the exact input than half a step of a bf16 input
+    moves that, plus the rounding of the result (half a step); singular values spread over up to six orders of magnitude."""
+    lib = _lib()
+    r = min(size)
+    u, v = torch.linalg.qr(data(1, torch.float64, size[0], r).cpu())[0], torch.linalg.qr(data(2, torch.float64, size[1], r).cpu())[0]
+    g = ((u * torch.logspace(0, -spread, r, dtype=torch.float64)) @ v.T).to("cuda").to(torch.bfloat16)
+    want, _ = oracle.orthogonalize(g)
+    sign = torch.where(data(3, torch.float64, *size) < 0, -1.0, 1.0)
+    moved, _ = oracle.orthogonalize(g.double() * (1 + 2.0 ** -8 * sign))
+    off = lambda a: float(torch.linalg.norm(a.double() - want))  # noqa: E731
+    assert off(lib.orthogonalize(g, torch.empty_like(g))) <= off(moved) + 2.0 ** -8 * float(torch.linalg.norm(want))
+
+
 def test_cubic_steps_reach_the_polar_factor():
     """(1.5, -0.5, 0) converges to U V^T: the rows of the result are orthonormal."""
     lib = _lib()
@@ -184,6 +200,7 @@ def test_refusals():
         lambda: lib.orthogonalize(g, g, eps=float("nan")),
         lambda: lib.orthogonalize(g, g, coef=(float("inf"), 0.0, 0.0)),
         lambda: lib.orthogonalize(g, g[:1].expand(2, 4, 6)),
+        lambda: lib.orthogonalize(g, g, steps=20, coef=(100.0, 0.0, 0.0)),
     ):
         with pytest.raises(lib.GpxError):
             bad()
