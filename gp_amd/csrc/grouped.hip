@@ -22,7 +22,6 @@ struct GroupedArgs {
     long T;
     int groups, N, K;
     double alpha, beta;
-    int vec;   // Y's rows allow 16-byte stores
 };
 
 __device__ __forceinline__ long clamped(const int64_t* offsets, int g, long T) {
@@ -94,16 +93,15 @@ template <int BM, int CHUNK, int HIGH = 8> __device__ RowTile find_tile(const in
     return row_tile(first, offsets, groups, T, (long)HIGH * band + in % high, BM);
 }
 
-// p[0..R) (those j + x < N) = alpha v + beta p in the type O, R of them 16 bytes; vec: the row allows 16-byte stores from
-// multiples of R on
-template <class O, int R> __device__ __forceinline__ void put_run(char* row, int j, int N, const float (&v)[R], float alpha, float beta, bool vec) {
+// p[0..R) (those j + x < N) = alpha v + beta p in the type O, R of them 16 bytes, at any alignment
+template <class O, int R> __device__ __forceinline__ void put_run(char* row, int j, int N, const float (&v)[R], float alpha, float beta) {
     static_assert(R * sizeof(O) == 16, "16 bytes");
     O* p = reinterpret_cast<O*>(row) + j;
     union { O e[R]; mm::v4i w; } u;
-    const bool whole = vec && j + R <= N;
+    const bool whole = j + R <= N;
     if (beta != 0.0f) {
         if (whole) {
-            u.w = *reinterpret_cast<const mm::v4i*>(p);
+            __builtin_memcpy(&u.w, p, 16);
         } else {
 #pragma unroll
             for (int x = 0; x < R; ++x) u.e[x] = j + x < N ? p[x] : (O)0.0f;
@@ -115,7 +113,11 @@ template <class O, int R> __device__ __forceinline__ void put_run(char* row, int
         for (int x = 0; x < R; ++x) u.e[x] = (O)(alpha * v[x]);
     }
     if (whole) {
-        *reinterpret_cast<mm::v4i*>(p) = u.w;
+        // between fences: or the compiler takes what both branches store out of them, and the 16 bytes apart (165 -> 205 us for
+        // 16 weight gradients of 2816 x 2048)
+        asm volatile("" ::: "memory");
+        __builtin_memcpy(p, &u.w, 16);
+        asm volatile("" ::: "memory");
     } else {
 #pragma unroll
         for (int x = 0; x < R; ++x)
@@ -125,7 +127,7 @@ template <class O, int R> __device__ __forceinline__ void put_run(char* row, int
 
 // the tile's result: rows x cols of it at `row0`, `ld` bytes apart
 template <class O, class Tile>
-__device__ __forceinline__ void store_tile(Tile& t, char* lds, char* row0, long ld, int rows, int cols, double alpha, double beta, bool vec) {
+__device__ __forceinline__ void store_tile(Tile& t, char* lds, char* row0, long ld, int rows, int cols, double alpha, double beta) {
     typedef typename Tile::one A;
     const A al = (A)alpha, be = (A)beta;
     if constexpr (Tile::SWAP) {   // 16 neighbouring lanes store 16 neighbouring columns
@@ -136,7 +138,7 @@ __device__ __forceinline__ void store_tile(Tile& t, char* lds, char* row0, long 
         });
     } else {
         constexpr int R = 16 / (int)sizeof(O);
-        t.template each_run<R>(lds, rows, cols, [&](int i, int j, const float (&v)[R]) { put_run<O, R>(row0 + i * ld, j, cols, v, al, be, vec); });
+        t.template each_run<R>(lds, rows, cols, [&](int i, int j, const float (&v)[R]) { put_run<O, R>(row0 + i * ld, j, cols, v, al, be); });
     }
 }
 
@@ -158,7 +160,7 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void grouped_kernel(const GroupedA
     t.clear();
     if (DIRECT) t.run_direct(lds, p, q, g.K);
     else t.run_staged(lds, p, q, g.K);
-    store_tile<T>(t, lds, g.Y + rt.row0 * g.ldy + n0 * (long)sizeof(T), g.ldy, rt.rows, cols, g.alpha, g.beta, g.vec);
+    store_tile<T>(t, lds, g.Y + rt.row0 * g.ldy + n0 * (long)sizeof(T), g.ldy, rt.rows, cols, g.alpha, g.beta);
 }
 
 // Short k (at most 512 bytes of it: inputs of a few dozen dimensions) in floats and doubles, where the result is most of the
@@ -251,7 +253,7 @@ __global__ __launch_bounds__(256, 4) void grouped_short_kernel(const GroupedArgs
                 else asm volatile("global_store_dword %0, %1, %2 nt" ::"v"(off), "v"(o), "s"(at_y) : "memory");
             });
         } else {
-            store_tile<T>(m, lds, y, g.ldy, rows, cols, g.alpha, g.beta, g.vec);
+            store_tile<T>(m, lds, y, g.ldy, rows, cols, g.alpha, g.beta);
         }
         counted = whole && t + 2 < tiles;
         if (t + 2 < tiles) {
@@ -269,7 +271,6 @@ struct GroupedDwArgs {
     int M, N;   // columns of X (contiguous in C) and of Z
     int groups;
     double alpha, beta;
-    int vec;
     char* slabs;     // SPLIT: the sum over every part of `part_rows` rows, N x M each, in the accumulators' type
     int part_rows, parts;
 };
@@ -318,9 +319,9 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void grouped_dw_kernel(const Group
     else t.run_staged(lds, p, q, rows);
     if (SPLIT) {
         const long ld = (long)g.M * sizeof(A);
-        store_tile<A>(t, lds, g.slabs + (blockIdx.y * (long)g.N + n0) * ld + m0 * (long)sizeof(A), ld, p.rows, q.rows, 1.0, 0.0, g.M % 4 == 0);
+        store_tile<A>(t, lds, g.slabs + (blockIdx.y * (long)g.N + n0) * ld + m0 * (long)sizeof(A), ld, p.rows, q.rows, 1.0, 0.0);
     } else {
-        store_tile<O>(t, lds, g.C + group * g.stride_c + n0 * g.ldc + m0 * (long)sizeof(O), g.ldc, p.rows, q.rows, g.alpha, g.beta, g.vec);
+        store_tile<O>(t, lds, g.C + group * g.stride_c + n0 * g.ldc + m0 * (long)sizeof(O), g.ldc, p.rows, q.rows, g.alpha, g.beta);
     }
 }
 
@@ -394,17 +395,19 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
         const unsigned grid = (unsigned)((tiles + 7) / 8 * 8);   // as many for every XCD
         if (w_kc && direct) grouped_kernel<T, BM, BN, WR, WC, ST, true, true><<<grid, WR * WC * 64, 0, st>>>(g);
         else if (direct) grouped_kernel<T, BM, BN, WR, WC, ST, false, true><<<grid, WR * WC * 64, 0, st>>>(g);
+        else if constexpr (BM == 256) rc = GPX_ERR_STATE;   // (never chosen for rows that are not direct)
         else if (w_kc) grouped_kernel<T, BM, BN, WR, WC, 2, true, false><<<grid, WR * WC * 64, 0, st>>>(g);
         else grouped_kernel<T, BM, BN, WR, WC, 2, false, false><<<grid, WR * WC * 64, 0, st>>>(g);
     };
-    auto best_of = [&](const TileCost* c, int n, int not_this) {
-        int best = 0;
-        for (int i = 1; i < n; ++i)
+    // from: rows that have to pass through registers take 128-tiles at most (20000 x 1001 x 2003 in bf16: 166 us, 256-tiles 241)
+    auto best_of = [&](const TileCost* c, int from, int n, int not_this) {
+        int best = from;
+        for (int i = from + 1; i < n; ++i)
             if (i != not_this && time_of(c[i]) < time_of(c[best])) best = i;
         return best;
     };
     if constexpr (sizeof(T) == 2) {
-        switch (best_of(kCost16, 5, w_kc ? 3 : 4)) {
+        switch (best_of(kCost16, direct ? 0 : 1, 5, w_kc ? 3 : 4)) {
             case 0: go(Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{}); break;
             case 1: go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}); break;
             case 2: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<4>{}); break;
@@ -418,7 +421,7 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
         if (w_kc) grouped_short_kernel<T, true><<<grid, 256, 0, st>>>(g);
         else grouped_short_kernel<T, false><<<grid, 256, 0, st>>>(g);
     } else {
-        switch (best_of(sizeof(T) == 4 ? kCost32 : kCost64, 3, -1)) {
+        switch (best_of(sizeof(T) == 4 ? kCost32 : kCost64, 0, 3, -1)) {
             case 0: go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}); break;
             case 1: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{}); break;
             default: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<4>{});
@@ -492,6 +495,7 @@ template <class T, class O> int grouped_dw_typed(hipStream_t st, const GroupedDw
         if (plan.part_rows) {
             const dim3 grid((unsigned)tiles, (unsigned)plan.parts);
             if (direct) grouped_dw_kernel<T, O, B, WR, WC, ST, true, true><<<grid, WR * WC * 64, 0, st>>>(g);
+            else if constexpr (B == 256) rc = GPX_ERR_STATE;
             else grouped_dw_kernel<T, O, B, WR, WC, 2, false, true><<<grid, WR * WC * 64, 0, st>>>(g);
             const long size = (long)g.M * g.N;
             grouped_dw_join_kernel<typename mm::Acc<T>::one, O>
@@ -499,12 +503,13 @@ template <class T, class O> int grouped_dw_typed(hipStream_t st, const GroupedDw
         } else {
             const dim3 grid((unsigned)tiles, (unsigned)g.groups);
             if (direct) grouped_dw_kernel<T, O, B, WR, WC, ST, true, false><<<grid, WR * WC * 64, 0, st>>>(g);
+            else if constexpr (B == 256) rc = GPX_ERR_STATE;
             else grouped_dw_kernel<T, O, B, WR, WC, 2, false, false><<<grid, WR * WC * 64, 0, st>>>(g);
         }
     };
     if constexpr (sizeof(T) == 2) {
-        if (plan.tile == 0) go(Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{});
-        else if (plan.tile == 1) go(Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{});
+        if (plan.tile == 0 && direct) go(Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{});
+        else if (plan.tile <= 1) go(Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{});
         else go(Int<64>{}, Int<2>{}, Int<2>{}, Int<4>{});
     } else {
         if (plan.tile == 0) go(Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{});
@@ -519,9 +524,6 @@ constexpr int kMaxGroups = 65535;
 
 int elem_bytes(int dtype) { return dtype == GPX_F64 ? 8 : dtype == GPX_F32 ? 4 : dtype == GPX_BF16 || dtype == GPX_F16 ? 2 : 0; }
 bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes != 0; }
-bool aligned_rows(const void* p, long ld_bytes, long stride_bytes) {   // 16-byte stores
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld_bytes % 16 == 0 && stride_bytes % 16 == 0;
-}
 
 }  // namespace
 
@@ -538,7 +540,7 @@ extern "C" int gpx_grouped_gemm(int dtype, int w_kc, int64_t groups, int64_t T, 
     StreamDevice dev(static_cast<hipStream_t>(hip_stream));
     if (dev.status) return dev.status;
     GroupedArgs g = {static_cast<const char*>(X), static_cast<const char*>(W), static_cast<char*>(Y), offsets, ldx * e, ldw * e,
-                     stride_w * e, ldy * e, T, (int)groups, (int)N, (int)K, alpha, beta, aligned_rows(Y, ldy * e, 0)};
+                     stride_w * e, ldy * e, T, (int)groups, (int)N, (int)K, alpha, beta};
     const hipStream_t st = static_cast<hipStream_t>(hip_stream);
     switch (dtype) {
         case GPX_F64: return grouped_typed<double>(st, w_kc != 0, g);
@@ -565,7 +567,7 @@ extern "C" int gpx_grouped_gemm_dw(int dtype, int c_dtype, int64_t groups, int64
     StreamDevice dev(static_cast<hipStream_t>(hip_stream));
     if (dev.status) return dev.status;
     const GroupedDwArgs g = {static_cast<const char*>(X), static_cast<const char*>(Z), static_cast<char*>(C), offsets, ldx * e, ldz * e, ldc * ec,
-                             stride_c * ec, T, (int)M, (int)N, (int)groups, alpha, beta, aligned_rows(C, ldc * ec, stride_c * ec),
+                             stride_c * ec, T, (int)M, (int)N, (int)groups, alpha, beta,
                              static_cast<char*>(work), plan.part_rows, (int)plan.parts};
     const hipStream_t st = static_cast<hipStream_t>(hip_stream);
     switch (dtype) {

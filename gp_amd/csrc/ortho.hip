@@ -35,15 +35,8 @@ template <class Body> __device__ __forceinline__ void each_run(int rows, int col
 }
 // v = the run at p, of which `count` elements exist
 template <class T> __device__ __forceinline__ void load_run(const T* p, int count, T (&v)[8]) {
-    if (count >= 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
-        constexpr int E = 16 / (int)sizeof(T);
-#pragma unroll
-        for (int x = 0; x < 8; x += E) {
-            union { mm::v4i w; T e[E]; } u;
-            u.w = *reinterpret_cast<const mm::v4i*>(p + x);
-#pragma unroll
-            for (int y = 0; y < E; ++y) v[x + y] = u.e[y];
-        }
+    if (count >= 8) {   // at any alignment
+        __builtin_memcpy(v, p, sizeof v);
     } else {
 #pragma unroll
         for (int x = 0; x < 8; ++x) v[x] = x < count ? p[x] : (T)0.0f;
@@ -299,11 +292,13 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
                 if constexpr (LAST) {
                     O* d = reinterpret_cast<O*>(D + i * g.ldd) + j;
                     typedef O o8 __attribute__((ext_vector_type(8)));
-                    if (j + 8 <= g.J && reinterpret_cast<uintptr_t>(d) % 16 == 0) {
+                    if (j + 8 <= g.J) {   // at any alignment
                         o8 w;
 #pragma unroll
                         for (int x = 0; x < 8; ++x) w[x] = (O)v[x];
-                        *reinterpret_cast<o8*>(d) = w;
+                        asm volatile("" ::: "memory");   // keep the run in one piece
+                        __builtin_memcpy(d, &w, sizeof w);
+                        asm volatile("" ::: "memory");
                     } else {
 #pragma unroll
                         for (int x = 0; x < 8; ++x)
