@@ -147,7 +147,8 @@ template <class F, int ROWS, bool KC, int NT> struct Operand {
     static constexpr int COLS = ROWS * Stored<F>::WIDE;   // elements per k of an operand with k strided
     static constexpr int NL = ROWS * 8 / NT;   // chunks per thread
     static constexpr int BYTES = ROWS * 128;
-    static_assert(ROWS * 8 % NT == 0, "whole chunks per thread");
+    static_assert(ROWS * 8 % NT == 0 && (NT & (NT - 1)) == 0, "whole chunks per thread");
+    __device__ static __forceinline__ int tid() { return threadIdx.x & (NT - 1); }   // of the K group
     const char* base;   // element (0, 0) of the tile's rows
     long ld;            // bytes between rows (KC) or between k (otherwise)
     int rows, K;        // rows of the tile (split, k strided: elements) and extent of k that exist
@@ -169,7 +170,7 @@ template <class F, int ROWS, bool KC, int NT> struct Operand {
 #pragma unroll
         for (int it = 0; it < NL; ++it) {
             int row, k;
-            place(it * NT + (int)threadIdx.x, row, k);
+            place(it * NT + tid(), row, k);
             k += k0;
             if (KC) r[it] = load_chunk<T>(base + row * ld + (long)k * sizeof(T), row < rows ? K - k : 0);
             else r[it] = load_chunk<T>(base + k * ld + (long)row * sizeof(T), k < K ? rows - row : 0);
@@ -181,7 +182,7 @@ template <class F, int ROWS, bool KC, int NT> struct Operand {
 #pragma unroll
         for (int it = 0; it < NL; ++it) {
             int row, k;
-            place(it * NT + (int)threadIdx.x, row, k);
+            place(it * NT + tid(), row, k);
             row = min(row, rows - 1);
             k += k0;
             const char* p = KC ? base + row * ld + (long)k * sizeof(T) : base + k * ld + (long)row * sizeof(T);
@@ -197,7 +198,7 @@ template <class F, int ROWS, bool KC, int NT> struct Operand {
 #pragma unroll
         for (int it = 0; it < NL; ++it) {
             int row, k;
-            place(it * NT + (int)threadIdx.x, row, k);
+            place(it * NT + tid(), row, k);
             const unsigned at = KC ? (unsigned)(row * ld) + k * (unsigned)sizeof(T) : (unsigned)(k * ld) + row * (unsigned)sizeof(T);
             l.off[it] = row < rows && (k < k_valid || (KC && Stored<F>::split)) ? at : kOutside;
         }
@@ -208,7 +209,7 @@ template <class F, int ROWS, bool KC, int NT> struct Operand {
         v4i rsrc = {__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff)),
                     (int)kRange, 0x00027000};
         settle(rsrc);
-        const unsigned wave_addr = __builtin_amdgcn_readfirstlane(lds_addr + (threadIdx.x >> 6) * 1024);
+        const unsigned wave_addr = __builtin_amdgcn_readfirstlane(lds_addr + (tid() >> 6) * 1024);
 #pragma unroll
         for (int it = 0; it < NL; ++it)   // lane l of the wave writes the 16 bytes at M0 + 16 l
             asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(l.off[it]), "s"(rsrc),
@@ -217,7 +218,7 @@ template <class F, int ROWS, bool KC, int NT> struct Operand {
     }
     __device__ __forceinline__ void stash(char* s, const v4i (&r)[NL]) const {
 #pragma unroll
-        for (int it = 0; it < NL; ++it) *reinterpret_cast<v4i*>(s + (it * NT + (int)threadIdx.x) * 16) = r[it];
+        for (int it = 0; it < NL; ++it) *reinterpret_cast<v4i*>(s + (it * NT + tid()) * 16) = r[it];
     }
 };
 
@@ -225,7 +226,7 @@ template <class F, int ROWS, bool KC, int NT> struct Operand {
 // Waves in a WR (rows i) x WC (columns j) grid; each owns TI x TJ fragments of 16.  SWAP: the accumulator's contiguous
 // lanes run along j (doubles and floats: whole 64..128-byte runs per store); otherwise its four registers do (16-bit
 // results: 8-byte stores instead of single elements).
-template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGES = 2> struct Tile {
+template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGES = 2, int GROUPS = 1> struct Tile {
     typedef typename Stored<F>::type T;
     static constexpr int NT = WR * WC * 64;
     static constexpr int TI = BM / WR / 16, TJ = BN / WC / 16;
@@ -235,7 +236,10 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
     typedef typename Acc<T>::vec vec;
     typedef typename Acc<T>::one one;
     static constexpr int STAGE = OpP::BYTES + OpQ::BYTES;
-    static constexpr int LDS = STAGES * STAGE;
+    static constexpr int LDS = STAGES * GROUPS * STAGE;
+    static constexpr int THREADS = NT * GROUPS;
+    __device__ static __forceinline__ int wave_id() { return (threadIdx.x & (NT - 1)) >> 6; }
+    __device__ static __forceinline__ int group() { return GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT); }
     vec acc[TI][TJ];
 
     __device__ __forceinline__ void clear() {
@@ -246,12 +250,12 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
     }
     // whether any of this wave's rows and columns exist: a ragged last tile costs the matrix cores only the wave rows it has
     __device__ __forceinline__ bool has_rows(int rows_p, int rows_q) const {
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wave = __builtin_amdgcn_readfirstlane(wave_id());
         return wave / WC * (BM / WR) < rows_p && wave % WC * (BN / WC) < rows_q;   // (split, k strided: twice the rows, never less)
     }
     // halves: 1 if the second 64 bytes of k are all zeros (the end of K)
     __device__ __forceinline__ void multiply(const char* sp, const char* sq, int halves = 2) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int lane = threadIdx.x & 63, wave = wave_id();
         const int i0 = wave / WC * (BM / WR), j0 = wave % WC * (BN / WC);
         if constexpr (Stored<F>::split) {
             // (ph + pl)(qh + ql) without pl ql, which is 2^-22 of the product at most
@@ -342,14 +346,64 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
             into = into + 1 == STAGES ? 0 : into + 1;
         }
     }
+    // The same for few tiles with long sums: GROUPS sets of NT threads take the steps in turn, each with LDS stages of its own,
+    // and add their accumulators at the end in one order, the sum in group 0.  A step of a 64-tile alone on its CU costs
+    // 0.36 us, most of it waiting; four groups do four in 0.5 us.
+    __device__ __forceinline__ void run_groups(char* lds, const OpP& p, const OpQ& q, int K) {
+        static_assert(STAGES == 2 && GROUPS > 1, "two stages of every group");
+        constexpr int BK = OpP::BK;
+        const int full = K / BK, rest = K - full * BK, steps = full + (rest != 0), turns = (steps + GROUPS - 1) / GROUPS, mine = group();
+        typename OpP::Lanes lp = p.lanes(BK);
+        typename OpQ::Lanes lq = q.lanes(BK);
+        char* own = lds + mine * 2 * STAGE;
+        const unsigned at = (unsigned)reinterpret_cast<unsigned long long>((__attribute__((address_space(3))) char*)own);
+        auto issue = [&](int turn) {
+            const int s = turn * GROUPS + mine;
+            if (s >= steps) return;
+            if (s >= full) {
+                lp = p.lanes(rest);
+                lq = q.lanes(rest);
+            }
+            p.issue(at + (turn & 1) * STAGE, lp, s);
+            q.issue(at + (turn & 1) * STAGE + OpP::BYTES, lq, s);
+        };
+        const bool busy = has_rows(p.rows, q.rows);
+        if (turns) issue(0);
+        for (int t = 0; t < turns; ++t) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (t + 1 < turns) issue(t + 1);
+            const int s = t * GROUPS + mine;
+            const char* st = own + (t & 1) * STAGE;
+            if (busy && s < steps) multiply(st, st + OpP::BYTES, s >= full && rest * 2 <= BK ? 1 : 2);
+        }
+        __syncthreads();
+        vec* meet = reinterpret_cast<vec*>(lds);
+        constexpr int EACH = TI * TJ * NT;
+        static_assert((GROUPS - 1) * EACH * (int)sizeof(vec) <= LDS, "the accumulators take the place of the stages");
+        if (mine > 0) {
+#pragma unroll
+            for (int i = 0; i < TI; ++i)
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) meet[(mine - 1) * EACH + (i * TJ + j) * NT + (threadIdx.x & (NT - 1))] = acc[i][j];
+        }
+        __syncthreads();
+        if (mine == 0) {
+#pragma unroll
+            for (int g = 0; g < GROUPS - 1; ++g)
+#pragma unroll
+                for (int i = 0; i < TI; ++i)
+#pragma unroll
+                    for (int j = 0; j < TJ; ++j) acc[i][j] += meet[g * EACH + (i * TJ + j) * NT + threadIdx.x];
+        }
+    }
     // The accumulators of wave row `pass` (BM / WR rows of the tile) as floats in LDS, rows of SLAB_LD: what an epilogue that
     // reads and writes whole 16-byte runs needs.  Between barriers of the caller.
     static constexpr int SLAB_ROWS = BM / WR, SLAB_LD = BN + 4, SLAB = SLAB_ROWS * SLAB_LD * 4;
     // groups of four columns permuted by the row, so that a column of eight-row runs does not meet in one bank
     __device__ static __forceinline__ int slab_at(int row, int col) { return row * SLAB_LD + (col ^ (row >> 3 & 7) << 2); }
     __device__ __forceinline__ void to_slab(float* slab, int pass) const {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-        if (wave / WC != pass) return;
+        const int lane = threadIdx.x & 63, wave = wave_id(), r = lane & 15, q = lane >> 4;
+        if (wave / WC != pass || group() != 0) return;
         const int j0 = wave % WC * (BN / WC);
 #pragma unroll
         for (int i = 0; i < TI; ++i)
@@ -367,7 +421,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
             __syncthreads();
             to_slab(slab, pass);
             __syncthreads();
-            for (int e = threadIdx.x; e < SLAB_ROWS * (BN / RUN); e += NT) {
+            for (int e = threadIdx.x; e < SLAB_ROWS * (BN / RUN); e += THREADS) {
                 const int il = e / (BN / RUN), j = e % (BN / RUN) * RUN;
                 if (ib + il >= rows || j >= cols) continue;
                 union { v4f w[RUN / 4]; float v[RUN]; } u;
@@ -379,7 +433,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
     }
     // f(i, j, value pointer, count): count consecutive columns j.. of row i of the tile
     template <class Put> __device__ __forceinline__ void each(Put&& f) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+        const int lane = threadIdx.x & 63, wave = wave_id(), r = lane & 15, q = lane >> 4;
         const int i0 = wave / WC * (BM / WR), j0 = wave % WC * (BN / WC);
 #pragma unroll
         for (int i = 0; i < TI; ++i)

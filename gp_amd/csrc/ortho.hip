@@ -215,9 +215,9 @@ struct OrthoArgs {
     int I, J, K, batch;
     double c1, c2;
 };
-template <class F, class O, bool LAST, int B, int WR, int WC, int ST, bool PKC, bool QKC, bool SYM>
-__global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2) void ortho_mm_kernel(const OrthoArgs g) {
-    typedef mm::Tile<F, B, B, WR, WC, PKC, QKC, ST> Tile;
+template <class F, class O, bool LAST, int B, int WR, int WC, int ST, int KG, bool PKC, bool QKC, bool SYM>
+__global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) > 128 * 64 ? 1 : 2) void ortho_mm_kernel(const OrthoArgs g) {
+    typedef mm::Tile<F, B, B, WR, WC, PKC, QKC, ST, KG> Tile;
     typedef typename Tile::one one;
     constexpr int W = mm::Stored<F>::WIDE * (int)sizeof(typename Tile::T);   // bytes per value
     constexpr int WE = mm::Stored<F>::WIDE;
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
     __shared__ __attribute__((aligned(128))) char lds[LDS];
     // Bands of eight tile rows, column by column, matrix after matrix; XCD x takes the x-th eighth of every chunk of
     // workgroups that the chip holds at a time, so that its CUs share eight row panels and a few column panels in their L2.
-    constexpr int CHUNK = B > 128 ? 256 : 512;
+    constexpr int CHUNK = B > 128 || KG > 1 ? 256 : 512;
     const int it = (g.I + B - 1) / B, jt = (g.J + B - 1) / B;
     const unsigned tiles = SYM ? it * (it + 1) / 2 : it * jt, all = tiles * g.batch, start = blockIdx.x / CHUNK * CHUNK;
     if (start >= all) return;
@@ -264,7 +264,8 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
     typename Tile::OpQ q = {g.Q + mat * g.sq + (QKC ? j0 * g.ldq : j0 * (long)W), g.ldq, QKC ? min(g.J - j0, B) : min(Jp - j0, B) * WE, g.K};
     Tile t;
     t.clear();
-    t.run_direct(lds, p, q, g.K);
+    if constexpr (KG > 1) t.run_groups(lds, p, q, g.K);
+    else t.run_direct(lds, p, q, g.K);
     const one c1 = (one)g.c1, c2 = (one)g.c2;
     const char* E = g.E + mat * g.se;
     char* D = g.D + mat * g.sd;
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(WR * WC * 64, B * B / (WR * WC) > 128 * 64 ? 1 : 2)
         // Through LDS, one wave row of the tile at a time, so that planes are read and written in runs of 16 bytes, the mirrored
         // tile too (single elements from the accumulators: 90 us for a 256 x 256 tile, most of it the mirrored stores).
         float* slab = reinterpret_cast<float*>(lds);
-        constexpr int NT = WR * WC * 64, R = Tile::SLAB_ROWS;
+        constexpr int NT = Tile::THREADS, R = Tile::SLAB_ROWS;
         for (int pass = 0; pass < WR; ++pass) {
             const int ib = i0 + pass * R;
             __syncthreads();
@@ -381,18 +382,19 @@ OrthoWork ortho_work(int dtype, long batch, int rows, int cols) {
 // a CU) 2.3 / 20, 192 (one of 8) 1.65 / 10, 128 (two of 4; alone on its CU) 1.4 (0.85) / 8, 64 (two of 4, four LDS stages: a
 // grid that does not fill the chip waits for memory more than for the matrix cores) 0.55 (0.36) / 4.  Rounds decide: the 136
 // lower 256-tiles of a 4096 x 4096 Gram matrix take as long as all 256, its 253 lower 192-tiles 0.7 of that.
-// Products of rounded values: K / 64 steps of 1.5 / 14, 0.95 (0.52) / 5, 0.38 (0.25) / 3, no 192.
-enum TileChoice { TILE256, TILE128, TILE64, TILE192 };
+// Long sums on few 64-tiles: four groups of waves on one tile, 0.30 (0.13) / 6.5 (1024 x 1024: 235 -> 210 us in all, 300 x 2000: 205 -> 187).
+// Products of rounded values: K / 64 steps of 1.5 / 14, 0.95 (0.52) / 5, 0.38 (0.25) / 3, groups 0.25 (0.11) / 6, no 192.
+enum TileChoice { TILE256, TILE128, TILE64, TILE64_GROUPS, TILE192 };
 TileChoice choose_tile(bool split, bool sym, int I, int J, int K, int batch) {
     struct Cost { int b; double step, step_alone, rest; };
-    static const Cost of_split[4] = {{256, 2.3, 2.3, 20.0}, {128, 1.4, 0.85, 8.0}, {64, 0.55, 0.36, 4.0}, {192, 1.65, 1.65, 10.0}};
-    static const Cost of_rounded[3] = {{256, 1.5, 1.5, 14.0}, {128, 0.95, 0.52, 5.0}, {64, 0.38, 0.25, 3.0}};
+    static const Cost of_split[5] = {{256, 2.3, 2.3, 20.0}, {128, 1.4, 0.85, 8.0}, {64, 0.55, 0.36, 4.0}, {64, 0.30, 0.13, 6.5}, {192, 1.65, 1.65, 10.0}};
+    static const Cost of_rounded[4] = {{256, 1.5, 1.5, 14.0}, {128, 0.95, 0.52, 5.0}, {64, 0.38, 0.25, 3.0}, {64, 0.25, 0.11, 6.0}};
     const Cost* t = split ? of_split : of_rounded;
     int best = 0;
     double least = 1e300;
-    for (int c = 0; c < (split ? 4 : 3); ++c) {
+    for (int c = 0; c < (split ? 5 : 4); ++c) {
         const double it = (I + t[c].b - 1) / t[c].b, jt = (J + t[c].b - 1) / t[c].b;
-        const double tiles = (sym ? it * (it + 1) / 2 : it * jt) * batch, slots = t[c].b >= 192 ? 256.0 : 512.0;
+        const double tiles = (sym ? it * (it + 1) / 2 : it * jt) * batch, slots = t[c].b >= 192 || c == TILE64_GROUPS ? 256.0 : 512.0;
         const double step = tiles <= 256.0 ? t[c].step_alone : t[c].step;
         const double cost = ceil(tiles / slots) * (step * (split ? (K + 31) / 32 : (K + 63) / 64) + t[c].rest);
         if (cost < least) {
@@ -403,29 +405,32 @@ TileChoice choose_tile(bool split, bool sym, int I, int J, int K, int batch) {
     return (TileChoice)best;
 }
 
+template <int V> using Int = std::integral_constant<int, V>;
+
 template <class F, class O, bool LAST, bool PKC, bool QKC, bool SYM> int launch(hipStream_t st, const OrthoArgs& g, int batch) {
-#define GO(B, R, C, S) go(std::integral_constant<int, B>{}, std::integral_constant<int, R>{}, std::integral_constant<int, C>{}, std::integral_constant<int, S>{})
+#define GO(B, R, C, S, G) go(Int<B>{}, Int<R>{}, Int<C>{}, Int<S>{}, Int<G>{})
     int rc = GPX_OK;
-    auto go = [&](auto tile, auto wr, auto wc, auto stages) {
-        constexpr int B = decltype(tile)::value, WR = decltype(wr)::value, WC = decltype(wc)::value, ST = decltype(stages)::value;
+    auto go = [&](auto tile, auto wr, auto wc, auto stages, auto groups) {
+        constexpr int B = decltype(tile)::value, WR = decltype(wr)::value, WC = decltype(wc)::value, ST = decltype(stages)::value, KG = decltype(groups)::value;
         const long it = (g.I + B - 1) / B, jt = (g.J + B - 1) / B;
         const long grid = ((SYM ? it * (it + 1) / 2 : it * jt) * batch + 7) / 8 * 8;   // as many for every XCD
         if (grid >= 1L << 31) {
             rc = GPX_ERR_UNSUPPORTED;
             return;
         }
-        ortho_mm_kernel<F, O, LAST, B, WR, WC, ST, PKC, QKC, SYM><<<(unsigned)grid, WR * WC * 64, 0, st>>>(g);
+        ortho_mm_kernel<F, O, LAST, B, WR, WC, ST, KG, PKC, QKC, SYM><<<(unsigned)grid, WR * WC * 64 * KG, 0, st>>>(g);
     };
     if constexpr (!__is_same(F, double)) {
         const TileChoice c = choose_tile(mm::Stored<F>::split, SYM, g.I, g.J, g.K, batch);
-        if (c == TILE256) GO(256, 2, 4, 2);
-        else if (c == TILE128) GO(128, 2, 2, 2);
-        else if (c == TILE64) GO(64, 2, 2, 4);
-        else if constexpr (mm::Stored<F>::split) GO(192, 2, 4, 2);
+        if (c == TILE256) GO(256, 2, 4, 2, 1);
+        else if (c == TILE128) GO(128, 2, 2, 2, 1);
+        else if (c == TILE64) GO(64, 2, 2, 4, 1);
+        else if (c == TILE64_GROUPS) GO(64, 2, 2, 2, 4);
+        else if constexpr (mm::Stored<F>::split) GO(192, 2, 4, 2, 1);
     } else {   // doubles: 64 x 64 tiles cost 4 % on a full chip and are three to four times as many; 32 x 32 where these are few
         const long it = (g.I + 63) / 64, jt = (g.J + 63) / 64;
-        if ((SYM ? it * (it + 1) / 2 : it * jt) * batch >= 192) GO(64, 2, 2, 2);
-        else GO(32, 2, 2, 4);
+        if ((SYM ? it * (it + 1) / 2 : it * jt) * batch >= 192) GO(64, 2, 2, 2, 1);
+        else GO(32, 2, 2, 4, 1);
     }
 #undef GO
     HIP_TRY(hipGetLastError());
