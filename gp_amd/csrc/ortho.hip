@@ -508,13 +508,14 @@ struct OrthoSmallArgs {
     float gram[64], square[64], linear[64], apply[64], keep[64];   // factors of every step, powers of two included
 };
 constexpr int small_row(int values) { return values * 4 + 32; }
-// Bytes of LDS, or 0 where the matrix does not fit or one workgroup would need longer than the many of the general path:
+// Bytes of LDS (two: enough for a second X and A), or 0 where the matrix does not fit or one workgroup would need longer than the many of the general path:
 // 0.9 us + 1.5 us per 10^6 of S S (2 L + S) a step (128 x 128: 10 us) against 13 us there, most of it three launches.
-long small_lds(int rows, int cols) {
+long small_lds(int rows, int cols, bool& two) {
     const long s = (std::min(rows, cols) + 31) / 32 * 32, l = (std::max(rows, cols) + 31) / 32 * 32;
     if (s > kSmallSide || l > (1 << 16) || s * s * (2 * l + s) > 6500000) return 0;
-    const long bytes = s * (small_row((int)l) + small_row((int)s)) + (s == 32 ? kSmallWaves * 3 * 1024 : 0);
-    return bytes <= kSmallLds ? bytes : 0;
+    const long one = s * (small_row((int)l) + small_row((int)s)), more = s == 32 ? kSmallWaves * 3 * 1024 : 0;
+    two = 2 * one + more <= kSmallLds;
+    return two ? 2 * one + more : one + more <= kSmallLds ? one + more : 0;
 }
 __device__ __forceinline__ mm::v4i small_frag_kc(const char* m, int ld, int row0, int k32, int lo, int lane) {
     return *reinterpret_cast<const mm::v4i*>(m + (row0 + (lane & 15)) * ld + k32 * 128 + lo * 64 + (lane >> 4) * 16);
@@ -563,7 +564,9 @@ __device__ __forceinline__ mm::v4f small_load4(const char* row, int j) {
     return v;
 }
 
-template <class T, int NB>   // NB: blocks of 32 of the short side
+// NB: blocks of 32 of the short side.  TWO: room for a second X and A, so that nobody waits before writing, and two waves can
+// share a block of 16 columns (128 x 50: 21.6 -> 20.9 us, 300 of 128 x 128: 153 -> 126).
+template <class T, int NB, bool TWO>
 __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* G, T* O, const OrthoSmallArgs g) {
     extern __shared__ __attribute__((aligned(128))) char lds[];
     __shared__ double ws[kSmallWaves];
@@ -574,20 +577,29 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
     const int Lp = (L + 31) / 32 * 32;
     const int ldx = small_row(Lp), lda = small_row(Sp);
     char* X = lds;
-    char* A = lds + (long)Sp * ldx;
+    char* A = lds + (TWO ? 2L : 1L) * Sp * ldx;
+    char* X2 = TWO ? lds + (long)Sp * ldx : X;
+    char* B = TWO ? A + Sp * lda : A;
     G += blockIdx.x * g.stride_g;
     O += blockIdx.x * g.stride_o;
     double s = 0.0;
+    T first[8];   // this thread's first run stays in registers
+    bool held = false;
     each_run(g.rows, g.cols, threadIdx.x, kSmallWaves * 64, [&](int row, int c) {
         T v[8];
         load_run(G + row * g.ldg + c, g.cols - c, v);
 #pragma unroll
         for (int x = 0; x < 8; ++x) s = fma(as_double(v[x]), as_double(v[x]), s);
+        if (!held) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) first[x] = v[x];
+            held = true;
+        }
     });
 #pragma unroll
     for (int d = 32; d; d /= 2) s += __shfl_xor(s, d, 64);
     if (lane == 0) ws[wave] = s;
-    for (int e = threadIdx.x; e < Sp * ldx / 16; e += kSmallWaves * 64) reinterpret_cast<mm::v4i*>(X)[e] = mm::v4i{0, 0, 0, 0};
+    for (int e = threadIdx.x; e < (TWO ? 2 : 1) * Sp * ldx / 16; e += kSmallWaves * 64) reinterpret_cast<mm::v4i*>(X)[e] = mm::v4i{0, 0, 0, 0};
     __syncthreads();
     s = 0.0;
 #pragma unroll
@@ -595,7 +607,13 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
     const Factor by(g.scale / (sqrt(s) + g.eps));
     each_run(g.rows, g.cols, threadIdx.x, kSmallWaves * 64, [&](int row, int c) {
         T v[8];
-        load_run(G + row * g.ldg + c, g.cols - c, v);
+        if (held) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = first[x];
+            held = false;
+        } else {
+            load_run(G + row * g.ldg + c, g.cols - c, v);
+        }
         if (tall) {
 #pragma unroll
             for (int x = 0; x < 8; ++x)
@@ -618,17 +636,18 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
         ti[x] = i * 16;
         tj[x] = t * 16;
     }
-    auto store_both = [&](int i0, int j0, mm::v4f c) {
-        small_store4(A + (i0 + r) * lda, j0 + 4 * q, c);
+    auto store_both = [&](char* to, int i0, int j0, mm::v4f c) {
+        small_store4(to + (i0 + r) * lda, j0 + 4 * q, c);
         if (i0 != j0) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y) Iterate<mm::Split>::store(A + (j0 + 4 * q + y) * lda, i0 + r, c[y]);
+            for (int y = 0; y < 4; ++y) Iterate<mm::Split>::store(to + (j0 + 4 * q + y) * lda, i0 + r, c[y]);
         }
     };
     for (int step = 0; step < g.steps; ++step) {
+        mm::v4f a[TURNS], b[TURNS];   // this wave's tiles of A and of the square factor
         if constexpr (NB == 1) {
             // three tiles: every wave takes each sixteenth block of k for all of them, the sums meet in LDS behind A
-            mm::v4f* meet = reinterpret_cast<mm::v4f*>(A + Sp * lda);
+            mm::v4f* meet = reinterpret_cast<mm::v4f*>(A + (TWO ? 2 : 1) * Sp * lda);
             SmallAcc c[3];
             for (int k = wave; k < kx; k += kSmallWaves) {
                 mm::v4i f[2][2];
@@ -647,7 +666,8 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
                 mm::v4f c = meet[wave * 64 + lane];
 #pragma unroll
                 for (int w = 1; w < kSmallWaves; ++w) c += meet[(w * 3 + wave) * 64 + lane];
-                store_both(ti[0], tj[0], c * g.gram[step]);
+                a[0] = c * g.gram[step];
+                store_both(A, ti[0], tj[0], a[0]);
             }
         } else {
 #pragma unroll
@@ -658,11 +678,11 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
                 for (int k = 0; k < kx; ++k)
                     c.add(small_frag_kc(X, ldx, tj[x], k, 0, lane), small_frag_kc(X, ldx, tj[x], k, 1, lane), small_frag_kc(X, ldx, ti[x], k, 0, lane),
                           small_frag_kc(X, ldx, ti[x], k, 1, lane));
-                store_both(ti[x], tj[x], c.sum() * g.gram[step]);
+                a[x] = c.sum() * g.gram[step];
+                store_both(A, ti[x], tj[x], a[x]);
             }
         }
         __syncthreads();
-        mm::v4f b[TURNS];
 #pragma unroll
         for (int x = 0; x < TURNS; ++x) {
             if (wave + kSmallWaves * x >= TILES) break;
@@ -671,20 +691,18 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
             for (int k = 0; k < NB; ++k)
                 c.add(small_frag_kc(A, lda, tj[x], k, 0, lane), small_frag_kc(A, lda, tj[x], k, 1, lane), small_frag_kc(A, lda, ti[x], k, 0, lane),
                       small_frag_kc(A, lda, ti[x], k, 1, lane));
-            b[x] = c.sum();
+            b[x] = c.sum() * g.square[step] + a[x] * g.linear[step];
+            if (TWO) store_both(B, ti[x], tj[x], b[x]);
+        }
+        __syncthreads();
+        if constexpr (!TWO) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                const float a = Iterate<mm::Split>::load(A + (ti[x] + r) * lda, tj[x] + 4 * q + y);
-                b[x][y] = g.square[step] * b[x][y] + g.linear[step] * a;
+            for (int x = 0; x < TURNS; ++x) {
+                if (wave + kSmallWaves * x >= TILES) break;
+                store_both(B, ti[x], tj[x], b[x]);
             }
+            __syncthreads();
         }
-        __syncthreads();
-#pragma unroll
-        for (int x = 0; x < TURNS; ++x) {
-            if (wave + kSmallWaves * x >= TILES) break;
-            store_both(ti[x], tj[x], b[x]);
-        }
-        __syncthreads();
         const bool last = step + 1 == g.steps;
         mm::v4i next[NB][2];   // the block of the next turn is read while this one is multiplied
         auto read_block = [&](int j0) {
@@ -694,22 +712,26 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
                 next[k][1] = small_frag_strided(X, ldx, j0, k, 1, lane);
             }
         };
-        if (wave * 16 < Lp) read_block(wave * 16);
-        for (int j0 = wave * 16; j0 < Lp; j0 += kSmallWaves * 16) {
+        // two waves a block of columns, half of its rows each, where there are no more than 8 blocks
+        const bool halves = TWO && Lp <= 128;
+        const int first_block = halves ? wave >> 1 : wave, blocks = halves ? kSmallWaves / 2 : kSmallWaves;
+        const int from = halves && (wave & 1) ? Sp / 2 : 0, to = halves && !(wave & 1) ? Sp / 2 : Sp;
+        if (first_block * 16 < Lp) read_block(first_block * 16);
+        for (int j0 = first_block * 16; j0 < Lp; j0 += blocks * 16) {
             mm::v4i qf[NB][2];
 #pragma unroll
             for (int k = 0; k < NB; ++k) {
                 qf[k][0] = next[k][0];
                 qf[k][1] = next[k][1];
             }
-            if (j0 + kSmallWaves * 16 < Lp) read_block(j0 + kSmallWaves * 16);
+            if (j0 + blocks * 16 < Lp) read_block(j0 + blocks * 16);
 #pragma unroll 2
-            for (int i0 = 0; i0 < Sp; i0 += 16) {
+            for (int i0 = from; i0 < to; i0 += 16) {
                 SmallAcc acc;
 #pragma unroll
                 for (int k = 0; k < NB; ++k)
-                    acc.add(qf[k][0], qf[k][1], small_frag_kc(A, lda, i0, k, 0, lane), small_frag_kc(A, lda, i0, k, 1, lane));
-                mm::v4f c = acc.sum() * g.apply[step] + small_load4(X + (i0 + r) * ldx, j0 + 4 * q) * g.keep[step];
+                    acc.add(qf[k][0], qf[k][1], small_frag_kc(B, lda, i0, k, 0, lane), small_frag_kc(B, lda, i0, k, 1, lane));
+                const mm::v4f c = acc.sum() * g.apply[step] + small_load4(X + (i0 + r) * ldx, j0 + 4 * q) * g.keep[step];
                 if (last) {
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
@@ -717,11 +739,16 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
                         if (i < S && j < L) O[tall ? j * g.ldo + i : i * g.ldo + j] = (T)c[y];
                     }
                 } else {
-                    small_store4(X + (i0 + r) * ldx, j0 + 4 * q, c);
+                    small_store4(X2 + (i0 + r) * ldx, j0 + 4 * q, c);
                 }
             }
         }
         __syncthreads();
+        if (TWO) {
+            char* t = X;
+            X = X2;
+            X2 = t;
+        }
     }
 }
 
@@ -732,7 +759,8 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
     OrthoFactors f;
     if (!ortho_factors(!__is_same(F, double), steps, coef, f)) return GPX_ERR_ARG;
     if constexpr (!__is_same(F, double)) {
-        const long bytes = small_lds(rows, cols);
+        bool two = false;
+        const long bytes = small_lds(rows, cols, two);
         if (steps > 0 && bytes) {
             OrthoSmallArgs g = {ldg, stride_g, ldo, stride_o, rows, cols, steps, eps, f.start, {}, {}, {}, {}, {}};   // split planes for bf16 too
             for (int k = 0; k < steps; ++k) {
@@ -743,10 +771,15 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
                 g.keep[k] = (float)f.keep[k];
             }
             const int nb = (std::min(rows, cols) + 31) / 32;
-            if (nb == 1) ortho_small_kernel<T, 1><<<batch, kSmallWaves * 64, (unsigned)bytes, st>>>(G, O, g);
-            else if (nb == 2) ortho_small_kernel<T, 2><<<batch, kSmallWaves * 64, (unsigned)bytes, st>>>(G, O, g);
-            else if (nb == 3) ortho_small_kernel<T, 3><<<batch, kSmallWaves * 64, (unsigned)bytes, st>>>(G, O, g);
-            else ortho_small_kernel<T, 4><<<batch, kSmallWaves * 64, (unsigned)bytes, st>>>(G, O, g);
+            auto go = [&](auto blocks) {
+                constexpr int NB = decltype(blocks)::value;
+                if (two) ortho_small_kernel<T, NB, true><<<batch, kSmallWaves * 64, (unsigned)bytes, st>>>(G, O, g);
+                else ortho_small_kernel<T, NB, false><<<batch, kSmallWaves * 64, (unsigned)bytes, st>>>(G, O, g);
+            };
+            if (nb == 1) go(Int<1>{});
+            else if (nb == 2) go(Int<2>{});
+            else if (nb == 3) go(Int<3>{});
+            else go(Int<4>{});
             HIP_TRY(hipGetLastError());
             return GPX_OK;
         }
