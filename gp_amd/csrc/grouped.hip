@@ -93,8 +93,10 @@ template <int BM, int CHUNK, int HIGH = 8> __device__ RowTile find_tile(const in
     return row_tile(first, offsets, groups, T, (long)HIGH * band + in % high, BM);
 }
 
-// p[0..R) (those j + x < N) = alpha v + beta p in the type O, R of them 16 bytes, at any alignment
-template <class O, int R> __device__ __forceinline__ void put_run(char* row, int j, int N, const float (&v)[R], float alpha, float beta) {
+// p[0..R) (those j + x < N) = alpha v + beta p in the type O, R of them 16 bytes, at any alignment.  PAST: whole runs go past the
+// caches (weight gradients, which nobody reads soon: 163 -> 142 us for 16 of 2816 x 2048; forward results, which somebody does,
+// gain nothing).
+template <class O, int R, bool PAST> __device__ __forceinline__ void put_run(char* row, int j, int N, const float (&v)[R], float alpha, float beta) {
     static_assert(R * sizeof(O) == 16, "16 bytes");
     O* p = reinterpret_cast<O*>(row) + j;
     union { O e[R]; mm::v4i w; } u;
@@ -116,7 +118,9 @@ template <class O, int R> __device__ __forceinline__ void put_run(char* row, int
         // between fences: or the compiler takes what both branches store out of them, and the 16 bytes apart (165 -> 205 us for
         // 16 weight gradients of 2816 x 2048)
         asm volatile("" ::: "memory");
-        __builtin_memcpy(p, &u.w, 16);
+        typedef int v4iu __attribute__((ext_vector_type(4), aligned(1)));
+        if (PAST) __builtin_nontemporal_store(u.w, reinterpret_cast<v4iu*>(p));
+        else *reinterpret_cast<v4iu*>(p) = u.w;
         asm volatile("" ::: "memory");
     } else {
 #pragma unroll
@@ -126,11 +130,12 @@ template <class O, int R> __device__ __forceinline__ void put_run(char* row, int
 }
 
 // the tile's result: rows x cols of it at `row0`, `ld` bytes apart
-template <class O, class Tile>
+template <class O, bool PAST, class Tile>
 __device__ __forceinline__ void store_tile(Tile& t, char* lds, char* row0, long ld, int rows, int cols, double alpha, double beta) {
     typedef typename Tile::one A;
     const A al = (A)alpha, be = (A)beta;
     if constexpr (Tile::SWAP) {   // 16 neighbouring lanes store 16 neighbouring columns
+        if (Tile::group() != 0) return;
         t.each([&](int i, int j, const A* v, auto) {
             if (i >= rows || j >= cols) return;
             O* p = reinterpret_cast<O*>(row0 + i * ld) + j;
@@ -138,7 +143,7 @@ __device__ __forceinline__ void store_tile(Tile& t, char* lds, char* row0, long 
         });
     } else {
         constexpr int R = 16 / (int)sizeof(O);
-        t.template each_run<R>(lds, rows, cols, [&](int i, int j, const float (&v)[R]) { put_run<O, R>(row0 + i * ld, j, cols, v, al, be); });
+        t.template each_run<R>(lds, rows, cols, [&](int i, int j, const float (&v)[R]) { put_run<O, R, PAST>(row0 + i * ld, j, cols, v, al, be); });
     }
 }
 
@@ -146,21 +151,22 @@ constexpr int kShortSub = 8;
 
 template <class Tile> constexpr int tile_lds() { return Tile::SWAP || Tile::LDS > Tile::SLAB ? Tile::LDS : Tile::SLAB; }
 
-template <class T, int BM, int BN, int WR, int WC, int ST, bool WKC, bool DIRECT>
-__global__ __launch_bounds__(WR * WC * 64, 2) void grouped_kernel(const GroupedArgs g) {
-    typedef mm::Tile<T, BM, BN, WR, WC, true, WKC, ST> Tile;
+template <class T, int BM, int BN, int WR, int WC, int ST, int KG, bool WKC, bool DIRECT>
+__global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : 2) void grouped_kernel(const GroupedArgs g) {
+    typedef mm::Tile<T, BM, BN, WR, WC, true, WKC, ST, KG> Tile;
     __shared__ __attribute__((aligned(128))) char lds[tile_lds<Tile>()];
     int col = 0;
-    const RowTile rt = find_tile<BM, (BM * BN > 128 * 128 ? 256 : 512)>(g.offsets, g.groups, g.T, (g.N + BN - 1) / BN, col);
+    const RowTile rt = find_tile<BM, (BM * BN > 128 * 128 || KG > 1 ? 256 : 512)>(g.offsets, g.groups, g.T, (g.N + BN - 1) / BN, col);
     if (rt.group < 0) return;
     const int n0 = col * BN, cols = min(g.N - n0, BN);
     typename Tile::OpP p = {g.X + rt.row0 * g.ldx, g.ldx, rt.rows, g.K};
     typename Tile::OpQ q = {g.W + rt.group * g.stride_w + (WKC ? n0 * g.ldw : n0 * (long)sizeof(T)), g.ldw, cols, g.K};
     Tile t;
     t.clear();
-    if (DIRECT) t.run_direct(lds, p, q, g.K);
+    if constexpr (KG > 1) t.run_groups(lds, p, q, g.K);
+    else if constexpr (DIRECT) t.run_direct(lds, p, q, g.K);
     else t.run_staged(lds, p, q, g.K);
-    store_tile<T>(t, lds, g.Y + rt.row0 * g.ldy + n0 * (long)sizeof(T), g.ldy, rt.rows, cols, g.alpha, g.beta);
+    store_tile<T, false>(t, lds, g.Y + rt.row0 * g.ldy + n0 * (long)sizeof(T), g.ldy, rt.rows, cols, g.alpha, g.beta);
 }
 
 // Short k (at most 512 bytes of it: inputs of a few dozen dimensions) in floats and doubles, where the result is most of the
@@ -253,7 +259,7 @@ __global__ __launch_bounds__(256, 4) void grouped_short_kernel(const GroupedArgs
                 else asm volatile("global_store_dword %0, %1, %2 nt" ::"v"(off), "v"(o), "s"(at_y) : "memory");
             });
         } else {
-            store_tile<T>(m, lds, y, g.ldy, rows, cols, g.alpha, g.beta);
+            store_tile<T, false>(m, lds, y, g.ldy, rows, cols, g.alpha, g.beta);
         }
         counted = whole && t + 2 < tiles;
         if (t + 2 < tiles) {
@@ -319,9 +325,9 @@ __global__ __launch_bounds__(WR * WC * 64, 2) void grouped_dw_kernel(const Group
     else t.run_staged(lds, p, q, rows);
     if (SPLIT) {
         const long ld = (long)g.M * sizeof(A);
-        store_tile<A>(t, lds, g.slabs + (blockIdx.y * (long)g.N + n0) * ld + m0 * (long)sizeof(A), ld, p.rows, q.rows, 1.0, 0.0);
+        store_tile<A, false>(t, lds, g.slabs + (blockIdx.y * (long)g.N + n0) * ld + m0 * (long)sizeof(A), ld, p.rows, q.rows, 1.0, 0.0);
     } else {
-        store_tile<O>(t, lds, g.C + group * g.stride_c + n0 * g.ldc + m0 * (long)sizeof(O), g.ldc, p.rows, q.rows, g.alpha, g.beta);
+        store_tile<O, true>(t, lds, g.C + group * g.stride_c + n0 * g.ldc + m0 * (long)sizeof(O), g.ldc, p.rows, q.rows, g.alpha, g.beta);
     }
 }
 
@@ -366,9 +372,16 @@ constexpr TileCost kCost16[] = {
     {128, 128, 512, 1.05, 0.52, 5.0},    // two of 4 waves: 1.00-1.07
     {64, 64, 512, 0.38, 0.25, 2.3},      // two of 4 waves, four LDS stages: 0.63
     {32, 128, 512, 0.43, 0.30, 2.0},     // a few rows a group, W in 256-byte runs (n contiguous): the read of W bounds it
-    {32, 64, 768, 0.36, 0.25, 2.0}};     // the same, k contiguous: 5.0 TB/s on 32 x 2816 x 2048, 6 TB/s where W is cached
-constexpr TileCost kCost32[] = {{128, 128, 512, 3.30, 2.40, 3.0}, {64, 64, 256, 0.52, 0.52, 1.0}, {32, 64, 256, 0.32, 0.32, 1.0}};   // 4-byte floats
-constexpr TileCost kCost64[] = {{128, 128, 512, 3.90, 2.20, 3.0}, {64, 64, 256, 0.51, 0.51, 1.0}, {32, 64, 256, 0.31, 0.31, 1.0}};   // doubles
+    {32, 64, 768, 0.36, 0.25, 2.0},      // the same, k contiguous: 5.5 TB/s on 32 x 2816 x 2048
+    {32, 64, 256, 0.25, 0.10, 4.0},      // few tiles and long k: four groups of waves share the sum (one of 8192 x 8192: 40 -> 28 us)
+    {64, 64, 256, 0.25, 0.11, 5.0},
+    {32, 16, 256, 0.12, 0.05, 4.0}};     // narrow ones, eight single waves
+// 4-byte floats and doubles; the last two as above: four groups of four waves (8 groups of 2 rows, 1024 x 1024 in doubles: 35 -> 27 us),
+// eight of one (30 rows, 512 x 8192 in floats, 512 x 4096 in doubles: 87 -> 32 us)
+constexpr TileCost kCost32[] = {{128, 128, 512, 3.30, 2.40, 3.0}, {64, 64, 256, 0.52, 0.52, 1.0}, {32, 64, 256, 0.32, 0.45, 1.0},
+                                 {32, 64, 256, 0.36, 0.33, 2.5}, {32, 16, 256, 0.18, 0.06, 3.0}};
+constexpr TileCost kCost64[] = {{128, 128, 512, 3.90, 2.20, 3.0}, {64, 64, 256, 0.51, 0.51, 1.0}, {32, 64, 256, 0.31, 0.45, 1.0},
+                                 {32, 64, 256, 0.36, 0.33, 2.5}, {32, 16, 256, 0.18, 0.06, 3.0}};
 double tile_time(const TileCost& c, double tiles, double steps) {
     const double full = floor(tiles / c.slots), left = tiles - full * c.slots;
     return full * (c.step * steps + c.rest) + (left > 256.0 ? c.step * steps + c.rest : left > 0.0 ? c.alone * steps + c.rest : 0.0);
@@ -385,19 +398,21 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
         return tile_time(c, mt * ((g.N + c.bn - 1) / c.bn), steps);
     };
     int rc = GPX_OK;
-    auto go = [&](auto bm, auto bn, auto wr, auto wc, auto stages) {
-        constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WR = decltype(wr)::value, WC = decltype(wc)::value, ST = decltype(stages)::value;
+    auto go = [&](auto bm, auto bn, auto wr, auto wc, auto stages, auto kgroups) {
+        constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WR = decltype(wr)::value, WC = decltype(wc)::value, ST = decltype(stages)::value,
+                      KG = decltype(kgroups)::value;
         const long tiles = row_tiles(g.T, g.groups, BM) * ((g.N + BN - 1) / BN);
         if (tiles >= (1L << 31) - 512) {
             rc = GPX_ERR_UNSUPPORTED;
             return;
         }
         const unsigned grid = (unsigned)((tiles + 7) / 8 * 8);   // as many for every XCD
-        if (w_kc && direct) grouped_kernel<T, BM, BN, WR, WC, ST, true, true><<<grid, WR * WC * 64, 0, st>>>(g);
-        else if (direct) grouped_kernel<T, BM, BN, WR, WC, ST, false, true><<<grid, WR * WC * 64, 0, st>>>(g);
-        else if constexpr (BM == 256) rc = GPX_ERR_STATE;   // (never chosen for rows that are not direct)
-        else if (w_kc) grouped_kernel<T, BM, BN, WR, WC, 2, true, false><<<grid, WR * WC * 64, 0, st>>>(g);
-        else grouped_kernel<T, BM, BN, WR, WC, 2, false, false><<<grid, WR * WC * 64, 0, st>>>(g);
+        constexpr int threads = WR * WC * 64 * KG;
+        if (w_kc && direct) grouped_kernel<T, BM, BN, WR, WC, ST, KG, true, true><<<grid, threads, 0, st>>>(g);
+        else if (direct) grouped_kernel<T, BM, BN, WR, WC, ST, KG, false, true><<<grid, threads, 0, st>>>(g);
+        else if constexpr (BM == 256 || KG > 1) rc = GPX_ERR_STATE;   // (never chosen for rows that are not direct)
+        else if (w_kc) grouped_kernel<T, BM, BN, WR, WC, 2, 1, true, false><<<grid, threads, 0, st>>>(g);
+        else grouped_kernel<T, BM, BN, WR, WC, 2, 1, false, false><<<grid, threads, 0, st>>>(g);
     };
     // from: rows that have to pass through registers take 128-tiles at most (20000 x 1001 x 2003 in bf16: 166 us, 256-tiles 241)
     auto best_of = [&](const TileCost* c, int from, int n, int not_this) {
@@ -407,12 +422,15 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
         return best;
     };
     if constexpr (sizeof(T) == 2) {
-        switch (best_of(kCost16, direct ? 0 : 1, 5, w_kc ? 3 : 4)) {
-            case 0: go(Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{}); break;
-            case 1: go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}); break;
-            case 2: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<4>{}); break;
-            case 3: go(Int<32>{}, Int<128>{}, Int<1>{}, Int<4>{}, Int<4>{}); break;
-            default: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<4>{});
+        switch (best_of(kCost16, direct ? 0 : 1, direct ? 8 : 5, w_kc ? 3 : 4)) {
+            case 0: go(Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{}, Int<1>{}); break;
+            case 1: go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<1>{}); break;
+            case 2: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<4>{}, Int<1>{}); break;
+            case 3: go(Int<32>{}, Int<128>{}, Int<1>{}, Int<4>{}, Int<4>{}, Int<1>{}); break;
+            case 4: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<4>{}, Int<1>{}); break;
+            case 5: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<3>{}, Int<4>{}); break;
+            case 6: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<4>{}); break;
+            default: go(Int<32>{}, Int<16>{}, Int<1>{}, Int<1>{}, Int<3>{}, Int<8>{});
         }
     } else if (const long units = row_tiles(g.T, g.groups, 32 * kShortSub) * ((g.N + 63) / 64);
                direct && g.K * (long)sizeof(T) <= 512 && 32 * g.ldy < (long)mm::kRange && g.K > 0 && units >= 512 && units < (1L << 31) - 512) {
@@ -421,10 +439,12 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
         if (w_kc) grouped_short_kernel<T, true><<<grid, 256, 0, st>>>(g);
         else grouped_short_kernel<T, false><<<grid, 256, 0, st>>>(g);
     } else {
-        switch (best_of(sizeof(T) == 4 ? kCost32 : kCost64, 0, 3, -1)) {
-            case 0: go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}); break;
-            case 1: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{}); break;
-            default: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<4>{});
+        switch (best_of(sizeof(T) == 4 ? kCost32 : kCost64, 0, direct ? 5 : 3, -1)) {
+            case 0: go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<1>{}); break;
+            case 1: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<1>{}); break;
+            case 2: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<4>{}, Int<1>{}); break;
+            case 3: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<3>{}, Int<4>{}); break;
+            default: go(Int<32>{}, Int<16>{}, Int<1>{}, Int<1>{}, Int<3>{}, Int<8>{});
         }
     }
     HIP_TRY(hipGetLastError());

@@ -204,7 +204,8 @@ template <class F, int ROWS, bool KC, int NT> struct Operand {
         }
         return l;
     }
-    __device__ __forceinline__ void issue(unsigned lds_addr, const Lanes& l, int step) const {
+    // ONCE: nobody else reads these bytes, they need not stay in a cache
+    template <bool ONCE = false> __device__ __forceinline__ void issue(unsigned lds_addr, const Lanes& l, int step) const {
         const unsigned long long a = reinterpret_cast<unsigned long long>(base) + (unsigned long long)step * (KC ? 128 : BK * ld);
         v4i rsrc = {__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff)),
                     (int)kRange, 0x00027000};
@@ -212,9 +213,14 @@ template <class F, int ROWS, bool KC, int NT> struct Operand {
         const unsigned wave_addr = __builtin_amdgcn_readfirstlane(lds_addr + (tid() >> 6) * 1024);
 #pragma unroll
         for (int it = 0; it < NL; ++it)   // lane l of the wave writes the 16 bytes at M0 + 16 l
-            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(l.off[it]), "s"(rsrc),
-                         "s"(wave_addr + it * NT * 16)
-                         : "memory");
+            if constexpr (ONCE)
+                asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds" ::"v"(l.off[it]), "s"(rsrc),
+                             "s"(wave_addr + it * NT * 16)
+                             : "memory");
+            else
+                asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(l.off[it]), "s"(rsrc),
+                             "s"(wave_addr + it * NT * 16)
+                             : "memory");
     }
     __device__ __forceinline__ void stash(char* s, const v4i (&r)[NL]) const {
 #pragma unroll
@@ -231,6 +237,8 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
     static constexpr int NT = WR * WC * 64;
     static constexpr int TI = BM / WR / 16, TJ = BN / WC / 16;
     static constexpr bool SWAP = sizeof(T) != 2;
+    // a tile of 32 rows is mostly all the rows of its group: its Q is read once (32 groups of 2816 x 2048: 4.9 -> 5.5 TB/s)
+    static constexpr bool ONCE = BM == 32;
     typedef Operand<F, BM, PKC, NT> OpP;
     typedef Operand<F, BN, QKC, NT> OpQ;
     typedef typename Acc<T>::vec vec;
@@ -331,7 +339,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
                 lq = q.lanes(rest);
             }
             p.issue(at + stage * STAGE, lp, s);
-            q.issue(at + stage * STAGE + OpP::BYTES, lq, s);
+            q.template issue<ONCE>(at + stage * STAGE + OpP::BYTES, lq, s);
         };
         const bool busy = has_rows(p.rows, q.rows);
         for (int s = 0; s < STAGES - 1 && s < steps; ++s) issue(s, s);
@@ -350,31 +358,36 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
     // and add their accumulators at the end in one order, the sum in group 0.  A step of a 64-tile alone on its CU costs
     // 0.36 us, most of it waiting; four groups do four in 0.5 us.
     __device__ __forceinline__ void run_groups(char* lds, const OpP& p, const OpQ& q, int K) {
-        static_assert(STAGES == 2 && GROUPS > 1, "two stages of every group");
-        constexpr int BK = OpP::BK;
+        static_assert(GROUPS > 1, "groups");
+        constexpr int BK = OpP::BK, AHEAD = (STAGES - 2) * (OpP::NL + OpQ::NL);
         const int full = K / BK, rest = K - full * BK, steps = full + (rest != 0), turns = (steps + GROUPS - 1) / GROUPS, mine = group();
+        const int own_turns = (steps - mine + GROUPS - 1) / GROUPS;   // (0 where steps <= mine)
         typename OpP::Lanes lp = p.lanes(BK);
         typename OpQ::Lanes lq = q.lanes(BK);
-        char* own = lds + mine * 2 * STAGE;
+        char* own = lds + mine * STAGES * STAGE;
         const unsigned at = (unsigned)reinterpret_cast<unsigned long long>((__attribute__((address_space(3))) char*)own);
-        auto issue = [&](int turn) {
+        auto issue = [&](int turn, int stage) {
             const int s = turn * GROUPS + mine;
             if (s >= steps) return;
             if (s >= full) {
                 lp = p.lanes(rest);
                 lq = q.lanes(rest);
             }
-            p.issue(at + (turn & 1) * STAGE, lp, s);
-            q.issue(at + (turn & 1) * STAGE + OpP::BYTES, lq, s);
+            p.issue(at + stage * STAGE, lp, s);
+            q.template issue<ONCE>(at + stage * STAGE + OpP::BYTES, lq, s);
         };
         const bool busy = has_rows(p.rows, q.rows);
-        if (turns) issue(0);
+        for (int t = 0; t < STAGES - 1; ++t) issue(t, t);
+        int stage = 0, into = STAGES - 1;
         for (int t = 0; t < turns; ++t) {
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (t + 1 < turns) issue(t + 1);
+            if (STAGES > 2 && t + STAGES - 2 < own_turns) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(AHEAD) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            issue(t + STAGES - 1, into);
             const int s = t * GROUPS + mine;
-            const char* st = own + (t & 1) * STAGE;
+            const char* st = own + stage * STAGE;
             if (busy && s < steps) multiply(st, st + OpP::BYTES, s >= full && rest * 2 <= BK ? 1 : 2);
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            into = into + 1 == STAGES ? 0 : into + 1;
         }
         __syncthreads();
         vec* meet = reinterpret_cast<vec*>(lds);
