@@ -107,9 +107,11 @@ __global__ __launch_bounds__(256) void ortho_normalize_kernel(const T* G, long l
 // step of the second plane is 2^-39 of that bound.
 // bf16: X is kept as the same two planes, but apart, and the products take the first one only, values rounded to 11 bits, one
 // matrix product instead of three and half the bytes.  That rounding is an eighth of the one that the bf16 matrix itself has
-// behind it, and the result is rounded to 8 bits; a X, where X's own bits count, is formed from both planes.
-// 16 matrices of 1024 x 2816: 2.61 -> 1.45 ms; off from 64 bits by 2.1e-3, of which 1.7e-3 is the rounding of the result; half a step
-// of the input moves the result by 4e-3 (by 4e-2 where the singular values span five orders of magnitude: 1.8e-3 here).
+// behind it, and the result is rounded to 8 bits.  Where X's own bits count, both planes are used: in a X, and in the diagonal of
+// b A + c A A, the largest of its elements, which is kept in floats beside that matrix (zero in it) and applied with a X.
+// 300 x 2000, six steps, error before the result's own rounding of 1.66e-3: 2.0e-3 with the diagonal rounded, 7.3e-4 without.
+// 16 matrices of 1024 x 2816: 2.61 -> 1.45 ms; off from 64 bits by 1.80e-3, 1.66e-3 of it the rounding of the result; half a step
+// of the input moves the result by 4e-3 (by 4e-2 where the singular values span five orders of magnitude: 1.78e-3 here).
 template <class F> struct Iterate;
 // v = h + l.  The compiler may form a converted product in one rounding and the product itself in two; h has to be one value
 // for both planes (told apart at ties, the planes would disagree by a step of the first one).
@@ -151,11 +153,11 @@ template <> struct Iterate<mm::Split> {
         *reinterpret_cast<mm::v8h*>(p) = h;
         *reinterpret_cast<mm::v8h*>(p + 32) = l;
     }
-    __device__ static void add8(const char* row, long, int j, float by, float (&v)[8]) {   // v += by * row
+    __device__ static void add8(const char* row, long, int j, const float (&by)[8], float (&v)[8]) {   // v += by * row
         const _Float16* p = reinterpret_cast<const _Float16*>(row) + at(j);
         const mm::v8h h = *reinterpret_cast<const mm::v8h*>(p), l = *reinterpret_cast<const mm::v8h*>(p + 32);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) v[x] += by * ((float)h[x] + (float)l[x]);
+        for (int x = 0; x < 8; ++x) v[x] += by[x] * ((float)h[x] + (float)l[x]);
     }
 };
 template <> struct Iterate<mm::Rounded> {
@@ -174,12 +176,12 @@ template <> struct Iterate<mm::Rounded> {
         *reinterpret_cast<mm::v8h*>(row + j * 2) = h;
         if (lo) *reinterpret_cast<mm::v8h*>(row + lo + j * 2) = l;
     }
-    __device__ static void add8(const char* row, long lo, int j, float by, float (&v)[8]) {
+    __device__ static void add8(const char* row, long lo, int j, const float (&by)[8], float (&v)[8]) {
         const mm::v8h h = *reinterpret_cast<const mm::v8h*>(row + j * 2);
         mm::v8h l = {};
         if (lo) l = *reinterpret_cast<const mm::v8h*>(row + lo + j * 2);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) v[x] += by * ((float)h[x] + (float)l[x]);
+        for (int x = 0; x < 8; ++x) v[x] += by[x] * ((float)h[x] + (float)l[x]);
     }
 };
 template <class F> int padded(int cols) { return (cols + Iterate<F>::PAD - 1) / Iterate<F>::PAD * Iterate<F>::PAD; }
@@ -208,12 +210,16 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ 
 
 // D = c1 P Q^T + c2 E over a batch, E and D in the format F, or (LAST) D in the type O of the result.
 // SYM: D is symmetric; tiles on and below the diagonal are computed, and those below it stored on both sides.
+// diag (Rounded only): a symmetric product with E moves its diagonal there, in floats; the product with X adds c1 diag to c2,
+// by the rows of D where the square factor is on the left, by its columns where it is on the right (QKC).
 struct OrthoArgs {
     const char* P; const char* Q; const char* E; char* D;
     long ldp, ldq, lde, ldd, sp, sq, se, sd;   // bytes
     long loe, lod;                             // from the first plane of E and D to the second, where there is one
     int I, J, K, batch;
     double c1, c2;
+    float* diag;
+    long sdiag;   // floats
 };
 template <class F, class O, bool LAST, int B, int WR, int WC, int ST, int KG, bool PKC, bool QKC, bool SYM>
 __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) > 128 * 64 ? 1 : 2) void ortho_mm_kernel(const OrthoArgs g) {
@@ -274,6 +280,11 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
         // tile too (single elements from the accumulators: 90 us for a 256 x 256 tile, most of it the mirrored stores).
         float* slab = reinterpret_cast<float*>(lds);
         constexpr int NT = Tile::THREADS, R = Tile::SLAB_ROWS;
+        constexpr bool DIAG = __is_same(F, mm::Rounded);
+        float* diag = DIAG && g.diag ? g.diag + mat * g.sdiag : nullptr;
+        float all[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) all[x] = c2;
         for (int pass = 0; pass < WR; ++pass) {
             const int ib = i0 + pass * R;
             __syncthreads();
@@ -289,7 +300,24 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
                     v[x] = c1 * lo[x];
                     v[4 + x] = c1 * hi[x];
                 }
-                if (c2 != 0.0f) Iterate<F>::add8(E + i * g.lde, g.loe, j, c2, v);
+                if constexpr (DIAG && !SYM) {
+                    float by[8];
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) by[x] = c2 + c1 * (!QKC ? diag[i] : j + x < g.J ? diag[j + x] : 0.0f);
+                    Iterate<F>::add8(E + i * g.lde, g.loe, j, by, v);
+                } else {
+                    if (c2 != 0.0f) Iterate<F>::add8(E + i * g.lde, g.loe, j, all, v);
+                }
+                if constexpr (DIAG && SYM) {
+                    if (diag && i >= j && i < j + 8) {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            if (i == j + x) {
+                                diag[i] = v[x];
+                                v[x] = 0.0f;
+                            }
+                    }
+                }
                 if constexpr (LAST) {
                     O* d = reinterpret_cast<O*>(D + i * g.ldd) + j;
                     typedef O o8 __attribute__((ext_vector_type(8)));
@@ -318,7 +346,7 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
                     float v[8];
 #pragma unroll
                     for (int x = 0; x < 8; ++x) v[x] = c1 * slab[Tile::slab_at(il + x, jl)];
-                    if (c2 != 0.0f) Iterate<F>::add8(E + j * g.lde, g.loe, i, c2, v);
+                    if (c2 != 0.0f) Iterate<F>::add8(E + j * g.lde, g.loe, i, all, v);
                     Iterate<F>::store8(D + j * g.ldd, g.lod, i, v);
                 }
             }
@@ -346,7 +374,7 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
 }
 
 struct OrthoWork {   // offsets and strides in bytes; rows of the iterates padded to whole blocks
-    long part, x[2], a, b, total;
+    long part, x[2], a, b, diag, total;
     long ldx, sx, lda, sa, lo;   // lo: from the first plane of X to the second
 };
 // Rows of a power of two of bytes would meet in few memory channels: the K step of a tile reads 128 bytes of every row.
@@ -368,7 +396,8 @@ template <class F> OrthoWork ortho_work_of(long batch, int rows, int cols) {
     o.x[1] = o.x[0] + Iterate<F>::PLANES * up(batch * o.sx);
     o.a = o.x[1] + Iterate<F>::PLANES * up(batch * o.sx);
     o.b = o.a + up(batch * o.sa);
-    o.total = o.b + up(batch * o.sa);
+    o.diag = o.b + up(batch * o.sa);
+    o.total = o.diag + (Iterate<F>::PLANES == 2 ? up(batch * s * 4) : 0);
     return o;
 }
 OrthoWork ortho_work(int dtype, long batch, int rows, int cols) {
@@ -798,23 +827,24 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
     }
     char* x[2] = {work + o.x[0], work + o.x[1]};
     char *a = work + o.a, *b = work + o.b;
+    float* diag = Iterate<F>::PLANES == 2 ? reinterpret_cast<float*>(work + o.diag) : nullptr;
     ortho_scale_kernel<T, F><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, padded<F>(cols), part, parts, eps, f.start, x[0], o.ldx, o.sx, o.lo);
     HIP_TRY(hipGetLastError());
     const bool tall = rows > cols;
     const int s = std::min(rows, cols), l = std::max(rows, cols);
     for (int k = 0; k < steps; ++k) {
         char *from = x[k & 1], *to = x[~k & 1];
-        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, 0, 0, s, s, l, batch, f.gram[k], 0.0};
+        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, 0, 0, s, s, l, batch, f.gram[k], 0.0, nullptr, 0};
         int rc = tall ? launch<F, F, false, false, false, true>(st, gram, batch) : launch<F, F, false, true, true, true>(st, gram, batch);
         if (rc) return rc;
         const OrthoArgs poly = {a, a, a, b, o.lda, o.lda, o.lda, o.lda, o.sa, o.sa, o.sa, o.sa, 0, 0, s, s, s, batch,
-                                f.square[k], f.linear[k]};
+                                f.square[k], f.linear[k], diag, s};
         if ((rc = launch<F, F, false, true, true, true>(st, poly, batch))) return rc;
         const bool last = k + 1 == steps;
         const long ldd = last ? ldo * (long)sizeof(T) : o.ldx, sd = last ? stride_o * (long)sizeof(T) : o.sx;
         char* d = last ? reinterpret_cast<char*>(O) : to;
-        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, o.lo, o.lo, rows, cols, s, batch, f.apply[k], f.keep[k]}
-                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, o.lo, o.lo, rows, cols, s, batch, f.apply[k], f.keep[k]};
+        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, o.lo, o.lo, rows, cols, s, batch, f.apply[k], f.keep[k], diag, s}
+                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, o.lo, o.lo, rows, cols, s, batch, f.apply[k], f.keep[k], diag, s};
         if (tall) rc = last ? launch<F, T, true, true, true, false>(st, apply, batch) : launch<F, F, false, true, true, false>(st, apply, batch);
         else rc = last ? launch<F, T, true, true, false, false>(st, apply, batch) : launch<F, F, false, true, false, false>(st, apply, batch);
         if (rc) return rc;

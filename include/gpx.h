@@ -105,9 +105,10 @@ int gpx_grouped_gemm_dw(int dtype, int c_dtype, int64_t groups, int64_t T, int64
 /* batch matrices G_b (M x N column-major at G + b*stride_g): X = G / (|G|_F + eps), then `steps` (0..64) times
  *   A = X X^T,  X = a X + (b A + c A A) X        (the odd polynomial a s + b s^3 + c s^5 of the singular values s)
  * into O.  The iterates of F64 are doubles, of F32 and F16 hold 22 bits or more, and BF16 products take operands rounded to 11
- * bits (the input has 8).  coef: HOST, 3*steps finite values a, b, c of every step; NULL: (3.4445, -4.7750, 2.0315) in each.  eps > 0: a
- * zero matrix gives zeros.  Coefficients that could carry singular values past 2^100 are refused, except for F64.  A matrix that holds an infinity or NaN gives non-finite values in its own result only.  O may
- * be G (same ld and stride).  work: as above, gpx_orthogonalize_work bytes. */
+ * bits (the input has 8) except for a X and the diagonal of b A + c A A.  coef: HOST, 3*steps finite values a, b, c of every
+ * step; NULL: (3.4445, -4.7750, 2.0315) in each.  eps > 0: a zero matrix gives zeros.  Coefficients that could carry singular
+ * values past 2^100 are refused, except for F64.  A matrix that holds an infinity or NaN gives non-finite values in its own
+ * result only.  O may be G (same ld and stride).  work: as above, gpx_orthogonalize_work bytes. */
 int gpx_orthogonalize_work(int dtype, int64_t batch, int64_t M, int64_t N, int64_t* work_bytes);
 int gpx_orthogonalize(int dtype, int64_t batch, int64_t M, int64_t N, const void* G, int64_t ldg, int64_t stride_g, int steps,
                       const double* coef, double eps, void* O, int64_t ldo, int64_t stride_o, void* work, int64_t work_bytes,

@@ -86,6 +86,20 @@ def test_bfloat16_is_as_good_as_its_input(size, spread):
     assert off(lib.orthogonalize(g, torch.empty_like(g))) <= off(moved) + 2.0 ** -8 * float(torch.linalg.norm(want))
 
 
+@pytest.mark.parametrize("size", [(300, 2000), (2000, 300), (60, 2900), (700, 690)], ids=str)
+@pytest.mark.parametrize("steps,coef", [(6, None), (6, (1.5, -0.5, 0.0)), (1, (0.5, 3.0, -2.0))], ids=str)
+def test_bfloat16_rounds_no_diagonal(size, steps, coef):
+    """A step rounds X (in two products), A and the square factor outside of its diagonal to 11 bits, each time by at most
+    2^-11 / sqrt(3) of a value in the mean square, and a step passes an earlier error on without growth once the singular
+    values have come near one: sqrt(4 steps) of these beside the rounding of the result."""
+    lib = _lib()
+    g = data(1, torch.bfloat16, *size)
+    want, _ = oracle.orthogonalize(g, steps=steps, coef=coef)
+    off = lambda a: float(torch.linalg.norm(a.double() - want) / torch.linalg.norm(want))  # noqa: E731
+    bound = (off(want.to(torch.bfloat16)) ** 2 + 4 * steps * 2.0 ** -22 / 3) ** 0.5
+    assert off(lib.orthogonalize(g, torch.empty_like(g), steps=steps, coef=coef)) <= bound
+
+
 def test_cubic_steps_reach_the_polar_factor():
     """(1.5, -0.5, 0) converges to U V^T: the rows of the result are orthonormal."""
     lib = _lib()
