@@ -541,6 +541,7 @@ template <class T, class O> int grouped_dw_typed(hipStream_t st, const GroupedDw
 
 constexpr long kMaxExtent = (1L << 31) - 1024;   // row, column and k numbers within one product are 32-bit
 constexpr int kMaxGroups = 65535;
+constexpr int64_t kMaxLd = 1L << 32, kMaxStride = 1L << 48;   // elements: no product of sizes below passes 63 bits
 
 int elem_bytes(int dtype) { return dtype == GPX_F64 ? 8 : dtype == GPX_F32 ? 4 : dtype == GPX_BF16 || dtype == GPX_F16 ? 2 : 0; }
 bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes != 0; }
@@ -554,6 +555,7 @@ extern "C" int gpx_grouped_gemm(int dtype, int w_kc, int64_t groups, int64_t T, 
     if (!e || groups < 0 || groups > kMaxGroups || T < 0 || N < 0 || K < 0) return GPX_ERR_ARG;
     if (T > kMaxExtent || N > kMaxExtent || K > kMaxExtent) return GPX_ERR_ARG;
     if (ldx < K || ldw < (w_kc ? K : N) || ldy < N || stride_w < 0) return GPX_ERR_ARG;
+    if (ldx > kMaxLd || ldw > kMaxLd || ldy > kMaxLd || stride_w > kMaxStride) return GPX_ERR_ARG;
     if (groups == 0 || T == 0 || N == 0) return GPX_OK;   // no row of Y belongs to a group
     if (!Y || !offsets || (K > 0 && (!X || !W))) return GPX_ERR_ARG;
     if (misaligned(X, e) || misaligned(W, e) || misaligned(Y, e) || misaligned(offsets, 8)) return GPX_ERR_ARG;
@@ -578,6 +580,7 @@ extern "C" int gpx_grouped_gemm_dw(int dtype, int c_dtype, int64_t groups, int64
     if (groups < 0 || groups > kMaxGroups || T < 0 || M < 0 || N < 0 || T > kMaxExtent || M > kMaxExtent || N > kMaxExtent)
         return GPX_ERR_ARG;
     if (ldx < M || ldz < N || ldc < M || stride_c < 0 || work_bytes < 0) return GPX_ERR_ARG;
+    if (ldx > kMaxLd || ldz > kMaxLd || ldc > kMaxLd || stride_c > kMaxStride) return GPX_ERR_ARG;
     if (groups == 0 || M == 0 || N == 0) return GPX_OK;
     if (groups > 1 && stride_c < (N - 1) * ldc + M) return GPX_ERR_ARG;   // results of two groups would overlap
     if (!C || !offsets || (T > 0 && (!X || !Z))) return GPX_ERR_ARG;

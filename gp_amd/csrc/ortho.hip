@@ -854,6 +854,8 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
 
 constexpr int kMaxSteps = 64;
 constexpr long kMaxSide = 1L << 20;
+constexpr int64_t kMaxLd = 1L << 32, kMaxStride = 1L << 48;   // elements: no product of sizes below passes 63 bits
+constexpr double kLeastEps = 1e-300;                          // 2^15 / eps stays finite: a zero matrix gives zeros
 const double kQuintic[3] = {3.4445, -4.7750, 2.0315};
 
 bool sizes_ok(int dtype, int64_t batch, int64_t M, int64_t N) {
@@ -871,8 +873,9 @@ extern "C" int gpx_orthogonalize_work(int dtype, int64_t batch, int64_t M, int64
 extern "C" int gpx_orthogonalize(int dtype, int64_t batch, int64_t M, int64_t N, const void* G, int64_t ldg, int64_t stride_g, int steps,
                                  const double* coef, double eps, void* O, int64_t ldo, int64_t stride_o, void* work, int64_t work_bytes,
                                  void* hip_stream) {
-    if (!sizes_ok(dtype, batch, M, N) || steps < 0 || steps > kMaxSteps || !(eps > 0.0) || !std::isfinite(eps)) return GPX_ERR_ARG;
+    if (!sizes_ok(dtype, batch, M, N) || steps < 0 || steps > kMaxSteps || !(eps >= kLeastEps) || !std::isfinite(eps)) return GPX_ERR_ARG;
     if (ldg < M || ldo < M || stride_g < 0 || stride_o < 0) return GPX_ERR_ARG;
+    if (ldg > kMaxLd || ldo > kMaxLd || stride_g > kMaxStride || stride_o > kMaxStride) return GPX_ERR_ARG;
     if (batch == 0 || M == 0 || N == 0) return GPX_OK;
     if (batch > 1 && stride_o < (N - 1) * ldo + M) return GPX_ERR_ARG;   // results of two matrices would overlap
     if (!G || !O || !work) return GPX_ERR_ARG;

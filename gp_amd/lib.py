@@ -337,7 +337,7 @@ def chol_solve(A, B=None, want_inverse=False):
 
 # ---- products grouped by expert, orthogonalised update ---------------------------------------------
 # These take torch tensors on the GPU (rows of any stride, the last dimension contiguous), launch on torch's current stream
-# of the tensors' device and return `out`; nothing is recorded for autograd.  torch is imported only when one is called.
+# of the tensors' device and return `out`, which overlaps no operand; nothing is recorded for autograd.  torch is imported only when one is called.
 F64, F32, BF16, F16 = 0, 1, 2, 3
 
 lib.gpx_grouped_gemm.argtypes = [_i, _i, _i64, _i64, _i64, _i64, _d, _vp, _i64, _vp, _i64, _i64, _vp, _d, _vp, _i64, _vp]

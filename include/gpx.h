@@ -76,7 +76,8 @@ int gpx_dgemm_splitk_noalloc(int a_kc, int b_kc, int64_t M, int64_t N, int64_t K
  * the gradients of both operands, and the Newton-Schulz update of a batch of weight matrices.  All buffers are DEVICE
  * memory of hip_stream's device (NULL: the legacy stream of the current device); every call is asynchronous, allocates
  * nothing, waits for nothing and may be captured into a HIP graph; the caller's current device is restored.  Element
- * types: dtype below; pointers are aligned to their element, rows of any length and leading dimension are taken.
+ * types: dtype below; pointers are aligned to their element, rows of any length are taken, leading dimensions up to 2^32 and
+ * strides up to 2^48 elements.  A result overlaps no operand (but see gpx_orthogonalize).
  * Products of F64 are summed in 64 bits, all others in 32; results are rounded once to the type they are stored in.
  * No result depends on the order in which workgroups run.  Status 1 (GPX_ERR_ARG): an argument is refused, nothing was
  * launched. */
@@ -106,9 +107,10 @@ int gpx_grouped_gemm_dw(int dtype, int c_dtype, int64_t groups, int64_t T, int64
  *   A = X X^T,  X = a X + (b A + c A A) X        (the odd polynomial a s + b s^3 + c s^5 of the singular values s)
  * into O.  The iterates of F64 are doubles, of F32 and F16 hold 22 bits or more, and BF16 products take operands rounded to 11
  * bits (the input has 8) except for a X and the diagonal of b A + c A A.  coef: HOST, 3*steps finite values a, b, c of every
- * step; NULL: (3.4445, -4.7750, 2.0315) in each.  eps > 0: a zero matrix gives zeros.  Coefficients that could carry singular
- * values past 2^100 are refused, except for F64.  A matrix that holds an infinity or NaN gives non-finite values in its own
- * result only.  O may be G (same ld and stride).  work: as above, gpx_orthogonalize_work bytes. */
+ * step; NULL: (3.4445, -4.7750, 2.0315) in each.  Coefficients that could carry singular values past 2^100 are refused,
+ * except for F64.  eps >= 1e-300: a zero matrix gives zeros (and so does one of F64 whose squares sum past 1.8e308).  A
+ * matrix that holds an infinity or NaN gives non-finite values in its own result only.  O may be G (same ld and stride).
+ * work: as above, gpx_orthogonalize_work bytes. */
 int gpx_orthogonalize_work(int dtype, int64_t batch, int64_t M, int64_t N, int64_t* work_bytes);
 int gpx_orthogonalize(int dtype, int64_t batch, int64_t M, int64_t N, const void* G, int64_t ldg, int64_t stride_g, int steps,
                       const double* coef, double eps, void* O, int64_t ldo, int64_t stride_o, void* work, int64_t work_bytes,

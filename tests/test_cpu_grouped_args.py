@@ -45,6 +45,19 @@ def test_orthogonalize_refuses(bad):
     assert ortho(**bad) == 1
 
 
+@pytest.mark.parametrize("call,bad", [(gemm, dict(ldx=(1 << 32) + 1)), (gemm, dict(ldw=1 << 62)), (gemm, dict(ldy=1 << 61)), (gemm, dict(sw=1 << 60)),
+                                      (dw, dict(N=5, ldc=1 << 62)), (dw, dict(ldx=1 << 61)), (dw, dict(ldz=1 << 61)), (dw, dict(sc=1 << 60)),
+                                      (ortho, dict(N=5, ldo=1 << 62)), (ortho, dict(ldg=1 << 61)), (ortho, dict(sg=1 << 60)),
+                                      (ortho, dict(so=1 << 60))], ids=str)
+def test_strides_whose_products_would_wrap_are_refused(call, bad):
+    assert call(**bad) == 1
+
+
+def test_an_eps_whose_inverse_overflows_is_refused():
+    assert ortho(eps=1e-305) == 1
+    assert ortho(eps=5e-324) == 1
+
+
 def test_orthogonalize_refuses_non_finite_coefficients():
     for v in (np.nan, np.inf):
         c = np.array([1.0, 2.0, 3.0, 1.0, v, 3.0])
