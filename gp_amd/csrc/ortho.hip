@@ -105,13 +105,18 @@ __global__ __launch_bounds__(256) void ortho_normalize_kernel(const T* G, long l
 // product of floats here, the three that the split needs leave a factor of five.  The host bounds the singular values of
 // every iterate from the coefficients and places the largest possible element at 2^15: nothing overflows, and the smallest
 // step of the second plane is 2^-39 of that bound.
-// bf16: X is kept as the same two planes, but apart, and the products take the first one only, values rounded to 11 bits, one
-// matrix product instead of three and half the bytes.  That rounding is an eighth of the one that the bf16 matrix itself has
-// behind it, and the result is rounded to 8 bits.  Where X's own bits count, both planes are used: in a X, and in the diagonal of
-// b A + c A A, the largest of its elements, which is kept in floats beside that matrix (zero in it) and applied with a X.
-// 300 x 2000, six steps, error before the result's own rounding of 1.66e-3: 2.0e-3 with the diagonal rounded, 7.3e-4 without.
-// 16 matrices of 1024 x 2816: 2.61 -> 1.45 ms; off from 64 bits by 1.80e-3, 1.66e-3 of it the rounding of the result; half a step
-// of the input moves the result by 4e-3 (by 4e-2 where the singular values span five orders of magnitude: 1.78e-3 here).
+// bf16: the products take values rounded to 11 bits, one f16 plane under the same powers of two: one matrix product instead of
+// three and half the bytes.  That rounding is an eighth of the one that the bf16 matrix itself has behind it, and the result is
+// rounded to 8 bits.  More is kept where it counts:
+// - X itself has a second plane of 8-bit floats, 15 bits in all, and a X is formed from both: small singular values grow by a
+//   in every step, and what rounding adds to them grows with them (five orders of magnitude of singular values, 300 x 2000,
+//   relative error of the result: 1.06e-2 with 11 bits of X, 1.9e-3 with 15 or 22, its own rounding 1.66e-3).  X_0 needs none,
+//   the 8 bits of bf16 times a power of two; nor does the last iterate, which grows once more only (1.88e-3 -> 1.93e-3);
+// - the largest elements of A and of b A + c A A, their diagonals, are kept in floats beside the matrices (zero in them) and
+//   applied where the products' results are written (six steps, 300 x 2000: 2.0e-3 without, 7e-4 with, before the result's rounding).
+// 16 matrices of 1024 x 2816: 2.61 -> 1.32 ms (two f16 planes of X: 1.44; the second plane through the caches: 0.03 more, it only
+// sweeps X and A out of them); off from 64 bits by 1.73e-3, 1.66e-3 of it the rounding of the result; half a step of the input
+// moves the result by 4e-3.
 template <class F> struct Iterate;
 // v = h + l.  The compiler may form a converted product in one rounding and the product itself in two; h has to be one value
 // for both planes (told apart at ties, the planes would disagree by a step of the first one).
@@ -121,14 +126,25 @@ __device__ __forceinline__ void split(float v, _Float16& h, _Float16& l) {
     h = __builtin_bit_cast(_Float16, (unsigned short)bits);
     l = (_Float16)(v - (float)h);
 }
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+// the same for two neighbours, without rounding what is left
+__device__ __forceinline__ v2h split2(v2f v, v2f& left) {
+    unsigned bits = __builtin_bit_cast(unsigned, __builtin_convertvector(v, v2h));
+    asm("" : "+v"(bits));
+    const v2h h = __builtin_bit_cast(v2h, bits);
+    left[0] = v[0] - (float)h[0];
+    left[1] = v[1] - (float)h[1];
+    return h;
+}
 template <> struct Iterate<double> {
-    static constexpr int PAD = 2, PLANES = 1;
+    static constexpr int PAD = 2;
     __device__ static void store(char* row, int j, double v) { reinterpret_cast<double*>(row)[j] = v; }
     __device__ static double load(const char* row, int j) { return reinterpret_cast<const double*>(row)[j]; }
     static long bytes(long cols) { return cols * 8; }
 };
 template <> struct Iterate<mm::Split> {
-    static constexpr int PAD = 32, PLANES = 1;
+    static constexpr int PAD = 32;
     __device__ static long at(int j) { return (long)(j >> 5) * 64 + (j & 31); }
     __device__ static void store(char* row, int j, float v) {
         _Float16* p = reinterpret_cast<_Float16*>(row) + at(j);
@@ -140,20 +156,22 @@ template <> struct Iterate<mm::Split> {
     }
     static long bytes(long cols) { return cols * 4; }
     // eight neighbours from column j on, j a multiple of 8
-    __device__ static void store8(char* row, long, int j, const float (&v)[8]) {
+    __device__ static void store8(char* row, char*, int j, const float (&v)[8]) {
         mm::v8h h, l;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-            _Float16 a, b;
-            split(v[x], a, b);
-            h[x] = a;
-            l[x] = b;
+        for (int x = 0; x < 8; x += 2) {
+            v2f left;
+            const v2h a = split2(v2f{v[x], v[x + 1]}, left), b = __builtin_convertvector(left, v2h);
+            h[x] = a[0];
+            h[x + 1] = a[1];
+            l[x] = b[0];
+            l[x + 1] = b[1];
         }
         _Float16* p = reinterpret_cast<_Float16*>(row) + at(j);
         *reinterpret_cast<mm::v8h*>(p) = h;
         *reinterpret_cast<mm::v8h*>(p + 32) = l;
     }
-    __device__ static void add8(const char* row, long, int j, const float (&by)[8], float (&v)[8]) {   // v += by * row
+    __device__ static void add8(const char* row, const char*, int j, const float (&by)[8], float (&v)[8]) {   // v += by * row
         const _Float16* p = reinterpret_cast<const _Float16*>(row) + at(j);
         const mm::v8h h = *reinterpret_cast<const mm::v8h*>(p), l = *reinterpret_cast<const mm::v8h*>(p + 32);
 #pragma unroll
@@ -161,27 +179,41 @@ template <> struct Iterate<mm::Split> {
     }
 };
 template <> struct Iterate<mm::Rounded> {
-    static constexpr int PAD = 8, PLANES = 2;
+    static constexpr int PAD = 8;
     static long bytes(long cols) { return cols * 2; }
-    // lo: bytes from the first plane to the second, 0 where there is none (the square factors)
-    __device__ static void store8(char* row, long lo, int j, const float (&v)[8]) {
-        mm::v8h h, l;
+    // lo: the row in the second plane, or null: 2^4 times what the first rounding leaves (2^4 at most, values stay below 2^15)
+    // as e4m3 values (448 at most)
+    __device__ static void store8(char* row, char* lo, int j, const float (&v)[8]) {
+        mm::v8h h;
+        v2f left[4];
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-            _Float16 a, b;
-            split(v[x], a, b);
-            h[x] = a;
-            l[x] = b;
+        for (int x = 0; x < 4; ++x) {
+            const v2h a = split2(v2f{v[2 * x], v[2 * x + 1]}, left[x]);
+            h[2 * x] = a[0];
+            h[2 * x + 1] = a[1];
+            left[x][0] *= 16.0f;
+            left[x][1] *= 16.0f;
         }
         *reinterpret_cast<mm::v8h*>(row + j * 2) = h;
-        if (lo) *reinterpret_cast<mm::v8h*>(row + lo + j * 2) = l;
-    }
-    __device__ static void add8(const char* row, long lo, int j, const float (&by)[8], float (&v)[8]) {
-        const mm::v8h h = *reinterpret_cast<const mm::v8h*>(row + j * 2);
-        mm::v8h l = {};
-        if (lo) l = *reinterpret_cast<const mm::v8h*>(row + lo + j * 2);
+        if (lo) {
+            int w[2];
 #pragma unroll
-        for (int x = 0; x < 8; ++x) v[x] += by[x] * ((float)h[x] + (float)l[x]);
+            for (int x = 0; x < 2; ++x)
+                w[x] = __builtin_amdgcn_cvt_pk_fp8_f32(left[2 * x + 1][0], left[2 * x + 1][1],
+                                                       __builtin_amdgcn_cvt_pk_fp8_f32(left[2 * x][0], left[2 * x][1], 0, false), true);
+            __builtin_nontemporal_store((long)(unsigned)w[0] | (long)w[1] << 32, reinterpret_cast<long*>(lo + j));
+        }
+    }
+    __device__ static void add8(const char* row, const char* lo, int j, const float (&by)[8], float (&v)[8]) {
+        const mm::v8h h = *reinterpret_cast<const mm::v8h*>(row + j * 2);
+        const long both = lo ? __builtin_nontemporal_load(reinterpret_cast<const long*>(lo + j)) : 0;
+        const int w[2] = {(int)both, (int)(both >> 32)};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const auto l = x % 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(w[x / 2], true) : __builtin_amdgcn_cvt_pk_f32_fp8(w[x / 2], false);
+            v[2 * x] += by[2 * x] * ((float)h[2 * x] + 0.0625f * l[0]);
+            v[2 * x + 1] += by[2 * x + 1] * ((float)h[2 * x + 1] + 0.0625f * l[1]);
+        }
     }
 };
 template <class F> int padded(int cols) { return (cols + Iterate<F>::PAD - 1) / Iterate<F>::PAD * Iterate<F>::PAD; }
@@ -189,8 +221,15 @@ template <class F> int padded(int cols) { return (cols + Iterate<F>::PAD - 1) / 
 template <class T, class F>
 __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ G, long ldg, long stride_g, int rows, int cols, int pcols,
                                                           const double* __restrict__ part, int parts, double eps, double scale, char* __restrict__ X,
-                                                          long ldx, long stride_x, long lo) {
-    const Factor by(scale / (norm_of(part + blockIdx.y * kParts, parts) + eps));
+                                                          long ldx, long stride_x, float* __restrict__ first) {
+    const double norm = norm_of(part + blockIdx.y * kParts, parts) + eps;
+    double factor = scale / norm;
+    if constexpr (__is_same(F, mm::Rounded)) {   // a power of two, so that bf16 values pass into f16 as they are; the rest is `first`
+        const int e = isfinite(norm) ? ilogb(norm) : 0;
+        if (isfinite(norm)) factor = ldexp(scale, -e);
+        if (blockIdx.x == 0 && threadIdx.x == 0) first[blockIdx.y] = (float)(ldexp(1.0, e) / norm);
+    }
+    const Factor by(factor);
     each_run(rows, pcols, blockIdx.x * 256L + threadIdx.x, gridDim.x * 256L, [&](int r, int c) {
         T v[8];
         load_run(G + blockIdx.y * stride_g + r * ldg + c, cols - c, v);
@@ -199,7 +238,7 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ 
             float w[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = by.times((float)v[e]);
-            Iterate<F>::store8(x, lo, c, w);
+            Iterate<F>::store8(x, nullptr, c, w);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -210,16 +249,17 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ 
 
 // D = c1 P Q^T + c2 E over a batch, E and D in the format F, or (LAST) D in the type O of the result.
 // SYM: D is symmetric; tiles on and below the diagonal are computed, and those below it stored on both sides.
-// diag (Rounded only): a symmetric product with E moves its diagonal there, in floats; the product with X adds c1 diag to c2,
-// by the rows of D where the square factor is on the left, by its columns where it is on the right (QKC).
+// Rounded: every square matrix has its diagonal, in floats, beside it, and zeros in its place.  A symmetric product leaves its own
+// in diag_out; the square of A + diag(d) is A A + (d_i + d_j) A_ij + d_i^2, and diag(d) X is added to the product with X, by the
+// rows of D where the square matrix is on the left, by its columns where it is on the right (QKC).
 struct OrthoArgs {
     const char* P; const char* Q; const char* E; char* D;
     long ldp, ldq, lde, ldd, sp, sq, se, sd;   // bytes
-    long loe, lod;                             // from the first plane of E and D to the second, where there is one
     int I, J, K, batch;
     double c1, c2;
-    float* diag;
-    long sdiag;   // floats
+    const float* diag; float* diag_out;        // min(rows, cols) per matrix
+    const char* Elo; char* Dlo;                // second planes of X, half as wide, or null
+    const float* first;                        // first step: what is missing from X, per matrix
 };
 template <class F, class O, bool LAST, int B, int WR, int WC, int ST, int KG, bool PKC, bool QKC, bool SYM>
 __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) > 128 * 64 ? 1 : 2) void ortho_mm_kernel(const OrthoArgs g) {
@@ -272,7 +312,14 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
     t.clear();
     if constexpr (KG > 1) t.run_groups(lds, p, q, g.K);
     else t.run_direct(lds, p, q, g.K);
-    const one c1 = (one)g.c1, c2 = (one)g.c2;
+    one c1 = (one)g.c1, c2 = (one)g.c2;
+    if constexpr (__is_same(F, mm::Rounded)) {
+        if (g.first) {
+            const float m = g.first[mat];
+            c1 *= SYM ? m * m : m;
+            c2 *= m;
+        }
+    }
     const char* E = g.E + mat * g.se;
     char* D = g.D + mat * g.sd;
     if constexpr (!Tile::SWAP) {
@@ -280,11 +327,17 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
         // tile too (single elements from the accumulators: 90 us for a 256 x 256 tile, most of it the mirrored stores).
         float* slab = reinterpret_cast<float*>(lds);
         constexpr int NT = Tile::THREADS, R = Tile::SLAB_ROWS;
-        constexpr bool DIAG = __is_same(F, mm::Rounded);
-        float* diag = DIAG && g.diag ? g.diag + mat * g.sdiag : nullptr;
-        float all[8];
+        constexpr bool DIAG = __is_same(F, mm::Rounded), LOW = DIAG && !SYM;
+        const float* diag = DIAG && g.diag ? g.diag + mat * (long)(SYM ? g.I : g.K) : nullptr;
+        float* diag_out = DIAG && SYM ? g.diag_out + mat * (long)g.I : nullptr;
+        auto factors = [&](int i, int j, int exist, float (&by)[8]) {   // of E(i, j..j+7)
 #pragma unroll
-        for (int x = 0; x < 8; ++x) all[x] = c2;
+            for (int x = 0; x < 8; ++x) by[x] = 0.0f;
+            if constexpr (DIAG && (SYM || QKC)) load_run(diag + j, exist, by);
+            const float of_row = DIAG && (SYM || !QKC) ? diag[i] : 0.0f;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) by[x] = DIAG ? c2 + c1 * (of_row + by[x]) : c2;
+        };
         for (int pass = 0; pass < WR; ++pass) {
             const int ib = i0 + pass * R;
             __syncthreads();
@@ -300,20 +353,18 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
                     v[x] = c1 * lo[x];
                     v[4 + x] = c1 * hi[x];
                 }
-                if constexpr (DIAG && !SYM) {
+                if (c2 != 0.0f || (DIAG && diag)) {
                     float by[8];
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) by[x] = c2 + c1 * (!QKC ? diag[i] : j + x < g.J ? diag[j + x] : 0.0f);
-                    Iterate<F>::add8(E + i * g.lde, g.loe, j, by, v);
-                } else {
-                    if (c2 != 0.0f) Iterate<F>::add8(E + i * g.lde, g.loe, j, all, v);
+                    factors(i, j, g.J - j, by);
+                    Iterate<F>::add8(E + i * g.lde, LOW && g.Elo ? g.Elo + (mat * g.se + i * g.lde) / 2 : nullptr, j, by, v);
                 }
                 if constexpr (DIAG && SYM) {
-                    if (diag && i >= j && i < j + 8) {
+                    if (i >= j && i < j + 8) {
+                        const float d = diag ? diag[i] : 0.0f;
 #pragma unroll
                         for (int x = 0; x < 8; ++x)
                             if (i == j + x) {
-                                diag[i] = v[x];
+                                diag_out[i] = v[x] + (c2 + c1 * d) * d;
                                 v[x] = 0.0f;
                             }
                     }
@@ -334,7 +385,7 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
                             if (j + x < g.J) d[x] = (O)v[x];
                     }
                 } else {
-                    Iterate<F>::store8(D + i * g.ldd, g.lod, j, v);
+                    Iterate<F>::store8(D + i * g.ldd, LOW && g.Dlo ? g.Dlo + (mat * g.sd + i * g.ldd) / 2 : nullptr, j, v);
                 }
             }
             if (SYM && ti != tj) {   // D(j, i): E is symmetric to the bit, so both triangles are
@@ -346,8 +397,12 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
                     float v[8];
 #pragma unroll
                     for (int x = 0; x < 8; ++x) v[x] = c1 * slab[Tile::slab_at(il + x, jl)];
-                    if (c2 != 0.0f) Iterate<F>::add8(E + j * g.lde, g.loe, i, all, v);
-                    Iterate<F>::store8(D + j * g.ldd, g.lod, i, v);
+                    if (c2 != 0.0f || (DIAG && diag)) {
+                        float by[8];
+                        factors(j, i, g.I - i, by);
+                        Iterate<F>::add8(E + j * g.lde, nullptr, i, by, v);
+                    }
+                    Iterate<F>::store8(D + j * g.ldd, nullptr, i, v);
                 }
             }
         }
@@ -374,8 +429,8 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
 }
 
 struct OrthoWork {   // offsets and strides in bytes; rows of the iterates padded to whole blocks
-    long part, x[2], a, b, diag, total;
-    long ldx, sx, lda, sa, lo;   // lo: from the first plane of X to the second
+    long part, x[2], lo[2], a, b, diag[2], first, total;   // lo: second planes of x; diag: of a and b; first: see OrthoArgs (Rounded)
+    long ldx, sx, lda, sa;
 };
 // Rows of a power of two of bytes would meet in few memory channels: the K step of a tile reads 128 bytes of every row.
 template <class F> long row_bytes(int cols) {
@@ -392,12 +447,16 @@ template <class F> OrthoWork ortho_work_of(long batch, int rows, int cols) {
     o.sa = o.lda * s;
     o.part = 0;
     o.x[0] = up(batch * kParts * 8);
-    o.lo = Iterate<F>::PLANES == 2 ? up(batch * o.sx) : 0;
-    o.x[1] = o.x[0] + Iterate<F>::PLANES * up(batch * o.sx);
-    o.a = o.x[1] + Iterate<F>::PLANES * up(batch * o.sx);
+    o.x[1] = o.x[0] + up(batch * o.sx);
+    const long low = __is_same(F, mm::Rounded) ? up(batch * o.sx / 2) : 0;
+    o.lo[0] = o.x[1] + up(batch * o.sx);
+    o.lo[1] = o.lo[0] + low;
+    o.a = o.lo[1] + low;
     o.b = o.a + up(batch * o.sa);
-    o.diag = o.b + up(batch * o.sa);
-    o.total = o.diag + (Iterate<F>::PLANES == 2 ? up(batch * s * 4) : 0);
+    o.diag[0] = o.b + up(batch * o.sa);
+    o.diag[1] = o.diag[0] + (__is_same(F, mm::Rounded) ? up(batch * s * 4) : 0);
+    o.first = o.diag[1] + (o.diag[1] - o.diag[0]);
+    o.total = o.first + (__is_same(F, mm::Rounded) ? up(batch * 4) : 0);
     return o;
 }
 OrthoWork ortho_work(int dtype, long batch, int rows, int cols) {
@@ -651,7 +710,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
             float w[8];
 #pragma unroll
             for (int x = 0; x < 8; ++x) w[x] = by.times((float)v[x]);
-            Iterate<mm::Split>::store8(X + row * ldx, 0, c, w);
+            Iterate<mm::Split>::store8(X + row * ldx, nullptr, c, w);
         }
     });
     __syncthreads();
@@ -826,25 +885,31 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
         return GPX_OK;
     }
     char* x[2] = {work + o.x[0], work + o.x[1]};
+    constexpr bool low = __is_same(F, mm::Rounded);
+    float* first = low ? reinterpret_cast<float*>(work + o.first) : nullptr;
     char *a = work + o.a, *b = work + o.b;
-    float* diag = Iterate<F>::PLANES == 2 ? reinterpret_cast<float*>(work + o.diag) : nullptr;
-    ortho_scale_kernel<T, F><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, padded<F>(cols), part, parts, eps, f.start, x[0], o.ldx, o.sx, o.lo);
+    float *da = reinterpret_cast<float*>(work + o.diag[0]), *db = reinterpret_cast<float*>(work + o.diag[1]);   // (Rounded)
+    ortho_scale_kernel<T, F><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, padded<F>(cols), part, parts, eps, f.start, x[0], o.ldx, o.sx, first);
     HIP_TRY(hipGetLastError());
     const bool tall = rows > cols;
     const int s = std::min(rows, cols), l = std::max(rows, cols);
     for (int k = 0; k < steps; ++k) {
         char *from = x[k & 1], *to = x[~k & 1];
-        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, 0, 0, s, s, l, batch, f.gram[k], 0.0, nullptr, 0};
+        // X_0 is exact in one plane; the last iterate, which one step is left to work on, has no second one either
+        char* from_lo = low && k > 0 && k + 1 < steps ? work + o.lo[k & 1] : nullptr;
+        char* to_lo = low && k + 2 < steps ? work + o.lo[~k & 1] : nullptr;
+        const float* missing = k == 0 ? first : nullptr;
+        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, s, s, l, batch, f.gram[k], 0.0, nullptr, da, nullptr, nullptr, missing};
         int rc = tall ? launch<F, F, false, false, false, true>(st, gram, batch) : launch<F, F, false, true, true, true>(st, gram, batch);
         if (rc) return rc;
-        const OrthoArgs poly = {a, a, a, b, o.lda, o.lda, o.lda, o.lda, o.sa, o.sa, o.sa, o.sa, 0, 0, s, s, s, batch,
-                                f.square[k], f.linear[k], diag, s};
+        const OrthoArgs poly = {a, a, a, b, o.lda, o.lda, o.lda, o.lda, o.sa, o.sa, o.sa, o.sa, s, s, s, batch,
+                                f.square[k], f.linear[k], da, db, nullptr, nullptr, nullptr};
         if ((rc = launch<F, F, false, true, true, true>(st, poly, batch))) return rc;
         const bool last = k + 1 == steps;
         const long ldd = last ? ldo * (long)sizeof(T) : o.ldx, sd = last ? stride_o * (long)sizeof(T) : o.sx;
         char* d = last ? reinterpret_cast<char*>(O) : to;
-        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, o.lo, o.lo, rows, cols, s, batch, f.apply[k], f.keep[k], diag, s}
-                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, o.lo, o.lo, rows, cols, s, batch, f.apply[k], f.keep[k], diag, s};
+        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k], db, nullptr, from_lo, to_lo, missing}
+                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k], db, nullptr, from_lo, to_lo, missing};
         if (tall) rc = last ? launch<F, T, true, true, true, false>(st, apply, batch) : launch<F, F, false, true, true, false>(st, apply, batch);
         else rc = last ? launch<F, T, true, true, false, false>(st, apply, batch) : launch<F, F, false, true, false, false>(st, apply, batch);
         if (rc) return rc;
