@@ -114,7 +114,7 @@ __global__ __launch_bounds__(256) void ortho_normalize_kernel(const T* G, long l
 //   the 8 bits of bf16 times a power of two; nor does the last iterate, which grows once more only (1.88e-3 -> 1.93e-3);
 // - the largest elements of A and of b A + c A A, their diagonals, are kept in floats beside the matrices (zero in them) and
 //   applied where the products' results are written (six steps, 300 x 2000: 2.0e-3 without, 7e-4 with, before the result's rounding).
-// 16 matrices of 1024 x 2816: 2.61 -> 1.32 ms (two f16 planes of X: 1.44; the second plane through the caches: 0.03 more, it only
+// 16 matrices of 1024 x 2816: 2.61 -> 1.24 ms (the second plane through the caches: 0.03 more, it only
 // sweeps X and A out of them); off from 64 bits by 1.73e-3, 1.66e-3 of it the rounding of the result; half a step of the input
 // moves the result by 4e-3.
 template <class F> struct Iterate;
@@ -171,7 +171,7 @@ template <> struct Iterate<mm::Split> {
         *reinterpret_cast<mm::v8h*>(p) = h;
         *reinterpret_cast<mm::v8h*>(p + 32) = l;
     }
-    __device__ static void add8(const char* row, const char*, int j, const float (&by)[8], float (&v)[8]) {   // v += by * row
+    __device__ static void add8(const char* row, int j, const float (&by)[8], float (&v)[8]) {   // v += by * row
         const _Float16* p = reinterpret_cast<const _Float16*>(row) + at(j);
         const mm::v8h h = *reinterpret_cast<const mm::v8h*>(p), l = *reinterpret_cast<const mm::v8h*>(p + 32);
 #pragma unroll
@@ -204,15 +204,18 @@ template <> struct Iterate<mm::Rounded> {
             __builtin_nontemporal_store((long)(unsigned)w[0] | (long)w[1] << 32, reinterpret_cast<long*>(lo + j));
         }
     }
-    __device__ static void add8(const char* row, const char* lo, int j, const float (&by)[8], float (&v)[8]) {
+    __device__ static void add8(const char* row, int j, const float (&by)[8], float (&v)[8]) {
         const mm::v8h h = *reinterpret_cast<const mm::v8h*>(row + j * 2);
-        const long both = lo ? __builtin_nontemporal_load(reinterpret_cast<const long*>(lo + j)) : 0;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] += by[x] * (float)h[x];
+    }
+    __device__ static void add8_low(long both, const float (&by)[8], float (&v)[8]) {
         const int w[2] = {(int)both, (int)(both >> 32)};
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const auto l = x % 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(w[x / 2], true) : __builtin_amdgcn_cvt_pk_f32_fp8(w[x / 2], false);
-            v[2 * x] += by[2 * x] * ((float)h[2 * x] + 0.0625f * l[0]);
-            v[2 * x + 1] += by[2 * x + 1] * ((float)h[2 * x + 1] + 0.0625f * l[1]);
+            v[2 * x] += by[2 * x] * (0.0625f * l[0]);
+            v[2 * x + 1] += by[2 * x + 1] * (0.0625f * l[1]);
         }
     }
 };
@@ -310,8 +313,6 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
     typename Tile::OpQ q = {g.Q + mat * g.sq + (QKC ? j0 * g.ldq : j0 * (long)W), g.ldq, QKC ? min(g.J - j0, B) : min(Jp - j0, B) * WE, g.K};
     Tile t;
     t.clear();
-    if constexpr (KG > 1) t.run_groups(lds, p, q, g.K);
-    else t.run_direct(lds, p, q, g.K);
     one c1 = (one)g.c1, c2 = (one)g.c2;
     if constexpr (__is_same(F, mm::Rounded)) {
         if (g.first) {
@@ -320,6 +321,58 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
             c2 *= m;
         }
     }
+    constexpr bool DIAG = __is_same(F, mm::Rounded), LOW = DIAG && !SYM;
+    const float* diag = DIAG && g.diag ? g.diag + mat * (long)(SYM ? g.I : g.K) : nullptr;
+    if constexpr (LOW) {
+        // a X + diag(d) X: the elements of X that the tile adds are on chip as an operand in the steps whose k are the tile's rows
+        // (QKC: columns), and go to the accumulators from there, so that only the second plane is
+        // read behind the sums (with all of its loads on their way at once: 16 of 1024 x 2816 1319 -> 1236 us)
+        constexpr int TI = Tile::TI, TJ = Tile::TJ, mask = mm::swizzle_mask<_Float16>(B);
+        typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(Tile::wave_id()), r = lane & 15, k4 = lane >> 4 << 2;
+        const int iw = wave / WC * (B / WR), jw = wave % WC * (B / WC);
+        const float ratio = c2 / c1;
+        float f[QKC ? TJ : TI][QKC ? 4 : 1];
+#pragma unroll
+        for (int n = 0; n < (QKC ? TJ : TI); ++n)
+#pragma unroll
+            for (int x = 0; x < (QKC ? 4 : 1); ++x) f[n][x] = ratio + diag[min(QKC ? j0 + jw + 16 * n + k4 + x : i0 + iw + 16 * n + r, g.K - 1)];
+        auto add_x = [&](int s, const char* sp, const char* sq) {
+            if constexpr (!QKC) {
+#pragma unroll
+                for (int i = 0; i < TI; ++i) {
+                    const int row = i0 + iw + 16 * i, k = (row & 63) + r;
+                    if (row >> 6 != s) continue;
+#pragma unroll
+                    for (int j = 0; j < TJ; ++j) {
+                        const int col = jw + 16 * j + k4;
+                        const v4h h = *reinterpret_cast<const v4h*>(sq + k * (B * 2) + (((col >> 4) ^ (mm::strided_swizzle<_Float16>(k) & mask)) << 5) + (col & 15) * 2);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) t.acc[i][j][x] += f[i][0] * (float)h[x];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) {
+                    const int col = j0 + jw + 16 * j, k = (col & 63) + k4;
+                    if (col >> 6 != s) continue;
+#pragma unroll
+                    for (int i = 0; i < TI; ++i) {
+                        const int row = iw + 16 * i + r;
+                        const v4h h = *reinterpret_cast<const v4h*>(sp + row * 128 + (((k >> 3) ^ (row & 7)) << 4) + (k & 7) * 2);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) t.acc[i][j][x] += f[j][x] * (float)h[x];
+                    }
+                }
+            }
+        };
+        if constexpr (KG > 1) t.run_groups(lds, p, q, g.K, add_x);
+        else t.run_direct(lds, p, q, g.K, add_x);
+    } else if constexpr (KG > 1) {
+        t.run_groups(lds, p, q, g.K);
+    } else {
+        t.run_direct(lds, p, q, g.K);
+    }
     const char* E = g.E + mat * g.se;
     char* D = g.D + mat * g.sd;
     if constexpr (!Tile::SWAP) {
@@ -327,8 +380,6 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
         // tile too (single elements from the accumulators: 90 us for a 256 x 256 tile, most of it the mirrored stores).
         float* slab = reinterpret_cast<float*>(lds);
         constexpr int NT = Tile::THREADS, R = Tile::SLAB_ROWS;
-        constexpr bool DIAG = __is_same(F, mm::Rounded), LOW = DIAG && !SYM;
-        const float* diag = DIAG && g.diag ? g.diag + mat * (long)(SYM ? g.I : g.K) : nullptr;
         float* diag_out = DIAG && SYM ? g.diag_out + mat * (long)g.I : nullptr;
         auto factors = [&](int i, int j, int exist, float (&by)[8]) {   // of E(i, j..j+7)
 #pragma unroll
@@ -340,10 +391,24 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
         };
         for (int pass = 0; pass < WR; ++pass) {
             const int ib = i0 + pass * R;
+            constexpr int RUNS = R * (B / 8), TURNS = (RUNS + NT - 1) / NT;
+            long low[LOW ? TURNS : 1];   // E's second plane: from addresses that exist in any case, without a test that each load would wait behind
+            if constexpr (LOW) {
+                if (g.Elo) {
+#pragma unroll
+                    for (int n = 0; n < TURNS; ++n) {
+                        const int e = threadIdx.x + n * NT, i = min(ib + e / (B / 8), g.I - 1), j = min(j0 + e % (B / 8) * 8, Jp - 8);
+                        low[n] = __builtin_nontemporal_load(reinterpret_cast<const long*>(g.Elo + (mat * g.se + i * g.lde) / 2 + j));
+                    }
+                }
+            }
             __syncthreads();
             t.to_slab(slab, pass);
             __syncthreads();
-            for (int e = threadIdx.x; e < R * (B / 8); e += NT) {
+#pragma unroll
+            for (int n = 0; n < TURNS; ++n) {
+                const int e = threadIdx.x + n * NT;
+                if (RUNS % NT != 0 && e >= RUNS) continue;
                 const int il = e / (B / 8), i = ib + il, jl = e % (B / 8) * 8, j = j0 + jl;
                 if (i >= g.I || j >= Jp) continue;
                 float v[8];
@@ -353,10 +418,11 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
                     v[x] = c1 * lo[x];
                     v[4 + x] = c1 * hi[x];
                 }
-                if (c2 != 0.0f || (DIAG && diag)) {
+                if (LOW ? g.Elo != nullptr : c2 != 0.0f || (DIAG && diag)) {
                     float by[8];
                     factors(i, j, g.J - j, by);
-                    Iterate<F>::add8(E + i * g.lde, LOW && g.Elo ? g.Elo + (mat * g.se + i * g.lde) / 2 : nullptr, j, by, v);
+                    if constexpr (LOW) Iterate<F>::add8_low(low[n], by, v);
+                    else Iterate<F>::add8(E + i * g.lde, j, by, v);
                 }
                 if constexpr (DIAG && SYM) {
                     if (i >= j && i < j + 8) {
@@ -400,7 +466,7 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
                     if (c2 != 0.0f || (DIAG && diag)) {
                         float by[8];
                         factors(j, i, g.I - i, by);
-                        Iterate<F>::add8(E + j * g.lde, nullptr, i, by, v);
+                        Iterate<F>::add8(E + j * g.lde, i, by, v);
                     }
                     Iterate<F>::store8(D + j * g.ldd, nullptr, i, v);
                 }
@@ -566,7 +632,8 @@ bool ortho_factors(bool scaled, int steps, const double* coef, OrthoFactors& f) 
         const double next = slack * largest_value(a, b, c, top);
         if (scaled && !(std::max(next, top * largest_quadratic(b, c, top * top)) < 0x1p100)) return false;
         const int ea = scaled ? place(slack * top * top) : 0;
-        const int eb = scaled ? place(slack * largest_quadratic(b, c, top * top)) : 0;
+        // (no further below a than 2^-20: a X passes through accumulators in the square factor's scale)
+        const int eb = scaled ? place(slack * std::max(largest_quadratic(b, c, top * top), fabs(a) * 0x1p-20)) : 0;
         const int en = scaled && k + 1 < steps ? place(next) : 0;
         f.gram[k] = ldexp(1.0, ea - 2 * ex);
         f.square[k] = ldexp(c, eb - 2 * ea);
