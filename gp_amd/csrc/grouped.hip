@@ -22,6 +22,7 @@ struct GroupedArgs {
     long T;
     int groups, N, K;
     double alpha, beta;
+    int slots, most;   // see the two levels of tiles; 0: one
 };
 
 __device__ __forceinline__ long clamped(const int64_t* offsets, int g, long T) {
@@ -76,21 +77,55 @@ __device__ RowTile row_tile(const GroupScan& first, const int64_t* offsets, int 
 // column by column.  That order is walked in chunks of CHUNK tiles, what the chip holds at a time, and since workgroups go
 // round the 8 XCDs, XCD x takes the x-th eighth of every chunk: its CUs share 8 row panels and a few column panels in their L2,
 // and all XCDs stay in one neighbourhood of X and W in the cache behind them.
-template <int BM, int CHUNK, int HIGH = 8> __device__ RowTile find_tile(const int64_t* offsets, int groups, long T, int nt, int& col) {
-    const GroupScan first(offsets, groups, T, 0, BM);
+//
+// Two levels (slots > 0): what is left behind the last whole round of `slots` tiles, if it is no more than `most`, is done in
+// tiles of half the rows and columns by a second launch (REST; the tiles of the first are 2 BM high then): a few large tiles
+// would take the time of a whole round (bf16 4 x 2048 x 4096 x 2304: 194 -> 174 us,
+// f32 5000 x 2000 x 2000: 356 -> 327).
+template <int BM, int CHUNK, int HIGH = 8, bool REST = false>
+__device__ RowTile find_tile(const int64_t* offsets, int groups, long T, int nt, int& col, int slots = 0, int most = 0) {
+    constexpr int UNIT = REST ? 2 * BM : BM;
+    const GroupScan first(offsets, groups, T, 0, UNIT);
     long total = __shfl(first.sum, 63, 64);
-    for (int g0 = 64; g0 < groups; g0 += 64) total += __shfl(GroupScan(offsets, groups, T, g0, BM).sum, 63, 64);
-    const long all = total * nt;
-    const long start = (long)(blockIdx.x / CHUNK) * CHUNK;
-    const unsigned here = (unsigned)min((long)CHUNK, all - start), xcd = blockIdx.x & 7;
-    if (start >= all) return {-1, 0, 0};
-    const unsigned in_chunk = here * xcd / 8 + (blockIdx.x % CHUNK >> 3);
-    if (in_chunk >= here * (xcd + 1) / 8) return {-1, 0, 0};
+    for (int g0 = 64; g0 < groups; g0 += 64) total += __shfl(GroupScan(offsets, groups, T, g0, UNIT).sum, 63, 64);
+    long all = total * nt, start, last;
+    const unsigned xcd = blockIdx.x & 7;
+    if (slots) {
+        const int left = (int)(all % slots);
+        const bool two = left <= most && left < all;
+        if (REST) {
+            if (!two) return {-1, 0, 0};
+            start = all - left;
+        } else if (two) {
+            all -= left;
+        }
+    }
+    unsigned in_chunk;
+    if (!REST) {
+        start = (long)(blockIdx.x / CHUNK) * CHUNK;
+        if (start >= all) return {-1, 0, 0};
+        const unsigned here = (unsigned)min((long)CHUNK, all - start);
+        in_chunk = here * xcd / 8 + (blockIdx.x % CHUNK >> 3);
+        last = here * (xcd + 1) / 8;
+    } else {   // four workgroups a tile
+        const unsigned here = (unsigned)(all - start);
+        in_chunk = here * xcd / 8 + (blockIdx.x >> 5);
+        last = here * (xcd + 1) / 8;
+    }
+    if (in_chunk >= last) return {-1, 0, 0};
     const long o = start + in_chunk;
     const unsigned band = (unsigned)(o / (HIGH * nt)), in = (unsigned)(o - (long)band * HIGH * nt);
     const unsigned high = (unsigned)min((long)HIGH, total - (long)HIGH * band);
     col = __builtin_amdgcn_readfirstlane((int)(in / high));
-    return row_tile(first, offsets, groups, T, (long)HIGH * band + in % high, BM);
+    RowTile t = row_tile(first, offsets, groups, T, (long)HIGH * band + in % high, UNIT);
+    if (REST) {
+        const int down = blockIdx.x >> 4 & 1;
+        col = 2 * col + (blockIdx.x >> 3 & 1);
+        t.row0 += down * BM;
+        t.rows = min(t.rows - down * BM, BM);
+        if (t.rows <= 0) t.group = -1;
+    }
+    return t;
 }
 
 // p[0..R) (those j + x < N) = alpha v + beta p in the type O, R of them 16 bytes, at any alignment.  PAST: whole runs go past the
@@ -151,14 +186,15 @@ constexpr int kShortSub = 8;
 
 template <class Tile> constexpr int tile_lds() { return Tile::SWAP || Tile::LDS > Tile::SLAB ? Tile::LDS : Tile::SLAB; }
 
-template <class T, int BM, int BN, int WR, int WC, int ST, int KG, bool WKC, bool DIRECT>
+template <class T, int BM, int BN, int WR, int WC, int ST, int KG, bool WKC, bool DIRECT, bool REST = false>
 __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : 2) void grouped_kernel(const GroupedArgs g) {
     typedef mm::Tile<T, BM, BN, WR, WC, true, WKC, ST, KG> Tile;
     __shared__ __attribute__((aligned(128))) char lds[tile_lds<Tile>()];
     int col = 0;
-    const RowTile rt = find_tile<BM, (BM * BN > 128 * 128 || KG > 1 ? 256 : 512)>(g.offsets, g.groups, g.T, (g.N + BN - 1) / BN, col);
-    if (rt.group < 0) return;
+    constexpr int CHUNK = BM * BN > 128 * 128 || KG > 1 ? 256 : 512, WIDTH = REST ? 2 * BN : BN;
+    const RowTile rt = find_tile<BM, CHUNK, 8, REST>(g.offsets, g.groups, g.T, (g.N + WIDTH - 1) / WIDTH, col, g.slots, g.most);
     const int n0 = col * BN, cols = min(g.N - n0, BN);
+    if (rt.group < 0 || (REST && cols <= 0)) return;
     typename Tile::OpP p = {g.X + rt.row0 * g.ldx, g.ldx, rt.rows, g.K};
     typename Tile::OpQ q = {g.W + rt.group * g.stride_w + (WKC ? n0 * g.ldw : n0 * (long)sizeof(T)), g.ldw, cols, g.K};
     Tile t;
@@ -388,32 +424,57 @@ double tile_time(const TileCost& c, double tiles, double steps) {
 }
 
 template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArgs& g) {
+    GroupedArgs a = g;
     // rows of X (k contiguous) and of W in 16-byte chunks, lane offsets of one K step within the buffer resource
     const long wn = w_kc ? g.K : g.N;   // W's contiguous extent
     const bool direct = whole_chunks(g.X, g.ldx, 0, g.K, sizeof(T)) && whole_chunks(g.W, g.ldw, g.stride_w, wn, sizeof(T)) &&
                         256 * g.ldx < (long)mm::kRange && 256 * g.ldw < (long)mm::kRange;
     const double busy = (double)std::min<long>(g.groups, g.T), steps = (double)((g.K * (long)sizeof(T) + 127) / 128);
-    auto time_of = [&](const TileCost& c) {   // half a row tile of every group is empty on average
-        const double mt = std::max(busy, g.T / (double)c.bm + 0.5 * busy);
-        return tile_time(c, mt * ((g.N + c.bn - 1) / c.bn), steps);
+    const TileCost* const costs = sizeof(T) == 2 ? kCost16 : sizeof(T) == 4 ? kCost32 : kCost64;
+    const int large = sizeof(T) == 2 ? 2 : 1;   // tiles that the next of the table is half of, in both directions
+    // whether so many tiles behind the last whole round are better done in the next smaller tile by a launch of their own, 5 us
+    auto better = [&](int i, double left) { return tile_time(costs[i + 1], 4.0 * left, steps) + 5.0 < tile_time(costs[i], left, steps); };
+    auto tiles_of = [&](const TileCost& c) {   // half a row tile of every group is empty on average
+        return std::max(busy, g.T / (double)c.bm + 0.5 * busy) * ((g.N + c.bn - 1) / c.bn);
     };
+    auto time_of = [&](const TileCost& c) { return tile_time(c, tiles_of(c), steps); };
     int rc = GPX_OK;
-    auto go = [&](auto bm, auto bn, auto wr, auto wc, auto stages, auto kgroups) {
+    auto go = [&](auto bm, auto bn, auto wr, auto wc, auto stages, auto kgroups, auto rest) {
         constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WR = decltype(wr)::value, WC = decltype(wc)::value, ST = decltype(stages)::value,
                       KG = decltype(kgroups)::value;
-        const long tiles = row_tiles(g.T, g.groups, BM) * ((g.N + BN - 1) / BN);
+        constexpr bool REST = decltype(rest)::value != 0;
+        const long tiles = REST ? 4L * a.most : row_tiles(g.T, g.groups, BM) * ((g.N + BN - 1) / BN);
         if (tiles >= (1L << 31) - 512) {
             rc = GPX_ERR_UNSUPPORTED;
             return;
         }
-        const unsigned grid = (unsigned)((tiles + 7) / 8 * 8);   // as many for every XCD
+        const unsigned grid = (unsigned)((tiles + 31) / 32 * 32);   // as many for every XCD (REST: whole tiles)
         constexpr int threads = WR * WC * 64 * KG;
-        if (w_kc && direct) grouped_kernel<T, BM, BN, WR, WC, ST, KG, true, true><<<grid, threads, 0, st>>>(g);
-        else if (direct) grouped_kernel<T, BM, BN, WR, WC, ST, KG, false, true><<<grid, threads, 0, st>>>(g);
-        else if constexpr (BM == 256 || KG > 1) rc = GPX_ERR_STATE;   // (never chosen for rows that are not direct)
-        else if (w_kc) grouped_kernel<T, BM, BN, WR, WC, 2, 1, true, false><<<grid, threads, 0, st>>>(g);
-        else grouped_kernel<T, BM, BN, WR, WC, 2, 1, false, false><<<grid, threads, 0, st>>>(g);
+        if (w_kc && direct) grouped_kernel<T, BM, BN, WR, WC, ST, KG, true, true, REST><<<grid, threads, 0, st>>>(a);
+        else if (direct) grouped_kernel<T, BM, BN, WR, WC, ST, KG, false, true, REST><<<grid, threads, 0, st>>>(a);
+        else if constexpr (BM == 256 || KG > 1 || REST) rc = GPX_ERR_STATE;   // (never chosen for rows that are not direct)
+        else if (w_kc) grouped_kernel<T, BM, BN, WR, WC, 2, 1, true, false, REST><<<grid, threads, 0, st>>>(a);
+        else grouped_kernel<T, BM, BN, WR, WC, 2, 1, false, false, REST><<<grid, threads, 0, st>>>(a);
     };
+    // The tile, or the larger one whose rest is done in smaller ones, if that saves more than the estimates are good for (chosen
+    // for any gain: 4 x 1000 x 2048 x 1000 in double 289 -> 297 us).
+    auto levels = [&](int best) {
+        if (!direct) return best;
+        double least = 0.93 * time_of(costs[best]);
+        for (int i = 0; i < large; ++i) {
+            const double tiles = tiles_of(costs[i]), left = fmod(tiles, costs[i].slots);
+            const double time = tile_time(costs[i], tiles - left, steps) + tile_time(costs[i + 1], 4.0 * left, steps) + 5.0;
+            if (tiles < costs[i].slots || left < 1.0 || time >= least) continue;
+            least = time;
+            best = i;
+            a.slots = costs[i].slots;
+            a.most = 0;
+            for (int n = 8; n < a.slots && better(i, n); n += 8) a.most = n;
+        }
+        return best;
+    };
+    constexpr Int<0> whole{};
+    constexpr Int<1> rest{};
     // from: rows that have to pass through registers take 128-tiles at most (20000 x 1001 x 2003 in bf16: 166 us, 256-tiles 241)
     auto best_of = [&](const TileCost* c, int from, int n, int not_this) {
         int best = from;
@@ -422,15 +483,21 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
         return best;
     };
     if constexpr (sizeof(T) == 2) {
-        switch (best_of(kCost16, direct ? 0 : 1, direct ? 8 : 5, w_kc ? 3 : 4)) {
-            case 0: go(Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{}, Int<1>{}); break;
-            case 1: go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<1>{}); break;
-            case 2: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<4>{}, Int<1>{}); break;
-            case 3: go(Int<32>{}, Int<128>{}, Int<1>{}, Int<4>{}, Int<4>{}, Int<1>{}); break;
-            case 4: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<4>{}, Int<1>{}); break;
-            case 5: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<3>{}, Int<4>{}); break;
-            case 6: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<4>{}); break;
-            default: go(Int<32>{}, Int<16>{}, Int<1>{}, Int<1>{}, Int<3>{}, Int<8>{});
+        switch (levels(best_of(kCost16, direct ? 0 : 1, direct ? 8 : 5, w_kc ? 3 : 4))) {
+            case 0:
+                go(Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{}, Int<2>{}, Int<1>{}, whole);
+                if (a.slots) go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<1>{}, rest);
+                break;
+            case 1:
+                go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<1>{}, whole);
+                if (a.slots) go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<4>{}, Int<1>{}, rest);
+                break;
+            case 2: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<4>{}, Int<1>{}, whole); break;
+            case 3: go(Int<32>{}, Int<128>{}, Int<1>{}, Int<4>{}, Int<4>{}, Int<1>{}, whole); break;
+            case 4: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<4>{}, Int<1>{}, whole); break;
+            case 5: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<3>{}, Int<4>{}, whole); break;
+            case 6: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<4>{}, whole); break;
+            default: go(Int<32>{}, Int<16>{}, Int<1>{}, Int<1>{}, Int<3>{}, Int<8>{}, whole);
         }
     } else if (const long units = row_tiles(g.T, g.groups, 32 * kShortSub) * ((g.N + 63) / 64);
                direct && g.K * (long)sizeof(T) <= 512 && 32 * g.ldy < (long)mm::kRange && g.K > 0 && units >= 512 && units < (1L << 31) - 512) {
@@ -439,12 +506,15 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
         if (w_kc) grouped_short_kernel<T, true><<<grid, 256, 0, st>>>(g);
         else grouped_short_kernel<T, false><<<grid, 256, 0, st>>>(g);
     } else {
-        switch (best_of(sizeof(T) == 4 ? kCost32 : kCost64, 0, direct ? 5 : 3, -1)) {
-            case 0: go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<1>{}); break;
-            case 1: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<1>{}); break;
-            case 2: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<4>{}, Int<1>{}); break;
-            case 3: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<3>{}, Int<4>{}); break;
-            default: go(Int<32>{}, Int<16>{}, Int<1>{}, Int<1>{}, Int<3>{}, Int<8>{});
+        switch (levels(best_of(costs, 0, direct ? 5 : 3, -1))) {
+            case 0:
+                go(Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<1>{}, whole);
+                if (a.slots) go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<1>{}, rest);
+                break;
+            case 1: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<1>{}, whole); break;
+            case 2: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<4>{}, Int<1>{}, whole); break;
+            case 3: go(Int<32>{}, Int<64>{}, Int<1>{}, Int<4>{}, Int<3>{}, Int<4>{}, whole); break;
+            default: go(Int<32>{}, Int<16>{}, Int<1>{}, Int<1>{}, Int<3>{}, Int<8>{}, whole);
         }
     }
     HIP_TRY(hipGetLastError());
@@ -562,7 +632,7 @@ extern "C" int gpx_grouped_gemm(int dtype, int w_kc, int64_t groups, int64_t T, 
     StreamDevice dev(static_cast<hipStream_t>(hip_stream));
     if (dev.status) return dev.status;
     GroupedArgs g = {static_cast<const char*>(X), static_cast<const char*>(W), static_cast<char*>(Y), offsets, ldx * e, ldw * e,
-                     stride_w * e, ldy * e, T, (int)groups, (int)N, (int)K, alpha, beta};
+                     stride_w * e, ldy * e, T, (int)groups, (int)N, (int)K, alpha, beta, 0, 0};
     const hipStream_t st = static_cast<hipStream_t>(hip_stream);
     switch (dtype) {
         case GPX_F64: return grouped_typed<double>(st, w_kc != 0, g);

@@ -139,6 +139,22 @@ def test_grouped_gemm_on_a_full_chip(dtype, w_kc, sizes, n, k):
     check(c, *oracle.grouped_dw(x, out, off.tolist(), torch.zeros_like(c), alpha=0.25))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("w_kc", [True, False], ids=["kc", "nc"])
+@pytest.mark.parametrize("sizes,wide", [([4300], 2000), ([2100, 0, 2290], 2008), ([700, 900, 1300, 1210, 33], 1960)], ids=["g1", "g3", "g5"])
+def test_rest_of_a_round(dtype, w_kc, sizes, wide):
+    """A few tiles more than whole rounds of the chip, which are done in smaller ones; beta, ragged last tiles."""
+    lib = _lib()
+    n, k = (2 * wide, 2304) if dtype.itemsize == 2 else (wide, 512)
+    rows = 5 + sum(sizes) + 7
+    x, w = data(1, dtype, rows, k), data(2, dtype, len(sizes), *((n, k) if w_kc else (k, n)))
+    off, old = table(sizes, 5), data(3, dtype, rows, n)
+    flat, out = framed(old, 8, 16)
+    lib.grouped_gemm(x, w, off, out, w_kc=w_kc, alpha=0.5, beta=-1.0)
+    check(out, *oracle.grouped(x, w, off.tolist(), old, w_kc, 0.5, -1.0))
+    assert torch.equal(out[:5], old[:5]) and torch.equal(out[rows - 7:], old[rows - 7:]) and untouched(flat, out)
+
+
 @pytest.mark.parametrize("dtype", [torch.float64, torch.float32], ids=str)
 @pytest.mark.parametrize("w_kc", [True, False], ids=["kc", "nc"])
 @pytest.mark.parametrize("sizes,n,k", [([20000, 0, 31, 15000, 4997], 256, 50), ([33, 40000], 1000, 8), ([30001, 9000], 264, 64), ([40000, 1], 320, 32),
