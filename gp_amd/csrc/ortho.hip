@@ -105,15 +105,17 @@ __global__ __launch_bounds__(256) void ortho_normalize_kernel(const T* G, long l
 // product of floats here, the three that the split needs leave a factor of five.  The host bounds the singular values of
 // every iterate from the coefficients and places the largest possible element at 2^15: nothing overflows, and the smallest
 // step of the second plane is 2^-39 of that bound.
+// In both formats the largest elements of A and of b A + c A A, their diagonals, are kept in floats beside the matrices (zero in
+// them) and applied where the products' results are written.  Relative error of the result without and with that: f32, 16 x 208 in
+// three steps 1.2e-6 and 3.3e-7 (products of floats: 5.7e-7), 300 x 2000 in six 2.5e-6 and 6.6e-7 (2.9e-6); bf16, 300 x 2000 in six,
+// before the result is rounded, 2.0e-3 and 7e-4.  It costs 0.5 us of 21 for a small matrix, 0.8 % for one of 4096 x 4096.
 // bf16: the products take values rounded to 11 bits, one f16 plane under the same powers of two: one matrix product instead of
 // three and half the bytes.  That rounding is an eighth of the one that the bf16 matrix itself has behind it, and the result is
 // rounded to 8 bits.  More is kept where it counts:
-// - X itself has a second plane of 8-bit floats, 15 bits in all, and a X is formed from both: small singular values grow by a
+//   X itself has a second plane of 8-bit floats, 15 bits in all, and a X is formed from both: small singular values grow by a
 //   in every step, and what rounding adds to them grows with them (five orders of magnitude of singular values, 300 x 2000,
 //   relative error of the result: 1.06e-2 with 11 bits of X, 1.9e-3 with 15 or 22, its own rounding 1.66e-3).  X_0 needs none,
-//   the 8 bits of bf16 times a power of two; nor does the last iterate, which grows once more only (1.88e-3 -> 1.93e-3);
-// - the largest elements of A and of b A + c A A, their diagonals, are kept in floats beside the matrices (zero in them) and
-//   applied where the products' results are written (six steps, 300 x 2000: 2.0e-3 without, 7e-4 with, before the result's rounding).
+//   the 8 bits of bf16 times a power of two; nor does the last iterate, which grows once more only (1.88e-3 -> 1.93e-3).
 // 16 matrices of 1024 x 2816: 2.61 -> 1.24 ms (the second plane through the caches: 0.03 more, it only
 // sweeps X and A out of them); off from 64 bits by 1.73e-3, 1.66e-3 of it the rounding of the result; half a step of the input
 // moves the result by 4e-3.
@@ -252,7 +254,7 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ 
 
 // D = c1 P Q^T + c2 E over a batch, E and D in the format F, or (LAST) D in the type O of the result.
 // SYM: D is symmetric; tiles on and below the diagonal are computed, and those below it stored on both sides.
-// Rounded: every square matrix has its diagonal, in floats, beside it, and zeros in its place.  A symmetric product leaves its own
+// Not for doubles: every square matrix has its diagonal, in floats, beside it, and zeros in its place.  A symmetric product leaves its own
 // in diag_out; the square of A + diag(d) is A A + (d_i + d_j) A_ij + d_i^2, and diag(d) X is added to the product with X, by the
 // rows of D where the square matrix is on the left, by its columns where it is on the right (QKC).
 struct OrthoArgs {
@@ -321,7 +323,7 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
             c2 *= m;
         }
     }
-    constexpr bool DIAG = __is_same(F, mm::Rounded), LOW = DIAG && !SYM;
+    constexpr bool DIAG = !__is_same(F, double), LOW = __is_same(F, mm::Rounded) && !SYM;
     const float* diag = DIAG && g.diag ? g.diag + mat * (long)(SYM ? g.I : g.K) : nullptr;
     if constexpr (LOW) {
         // a X + diag(d) X: the elements of X that the tile adds are on chip as an operand in the steps whose k are the tile's rows
@@ -520,7 +522,7 @@ template <class F> OrthoWork ortho_work_of(long batch, int rows, int cols) {
     o.a = o.lo[1] + low;
     o.b = o.a + up(batch * o.sa);
     o.diag[0] = o.b + up(batch * o.sa);
-    o.diag[1] = o.diag[0] + (__is_same(F, mm::Rounded) ? up(batch * s * 4) : 0);
+    o.diag[1] = o.diag[0] + (__is_same(F, double) ? 0 : up(batch * s * 4));
     o.first = o.diag[1] + (o.diag[1] - o.diag[0]);
     o.total = o.first + (__is_same(F, mm::Rounded) ? up(batch * 4) : 0);
     return o;
@@ -655,7 +657,7 @@ int place(double bound) { return bound > 0.0 ? 14 - std::ilogb(bound) : 14; }
 // than their values so that neighbouring rows do not share banks.  Per step: A = X X^T, one 16 x 16 tile per wave and turn;
 // A <- b A + c A A from registers once every wave has read A; X <- a X + A X by blocks of 16 columns, each read whole into
 // registers by the one wave that overwrites it.  What bounds it is latency: 15 short products behind barriers.
-constexpr int kSmallWaves = 16, kSmallSide = 128, kSmallLds = 160 * 1024 - 512;
+constexpr int kSmallWaves = 16, kSmallSide = 128, kSmallLds = 160 * 1024 - 1536;
 struct OrthoSmallArgs {
     long ldg, stride_g, ldo, stride_o;   // elements
     int rows, cols, steps;
@@ -725,6 +727,7 @@ template <class T, int NB, bool TWO>
 __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* G, T* O, const OrthoSmallArgs g) {
     extern __shared__ __attribute__((aligned(128))) char lds[];
     __shared__ double ws[kSmallWaves];
+    __shared__ __attribute__((aligned(16))) float da[kSmallSide], db[kSmallSide];   // the diagonals, which A and B hold zeros for
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
     const bool tall = g.rows > g.cols;
     const int S = tall ? g.cols : g.rows, L = tall ? g.rows : g.cols;
@@ -791,7 +794,15 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
         ti[x] = i * 16;
         tj[x] = t * 16;
     }
-    auto store_both = [&](char* to, int i0, int j0, mm::v4f c) {
+    auto store_both = [&](char* to, float* diag, int i0, int j0, mm::v4f c) {
+        if (i0 == j0) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+                if (r == 4 * q + y) {
+                    diag[i0 + r] = c[y];
+                    c[y] = 0.0f;
+                }
+        }
         small_store4(to + (i0 + r) * lda, j0 + 4 * q, c);
         if (i0 != j0) {
 #pragma unroll
@@ -822,7 +833,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
 #pragma unroll
                 for (int w = 1; w < kSmallWaves; ++w) c += meet[(w * 3 + wave) * 64 + lane];
                 a[0] = c * g.gram[step];
-                store_both(A, ti[0], tj[0], a[0]);
+                store_both(A, da, ti[0], tj[0], a[0]);
             }
         } else {
 #pragma unroll
@@ -834,7 +845,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
                     c.add(small_frag_kc(X, ldx, tj[x], k, 0, lane), small_frag_kc(X, ldx, tj[x], k, 1, lane), small_frag_kc(X, ldx, ti[x], k, 0, lane),
                           small_frag_kc(X, ldx, ti[x], k, 1, lane));
                 a[x] = c.sum() * g.gram[step];
-                store_both(A, ti[x], tj[x], a[x]);
+                store_both(A, da, ti[x], tj[x], a[x]);
             }
         }
         __syncthreads();
@@ -846,15 +857,23 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
             for (int k = 0; k < NB; ++k)
                 c.add(small_frag_kc(A, lda, tj[x], k, 0, lane), small_frag_kc(A, lda, tj[x], k, 1, lane), small_frag_kc(A, lda, ti[x], k, 0, lane),
                       small_frag_kc(A, lda, ti[x], k, 1, lane));
-            b[x] = c.sum() * g.square[step] + a[x] * g.linear[step];
-            if (TWO) store_both(B, ti[x], tj[x], b[x]);
+            // A = A0 + diag(d): A A = A0 A0 + (d_i + d_j) A0, on the diagonal A0 A0 + d^2
+            const float di = da[ti[x] + r];
+            const mm::v4f dj = *reinterpret_cast<const mm::v4f*>(da + tj[x] + 4 * q);
+            const mm::v4f sum = c.sum();
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const float of_d = ti[x] + r == tj[x] + 4 * q + y ? di : di + dj[y];
+                b[x][y] = sum[y] * g.square[step] + a[x][y] * (g.linear[step] + g.square[step] * of_d);
+            }
+            if (TWO) store_both(B, db, ti[x], tj[x], b[x]);
         }
         __syncthreads();
         if constexpr (!TWO) {
 #pragma unroll
             for (int x = 0; x < TURNS; ++x) {
                 if (wave + kSmallWaves * x >= TILES) break;
-                store_both(B, ti[x], tj[x], b[x]);
+                store_both(B, db, ti[x], tj[x], b[x]);
             }
             __syncthreads();
         }
@@ -886,7 +905,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
 #pragma unroll
                 for (int k = 0; k < NB; ++k)
                     acc.add(qf[k][0], qf[k][1], small_frag_kc(B, lda, i0, k, 0, lane), small_frag_kc(B, lda, i0, k, 1, lane));
-                const mm::v4f c = acc.sum() * g.apply[step] + small_load4(X + (i0 + r) * ldx, j0 + 4 * q) * g.keep[step];
+                const mm::v4f c = acc.sum() * g.apply[step] + small_load4(X + (i0 + r) * ldx, j0 + 4 * q) * (g.keep[step] + g.apply[step] * db[i0 + r]);
                 if (last) {
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {

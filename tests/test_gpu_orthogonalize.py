@@ -87,7 +87,8 @@ def test_bfloat16_is_as_good_as_its_input(size, spread):
 
 
 @pytest.mark.parametrize("size", [(300, 2000), (2000, 300), (60, 2900), (700, 690)], ids=str)
-@pytest.mark.parametrize("steps,coef", [(6, None), (6, (1.5, -0.5, 0.0)), (1, (0.5, 3.0, -2.0))], ids=str)
+@pytest.mark.parametrize("steps,coef", [(6, None), (6, (1.5, -0.5, 0.0)), (1, (0.5, 3.0, -2.0)), (3, (1.0, 0.0, 0.0)),
+                                        (2, (1.0, 1e-12, 0.0))], ids=str)
 def test_bfloat16_rounds_no_diagonal(size, steps, coef):
     """A step rounds X (in two products), A and the square factor outside of its diagonal to 11 bits, each time by at most
     2^-11 / sqrt(3) of a value in the mean square, and a step passes an earlier error on without growth once the singular
@@ -98,6 +99,20 @@ def test_bfloat16_rounds_no_diagonal(size, steps, coef):
     off = lambda a: float(torch.linalg.norm(a.double() - want) / torch.linalg.norm(want))  # noqa: E731
     bound = (off(want.to(torch.bfloat16)) ** 2 + 4 * steps * 2.0 ** -22 / 3) ** 0.5
     assert off(lib.orthogonalize(g, torch.empty_like(g), steps=steps, coef=coef)) <= bound
+
+
+@pytest.mark.parametrize("size", [(17, 116), (16, 208), (35, 16), (128, 100), (30, 1791), (300, 700), (700, 290)], ids=str)
+@pytest.mark.parametrize("steps", [3, 6])
+def test_float32_rounds_no_diagonal(size, steps):
+    """As above with 22 bits, and products that leave out one of two second planes: 2^-21 / sqrt(3) a time, 2^-24 for the result.
+    A step's sum over the long side is taken in 32 bits, 32 terms of three products a time: 3 side / 32 roundings of at most
+    2^-24 of a sum of squares that only grows, added to the bound after the first run (30 x 1791 in six steps: 168 roundings
+    in each, sqrt(6 * 168 / 3) 2^-24 = 1.1e-6 beside the 1.35e-6 of the operands; it measured 1.56e-6)."""
+    lib = _lib()
+    g = data(1, torch.float32, *size)
+    want, _ = oracle.orthogonalize(g, steps=steps)
+    off = lambda a: float(torch.linalg.norm(a.double() - want) / torch.linalg.norm(want))  # noqa: E731
+    assert off(lib.orthogonalize(g, torch.empty_like(g), steps=steps)) <= (4 * steps * 2.0 ** -42 / 3 + (1 + steps * max(size) / 32) * 2.0 ** -48) ** 0.5
 
 
 def test_cubic_steps_reach_the_polar_factor():
