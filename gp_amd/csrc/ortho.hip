@@ -475,6 +475,7 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
             }
         }
     } else {
+        if (Tile::group() != 0) return;
         t.each([&](int i, int j, const one* v, auto) {
             i += i0;
             j += j0;
@@ -527,12 +528,6 @@ template <class F> OrthoWork ortho_work_of(long batch, int rows, int cols) {
     o.total = o.first + (__is_same(F, mm::Rounded) ? up(batch * 4) : 0);
     return o;
 }
-OrthoWork ortho_work(int dtype, long batch, int rows, int cols) {
-    return dtype == GPX_F64    ? ortho_work_of<double>(batch, rows, cols)
-           : dtype == GPX_BF16 ? ortho_work_of<mm::Rounded>(batch, rows, cols)
-                               : ortho_work_of<mm::Split>(batch, rows, cols);
-}
-
 // The tile of one product of split matrices, by the time it takes: rounds of workgroups over the 256 CUs, each of them K / 32
 // steps and an epilogue.  us per step and per epilogue, measured with S = 4096 and 1024 matrices: 256 (one workgroup of 8 waves
 // a CU) 2.3 / 20, 192 (one of 8) 1.65 / 10, 128 (two of 4; alone on its CU) 1.4 (0.85) / 8, 64 (two of 4, four LDS stages: a
@@ -583,9 +578,16 @@ template <class F, class O, bool LAST, bool PKC, bool QKC, bool SYM> int launch(
         else if (c == TILE64) GO(64, 2, 2, 4, 1);
         else if (c == TILE64_GROUPS) GO(64, 2, 2, 2, 4);
         else if constexpr (mm::Stored<F>::split) GO(192, 2, 4, 2, 1);
-    } else {   // doubles: 64 x 64 tiles cost 4 % on a full chip and are three to four times as many; 32 x 32 where these are few
+    } else {
+        // doubles: 64 x 64 tiles cost 4 % on a full chip and are three to four times as many; 32 x 32 where these are few; where those
+        // are few too, four groups of waves share a sum (512 x 512: 233 -> 193 us), or 16 single waves that of a 16 x 16 tile
+        // (1296 x 264: 274 -> 150, 16 x 4000: 422 -> 143)
         const long it = (g.I + 63) / 64, jt = (g.J + 63) / 64;
+        const long in = (g.I + 31) / 32, jn = (g.J + 31) / 32, small = (SYM ? in * (in + 1) / 2 : in * jn) * batch;
+        const long im = (g.I + 15) / 16, jm = (g.J + 15) / 16, tiny = (SYM ? im * (im + 1) / 2 : im * jm) * batch;
         if ((SYM ? it * (it + 1) / 2 : it * jt) * batch >= 192) GO(64, 2, 2, 2, 1);
+        else if (tiny <= 512 && g.K >= (tiny <= 256 ? 64 : 512)) GO(16, 1, 1, 2, 16);
+        else if (small <= 256 && g.K >= 128) GO(32, 2, 2, 2, 4);
         else GO(32, 2, 2, 4, 1);
     }
 #undef GO
@@ -721,6 +723,41 @@ __device__ __forceinline__ mm::v4f small_load4(const char* row, int j) {
     return v;
 }
 
+// the 16 x 16 tile c of a symmetric matrix into both of its places, its diagonal into diag
+__device__ __forceinline__ void small_store_both(char* to, int ld, float* diag, int i0, int j0, mm::v4f c, int lane) {
+    const int r = lane & 15, q = lane >> 4;
+    if (i0 == j0) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+            if (r == 4 * q + y) {
+                diag[i0 + r] = c[y];
+                c[y] = 0.0f;
+            }
+    }
+    small_store4(to + (i0 + r) * ld, j0 + 4 * q, c);
+    if (i0 != j0) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y) Iterate<mm::Split>::store(to + (j0 + 4 * q + y) * ld, i0 + r, c[y]);
+    }
+}
+// tile of square A A + linear A, `a` its tile of A.  A = A0 + diag(d): A A = A0 A0 + (d_i + d_j) A0, on the diagonal A0 A0 + d^2.
+template <int NB> __device__ __forceinline__ mm::v4f small_square(const char* A, int ld, const float* d, int i0, int j0, mm::v4f a, float square, float linear, int lane) {
+    const int r = lane & 15, q = lane >> 4;
+    SmallAcc c;
+#pragma unroll
+    for (int k = 0; k < NB; ++k)
+        c.add(small_frag_kc(A, ld, j0, k, 0, lane), small_frag_kc(A, ld, j0, k, 1, lane), small_frag_kc(A, ld, i0, k, 0, lane), small_frag_kc(A, ld, i0, k, 1, lane));
+    const float di = d[i0 + r];
+    const mm::v4f dj = *reinterpret_cast<const mm::v4f*>(d + j0 + 4 * q), sum = c.sum();
+    mm::v4f b;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+        const float of_d = i0 + r == j0 + 4 * q + y ? di : di + dj[y];
+        b[y] = sum[y] * square + a[y] * (linear + square * of_d);
+    }
+    return b;
+}
+
 // NB: blocks of 32 of the short side.  TWO: room for a second X and A, so that nobody waits before writing, and two waves can
 // share a block of 16 columns (128 x 50: 21.6 -> 20.9 us, 300 of 128 x 128: 153 -> 126).
 template <class T, int NB, bool TWO>
@@ -794,21 +831,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
         ti[x] = i * 16;
         tj[x] = t * 16;
     }
-    auto store_both = [&](char* to, float* diag, int i0, int j0, mm::v4f c) {
-        if (i0 == j0) {
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-                if (r == 4 * q + y) {
-                    diag[i0 + r] = c[y];
-                    c[y] = 0.0f;
-                }
-        }
-        small_store4(to + (i0 + r) * lda, j0 + 4 * q, c);
-        if (i0 != j0) {
-#pragma unroll
-            for (int y = 0; y < 4; ++y) Iterate<mm::Split>::store(to + (j0 + 4 * q + y) * lda, i0 + r, c[y]);
-        }
-    };
+    auto store_both = [&](char* to, float* diag, int i0, int j0, mm::v4f c) { small_store_both(to, lda, diag, i0, j0, c, lane); };
     for (int step = 0; step < g.steps; ++step) {
         mm::v4f a[TURNS], b[TURNS];   // this wave's tiles of A and of the square factor
         if constexpr (NB == 1) {
@@ -852,20 +875,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
 #pragma unroll
         for (int x = 0; x < TURNS; ++x) {
             if (wave + kSmallWaves * x >= TILES) break;
-            SmallAcc c;
-#pragma unroll
-            for (int k = 0; k < NB; ++k)
-                c.add(small_frag_kc(A, lda, tj[x], k, 0, lane), small_frag_kc(A, lda, tj[x], k, 1, lane), small_frag_kc(A, lda, ti[x], k, 0, lane),
-                      small_frag_kc(A, lda, ti[x], k, 1, lane));
-            // A = A0 + diag(d): A A = A0 A0 + (d_i + d_j) A0, on the diagonal A0 A0 + d^2
-            const float di = da[ti[x] + r];
-            const mm::v4f dj = *reinterpret_cast<const mm::v4f*>(da + tj[x] + 4 * q);
-            const mm::v4f sum = c.sum();
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                const float of_d = ti[x] + r == tj[x] + 4 * q + y ? di : di + dj[y];
-                b[x][y] = sum[y] * g.square[step] + a[x][y] * (g.linear[step] + g.square[step] * of_d);
-            }
+            b[x] = small_square<NB>(A, lda, da, ti[x], tj[x], a[x], g.square[step], g.linear[step], lane);
             if (TWO) store_both(B, db, ti[x], tj[x], b[x]);
         }
         __syncthreads();
@@ -926,6 +936,167 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
     }
 }
 
+// ---- short sides up to 128 that one workgroup cannot hold: one launch a step ----------------------------------------------
+// Every workgroup keeps LC columns of X, and the launch of a step does, for them: A from the sums of all chunks (in one order),
+// the square factor (again in every workgroup: short products), X <- a X + (b A + c A A) X, and the chunk's part of the next X X^T.
+// Launches and their short dependent products bound it: 3 a step on the general path.  f32: 50 x 1203 (8, three steps) 70 -> 38 us,
+// 128 x 4096 237 -> 126, 16 x 2000 117 -> 34, 128 x 168 95 -> 75; bf16 keeps 22 bits here: 100 x 4000 156 -> 124, 24 of 120 x 1280 135 -> 139.
+struct OrthoChunkArgs {
+    long ldg, stride_g, ldo, stride_o;   // elements
+    int rows, cols, chunks, parts;
+    const double* part;                  // of the norm
+    double eps, scale;
+    char* X;                             // LDS images of the chunks
+    const mm::v4f* in; mm::v4f* out;     // parts of X X^T: tiles of 16 x 16 as accumulators
+    float gram, square, linear, apply, keep;
+    bool first, last;                    // first: X_0 and its part only
+};
+template <int NB> struct Chunk {
+    static constexpr int LC = NB <= 2 ? 256 : 128, S = NB * 32, NT = NB * 2, TILES = NT * (NT + 1) / 2;
+    static constexpr int LDX = LC * 4 + 32, LDA = S * 4 + 32, IMAGE = S * LDX, LDS = IMAGE + S * LDA;
+};
+template <class T, int NB>
+__global__ __launch_bounds__(kSmallWaves * 64) void ortho_chunk_kernel(const T* G, T* O, const OrthoChunkArgs g) {
+    typedef Chunk<NB> K;
+    constexpr int LC = K::LC, Sp = K::S, TILES = K::TILES, LDX = K::LDX, LDA = K::LDA, TURNS = (TILES + kSmallWaves - 1) / kSmallWaves;
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    __shared__ __attribute__((aligned(16))) float da[Sp], db[Sp];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+    const int mat = blockIdx.x / g.chunks, c0 = blockIdx.x % g.chunks * LC;
+    const bool tall = g.rows > g.cols;
+    const int S = tall ? g.cols : g.rows, L = tall ? g.rows : g.cols, wide = min(L - c0, LC);
+    char* X = lds;
+    char* A = lds + K::IMAGE;
+    mm::v4i* image = reinterpret_cast<mm::v4i*>(g.X + blockIdx.x * (long)K::IMAGE);
+    int ti[TURNS], tj[TURNS];   // this wave's tiles of the lower triangle
+#pragma unroll
+    for (int x = 0; x < TURNS; ++x) {
+        int t = wave + kSmallWaves * x, i = 0;
+        while (t > i) t -= ++i;
+        ti[x] = i * 16;
+        tj[x] = t * 16;
+    }
+    if (g.first) {
+        const Factor by(g.scale / (norm_of(g.part + mat * kParts, g.parts) + g.eps));
+        for (int e = threadIdx.x; e < K::IMAGE / 16; e += kSmallWaves * 64) reinterpret_cast<mm::v4i*>(X)[e] = mm::v4i{0, 0, 0, 0};
+        __syncthreads();
+        const T* from = G + mat * g.stride_g + (tall ? c0 * g.ldg : c0);
+        const int have = tall ? g.cols : wide;   // columns
+        each_run(tall ? wide : g.rows, have, threadIdx.x, kSmallWaves * 64, [&](int row, int c) {
+            T v[8];
+            load_run(from + row * g.ldg + c, have - c, v);
+            if (tall) {
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    if (c + x < have) Iterate<mm::Split>::store(X + (c + x) * LDX, row, by.times((float)v[x]));
+            } else {
+                float w[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) w[x] = by.times((float)v[x]);
+                Iterate<mm::Split>::store8(X + row * LDX, nullptr, c, w);
+            }
+        });
+    } else {
+        for (int e = threadIdx.x; e < K::IMAGE / 16; e += kSmallWaves * 64) reinterpret_cast<mm::v4i*>(X)[e] = image[e];
+        mm::v4f a[TURNS], b[TURNS];
+#pragma unroll
+        for (int x = 0; x < TURNS; ++x) {
+            const int t = wave + kSmallWaves * x;
+            if (t >= TILES) break;
+            a[x] = mm::v4f{};
+            const mm::v4f* in = g.in + ((long)mat * g.chunks * TILES + t) * 64 + lane;
+#pragma unroll 8
+            for (int c = 0; c < g.chunks; ++c) a[x] += in[(long)c * TILES * 64];
+            a[x] *= g.gram;
+            small_store_both(A, LDA, da, ti[x], tj[x], a[x], lane);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < TURNS; ++x) {
+            if (wave + kSmallWaves * x >= TILES) break;
+            b[x] = small_square<NB>(A, LDA, da, ti[x], tj[x], a[x], g.square, g.linear, lane);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < TURNS; ++x) {
+            if (wave + kSmallWaves * x >= TILES) break;
+            small_store_both(A, LDA, db, ti[x], tj[x], b[x], lane);
+        }
+        // LC / 16 blocks of 16 columns: a wave each, or two with half of the rows each
+        constexpr bool HALVES = LC / 16 < kSmallWaves;
+        const int j0 = (HALVES ? wave >> 1 : wave) * 16, from = HALVES && (wave & 1) ? Sp / 2 : 0, to = HALVES && !(wave & 1) ? Sp / 2 : Sp;
+        mm::v4i qf[NB][2];
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            qf[k][0] = small_frag_strided(X, LDX, j0, k, 0, lane);
+            qf[k][1] = small_frag_strided(X, LDX, j0, k, 1, lane);
+        }
+        __syncthreads();   // the square factor is there, and every block is in registers
+#pragma unroll 2
+        for (int i0 = from; i0 < to; i0 += 16) {
+            SmallAcc acc;
+#pragma unroll
+            for (int k = 0; k < NB; ++k) acc.add(qf[k][0], qf[k][1], small_frag_kc(A, LDA, i0, k, 0, lane), small_frag_kc(A, LDA, i0, k, 1, lane));
+            const mm::v4f c = acc.sum() * g.apply + small_load4(X + (i0 + r) * LDX, j0 + 4 * q) * (g.keep + g.apply * db[i0 + r]);
+            if (g.last) {
+                T* o = O + mat * g.stride_o;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const int i = i0 + r, j = c0 + j0 + 4 * q + y;
+                    if (i < S && j < L) o[tall ? j * g.ldo + i : i * g.ldo + j] = (T)c[y];
+                }
+            } else {
+                small_store4(X + (i0 + r) * LDX, j0 + 4 * q, c);
+            }
+        }
+        if (g.last) return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < TURNS; ++x) {
+        const int t = wave + kSmallWaves * x;
+        if (t >= TILES) break;
+        SmallAcc c;
+#pragma unroll
+        for (int k = 0; k < LC / 32; ++k)
+            c.add(small_frag_kc(X, LDX, tj[x], k, 0, lane), small_frag_kc(X, LDX, tj[x], k, 1, lane), small_frag_kc(X, LDX, ti[x], k, 0, lane),
+                  small_frag_kc(X, LDX, ti[x], k, 1, lane));
+        g.out[((long)blockIdx.x * TILES + t) * 64 + lane] = c.sum();
+    }
+    for (int e = threadIdx.x; e < K::IMAGE / 16; e += kSmallWaves * 64) image[e] = reinterpret_cast<mm::v4i*>(X)[e];
+}
+
+struct ChunkPlan { int chunks; long images, sums, total; };   // chunks 0: not this way.  bytes: images of X, one set of sums, workspace
+template <int NB> ChunkPlan chunk_plan_of(long batch, int l) {
+    typedef Chunk<NB> K;
+    const long chunks = (l + K::LC - 1) / K::LC;
+    // Two rounds of workgroups pay for short sides up to 64 (f32 24 x 50 x 4000: 250 -> 140 us), not for longer ones (24 x 128 x 2048:
+    // 212 -> 242); every workgroup reads all chunks' sums (1 x 128 x 8192, 2.4 MB: 371 -> 173).
+    if (chunks * batch > (NB <= 2 ? 512 : 256) || chunks * K::TILES > 2400) return {0, 0, 0, 0};
+    auto up = [](long v) { return (v + 255) / 256 * 256; };
+    const long images = up(batch * chunks * K::IMAGE), sums = batch * chunks * K::TILES * 1024L;
+    return {(int)chunks, images, sums, up(batch * kParts * 8) + images + 2 * sums};
+}
+ChunkPlan chunk_plan(long batch, int rows, int cols) {
+    const int s = std::min(rows, cols), l = std::max(rows, cols);
+    bool two;
+    if (s > kSmallSide || small_lds(rows, cols, two)) return {0, 0, 0, 0};
+    switch ((s + 31) / 32) {
+        case 1: return chunk_plan_of<1>(batch, l);
+        case 2: return chunk_plan_of<2>(batch, l);
+        case 3: return chunk_plan_of<3>(batch, l);
+        default: return chunk_plan_of<4>(batch, l);
+    }
+}
+
+OrthoWork ortho_work(int dtype, long batch, int rows, int cols) {
+    OrthoWork o = dtype == GPX_F64    ? ortho_work_of<double>(batch, rows, cols)
+                  : dtype == GPX_BF16 ? ortho_work_of<mm::Rounded>(batch, rows, cols)
+                                      : ortho_work_of<mm::Split>(batch, rows, cols);
+    if (dtype != GPX_F64) o.total = std::max(o.total, chunk_plan(batch, rows, cols).total);
+    return o;
+}
+
 // rows x cols row-major (the column-major cols x rows of the C interface)
 template <class T, class F>
 int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long ldg, long stride_g, int steps, const double* coef, double eps,
@@ -965,6 +1136,38 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
     ortho_norm_kernel<T><<<dim3(parts, batch), 256, 0, st>>>(G, ldg, stride_g, rows, cols, part);
     HIP_TRY(hipGetLastError());
     const dim3 grid((unsigned)std::min<long>((runs + 255) / 256, 2048), (unsigned)batch);
+    if constexpr (!__is_same(F, double)) {
+        const ChunkPlan plan = chunk_plan(batch, rows, cols);
+        if (steps > 0 && plan.chunks) {
+            char* images = work + (batch * kParts * 8L + 255) / 256 * 256;
+            mm::v4f* sums[2] = {reinterpret_cast<mm::v4f*>(images + plan.images), reinterpret_cast<mm::v4f*>(images + plan.images + plan.sums)};
+            OrthoChunkArgs g = {ldg, stride_g, ldo, stride_o, rows, cols, plan.chunks, parts, part, eps, f.start, images};
+            auto go = [&](auto blocks) {
+                constexpr int NB = decltype(blocks)::value;
+                for (int k = 0; k <= steps; ++k) {
+                    g.in = sums[~k & 1];
+                    g.out = sums[k & 1];
+                    g.first = k == 0;
+                    g.last = k == steps;
+                    if (k > 0) {
+                        g.gram = (float)f.gram[k - 1];
+                        g.square = (float)f.square[k - 1];
+                        g.linear = (float)f.linear[k - 1];
+                        g.apply = (float)f.apply[k - 1];
+                        g.keep = (float)f.keep[k - 1];
+                    }
+                    ortho_chunk_kernel<T, NB><<<batch * plan.chunks, kSmallWaves * 64, Chunk<NB>::LDS, st>>>(G, O, g);
+                }
+            };
+            const int nb = (std::min(rows, cols) + 31) / 32;
+            if (nb == 1) go(Int<1>{});
+            else if (nb == 2) go(Int<2>{});
+            else if (nb == 3) go(Int<3>{});
+            else go(Int<4>{});
+            HIP_TRY(hipGetLastError());
+            return GPX_OK;
+        }
+    }
     if (steps == 0) {
         ortho_normalize_kernel<T><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, part, parts, eps, O, ldo, stride_o);
         HIP_TRY(hipGetLastError());
