@@ -337,7 +337,8 @@ def chol_solve(A, B=None, want_inverse=False):
 
 # ---- products grouped by expert, orthogonalised update ---------------------------------------------
 # These take torch tensors on the GPU (rows of any stride, the last dimension contiguous), launch on torch's current stream
-# of the tensors' device and return `out`, which overlaps no operand; nothing is recorded for autograd.  torch is imported only when one is called.
+# of the tensors' device and return `out`, which overlaps no operand; nothing is recorded for autograd.  torch is
+# imported only when one is called, but has to have been imported before this module: there is one HIP runtime in a process.
 F64, F32, BF16, F16 = 0, 1, 2, 3
 
 lib.gpx_grouped_gemm.argtypes = [_i, _i, _i64, _i64, _i64, _i64, _d, _vp, _i64, _vp, _i64, _i64, _vp, _d, _vp, _i64, _vp]
@@ -353,6 +354,10 @@ _codes = {}
 def _load_torch():
     global _torch, _raw_stream
     import torch
+    # torch brings a HIP runtime of its own; loaded behind another one, it finds no GPU
+    with open("/proc/self/maps") as maps:
+        if len({line.split()[-1] for line in maps if "libamdhip64" in line}) > 1:
+            raise RuntimeError("import torch before gp_amd.lib: this process has loaded two HIP runtimes")
     _codes.update({torch.float64: F64, torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
     # the handle of torch's current stream of a device; the public way builds a Stream object for it (1 us of a 6 us call)
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)

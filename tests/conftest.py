@@ -3,6 +3,12 @@ import sys
 
 import pytest
 
+try:
+    # Before libgpx.so: torch brings a HIP runtime of its own, and a process that has loaded another one first sees no GPU in it.
+    import torch  # noqa: F401
+except ImportError:
+    pass
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 for p in (ROOT, os.path.join(ROOT, "tests")):
     if p not in sys.path:

@@ -207,6 +207,32 @@ def test_captured_replayed_and_on_two_streams():
             assert all(torch.equal(mine, out) for _, mine in graphs)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("size", [(2, 128, 1300), (3, 2100, 40), (1, 65, 257), (2, 70000, 1), (1, 100, 8000)], ids=str)
+def test_short_sides(dtype, size):
+    """Short sides up to 128 over many columns, with one and several steps, in place, a bad neighbour, captured and replayed."""
+    lib = _lib()
+    g = data(1, dtype, *size)
+    for steps in (1, 2, 5):
+        check(lib.orthogonalize(g, torch.empty_like(g), steps=steps), g, steps=steps)
+    first = lib.orthogonalize(g, torch.empty_like(g))
+    own = g.clone()
+    assert torch.equal(lib.orthogonalize(own, own), first)
+    if size[0] > 1:
+        own = g.clone()
+        own[0, -1, -1] = float("nan")
+        out = lib.orthogonalize(own, torch.empty_like(g))
+        assert torch.equal(out[1:], first[1:]) and not bool(torch.isfinite(out[0]).all())
+    graph, mine = torch.cuda.CUDAGraph(), torch.zeros_like(g)
+    with torch.cuda.graph(graph):
+        lib.orthogonalize(g, mine)
+    for seed in range(3):
+        g.copy_(data(5 + seed, dtype, *size))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(mine, lib.orthogonalize(g, torch.empty_like(g)))
+
+
 def test_refusals():
     lib = _lib()
     g = torch.zeros(2, 4, 6, device="cuda")
