@@ -208,11 +208,11 @@ def test_captured_replayed_and_on_two_streams():
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("size", [(2, 128, 1300), (3, 2100, 40), (1, 65, 257), (2, 70000, 1), (1, 100, 8000)], ids=str)
+@pytest.mark.parametrize("size", [(2, 128, 1300), (3, 2100, 40), (1, 65, 257), (2, 70000, 1), (1, 100, 8000), (2, 9000, 1)], ids=str)
 def test_short_sides(dtype, size):
     """Short sides up to 128 over many columns, with one and several steps, in place, a bad neighbour, captured and replayed."""
-    if dtype.itemsize == 2 and max(size) > 65536:
-        pytest.skip("refused: bf16 2 x 70000 x 1 ended in a GPU fault whose cause is not known")
+    if max(size) > 65536:   # (the oracle's X X^T has 4.9e9 elements there; sides above 65536 are refused for 16 bits)
+        pytest.skip("2 x 70000 x 1 ended in a GPU fault in bf16 whose cause is not known: not run")
     lib = _lib()
     g = data(1, dtype, *size)
     for steps in (1, 2, 5):
