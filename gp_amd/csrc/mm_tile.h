@@ -136,9 +136,6 @@ constexpr unsigned kOutside = 0x7fff8000u;   // an offset behind them
 
 // what a type is stored as, and the values of k in a step
 template <class T> struct Stored { typedef T type; static constexpr int BK = step_k<T>(), WIDE = 1; static constexpr bool split = false; };
-// the first plane alone, as an ordinary 16-bit matrix: products of values rounded to 11 bits
-struct Rounded {};
-template <> struct Stored<Rounded> : Stored<_Float16> {};
 template <> struct Stored<Split> { typedef _Float16 type; static constexpr int BK = 32, WIDE = 2; static constexpr bool split = true; };
 
 template <class F, int ROWS, bool KC, int NT> struct Operand {
@@ -326,9 +323,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
         }
     }
     // K loop on direct loads, STAGES LDS stages: while step s is multiplied, steps s + 1 .. s + STAGES - 1 are on their way.
-    // also(s, P, Q): after the products of step s, with its LDS images.
-    struct Nothing { __device__ void operator()(int, const char*, const char*) const {} };
-    template <class Also = Nothing> __device__ __forceinline__ void run_direct(char* lds, const OpP& p, const OpQ& q, int K, Also&& also = Also()) {
+    __device__ __forceinline__ void run_direct(char* lds, const OpP& p, const OpQ& q, int K) {
         constexpr int BK = OpP::BK;
         constexpr int AHEAD = (STAGES - 2) * (OpP::NL + OpQ::NL);   // loads of this wave behind those of the step waited for
         const int full = K / BK, rest = K - full * BK, steps = full + (rest != 0);
@@ -351,10 +346,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
             if (STAGES > 2 && s + STAGES - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(AHEAD) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (s + STAGES - 1 < steps) issue(s + STAGES - 1, into);
-            if (busy) {
-                multiply(lds + stage * STAGE, lds + stage * STAGE + OpP::BYTES, s >= full && rest * 2 <= BK ? 1 : 2);
-                also(s, lds + stage * STAGE, lds + stage * STAGE + OpP::BYTES);
-            }
+            if (busy) multiply(lds + stage * STAGE, lds + stage * STAGE + OpP::BYTES, s >= full && rest * 2 <= BK ? 1 : 2);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             into = into + 1 == STAGES ? 0 : into + 1;
         }
@@ -362,7 +354,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
     // The same for few tiles with long sums: GROUPS sets of NT threads take the steps in turn, each with LDS stages of its own,
     // and add their accumulators at the end in one order, the sum in group 0.  A step of a 64-tile alone on its CU costs
     // 0.36 us, most of it waiting; four groups do four in 0.5 us.
-    template <class Also = Nothing> __device__ __forceinline__ void run_groups(char* lds, const OpP& p, const OpQ& q, int K, Also&& also = Also()) {
+    __device__ __forceinline__ void run_groups(char* lds, const OpP& p, const OpQ& q, int K) {
         static_assert(GROUPS > 1, "groups");
         constexpr int BK = OpP::BK, AHEAD = (STAGES - 2) * (OpP::NL + OpQ::NL);
         const int full = K / BK, rest = K - full * BK, steps = full + (rest != 0), turns = (steps + GROUPS - 1) / GROUPS, mine = group();
@@ -390,10 +382,7 @@ template <class F, int BM, int BN, int WR, int WC, bool PKC, bool QKC, int STAGE
             issue(t + STAGES - 1, into);
             const int s = t * GROUPS + mine;
             const char* st = own + stage * STAGE;
-            if (busy && s < steps) {
-                multiply(st, st + OpP::BYTES, s >= full && rest * 2 <= BK ? 1 : 2);
-                also(s, st, st + OpP::BYTES);
-            }
+            if (busy && s < steps) multiply(st, st + OpP::BYTES, s >= full && rest * 2 <= BK ? 1 : 2);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             into = into + 1 == STAGES ? 0 : into + 1;
         }

@@ -100,25 +100,17 @@ __global__ __launch_bounds__(256) void ortho_normalize_kernel(const T* G, long l
 }
 
 // ---- the iterates ------------------------------------------------------------------------------------------------
-// Double matrices stay in double.  Floats and f16 are iterated in the split format, two f16 planes under one power of two per
+// Double matrices stay in double.  All others are iterated in the split format, two f16 planes under one power of two per
 // matrix and step: 22 bits of every value, the accumulators and all sums in 32.  One f16 product is 16 times the rate of a
 // product of floats here, the three that the split needs leave a factor of five.  The host bounds the singular values of
 // every iterate from the coefficients and places the largest possible element at 2^15: nothing overflows, and the smallest
 // step of the second plane is 2^-39 of that bound.
-// In both formats the largest elements of A and of b A + c A A, their diagonals, are kept in floats beside the matrices (zero in
-// them) and applied where the products' results are written.  Relative error of the result without and with that: f32, 16 x 208 in
-// three steps 1.2e-6 and 3.3e-7 (products of floats: 5.7e-7), 300 x 2000 in six 2.5e-6 and 6.6e-7 (2.9e-6); bf16, 300 x 2000 in six,
-// before the result is rounded, 2.0e-3 and 7e-4.  It costs 0.5 us of 21 for a small matrix, 0.8 % for one of 4096 x 4096.
-// bf16: the products take values rounded to 11 bits, one f16 plane under the same powers of two: one matrix product instead of
-// three and half the bytes.  That rounding is an eighth of the one that the bf16 matrix itself has behind it, and the result is
-// rounded to 8 bits.  More is kept where it counts:
-//   X itself has a second plane of 8-bit floats, 15 bits in all, and a X is formed from both: small singular values grow by a
-//   in every step, and what rounding adds to them grows with them (five orders of magnitude of singular values, 300 x 2000,
-//   relative error of the result: 1.06e-2 with 11 bits of X, 1.9e-3 with 15 or 22, its own rounding 1.66e-3).  X_0 needs none,
-//   the 8 bits of bf16 times a power of two; nor does the last iterate, which grows once more only (1.88e-3 -> 1.93e-3).
-// 16 matrices of 1024 x 2816: 2.61 -> 1.24 ms (the second plane through the caches: 0.03 more, it only
-// sweeps X and A out of them); off from 64 bits by 1.73e-3, 1.66e-3 of it the rounding of the result; half a step of the input
-// moves the result by 4e-3.
+// The largest elements of A and of b A + c A A, their diagonals, are kept in floats beside the matrices (zero in them) and applied
+// where the products' results are written.  Relative error of the result without and with that, f32: 16 x 208 in three steps
+// 1.2e-6 and 3.3e-7 (products of floats: 5.7e-7), 300 x 2000 in six 2.5e-6 and 6.6e-7 (2.9e-6).  It costs 0.5 us of 21 for a small
+// matrix, 0.8 % for one of 4096 x 4096.
+// bf16 matrices take the same planes.  In one plane of 11 bits their products take half the time (16 of 1024 x 2816), but the
+// result is then further from 64 bits than its own rounding (1.73e-3 against 1.66e-3).
 template <class F> struct Iterate;
 // v = h + l.  The compiler may form a converted product in one rounding and the product itself in two; h has to be one value
 // for both planes (told apart at ties, the planes would disagree by a step of the first one).
@@ -158,7 +150,7 @@ template <> struct Iterate<mm::Split> {
     }
     static long bytes(long cols) { return cols * 4; }
     // eight neighbours from column j on, j a multiple of 8
-    __device__ static void store8(char* row, char*, int j, const float (&v)[8]) {
+    __device__ static void store8(char* row, int j, const float (&v)[8]) {
         mm::v8h h, l;
 #pragma unroll
         for (int x = 0; x < 8; x += 2) {
@@ -180,61 +172,14 @@ template <> struct Iterate<mm::Split> {
         for (int x = 0; x < 8; ++x) v[x] += by[x] * ((float)h[x] + (float)l[x]);
     }
 };
-template <> struct Iterate<mm::Rounded> {
-    static constexpr int PAD = 8;
-    static long bytes(long cols) { return cols * 2; }
-    // lo: the row in the second plane, or null: 2^4 times what the first rounding leaves (2^4 at most, values stay below 2^15)
-    // as e4m3 values (448 at most)
-    __device__ static void store8(char* row, char* lo, int j, const float (&v)[8]) {
-        mm::v8h h;
-        v2f left[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const v2h a = split2(v2f{v[2 * x], v[2 * x + 1]}, left[x]);
-            h[2 * x] = a[0];
-            h[2 * x + 1] = a[1];
-            left[x][0] *= 16.0f;
-            left[x][1] *= 16.0f;
-        }
-        *reinterpret_cast<mm::v8h*>(row + j * 2) = h;
-        if (lo) {
-            int w[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-                w[x] = __builtin_amdgcn_cvt_pk_fp8_f32(left[2 * x + 1][0], left[2 * x + 1][1],
-                                                       __builtin_amdgcn_cvt_pk_fp8_f32(left[2 * x][0], left[2 * x][1], 0, false), true);
-            __builtin_nontemporal_store((long)(unsigned)w[0] | (long)w[1] << 32, reinterpret_cast<long*>(lo + j));
-        }
-    }
-    __device__ static void add8(const char* row, int j, const float (&by)[8], float (&v)[8]) {
-        const mm::v8h h = *reinterpret_cast<const mm::v8h*>(row + j * 2);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) v[x] += by[x] * (float)h[x];
-    }
-    __device__ static void add8_low(long both, const float (&by)[8], float (&v)[8]) {
-        const int w[2] = {(int)both, (int)(both >> 32)};
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const auto l = x % 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(w[x / 2], true) : __builtin_amdgcn_cvt_pk_f32_fp8(w[x / 2], false);
-            v[2 * x] += by[2 * x] * (0.0625f * l[0]);
-            v[2 * x + 1] += by[2 * x + 1] * (0.0625f * l[1]);
-        }
-    }
-};
 template <class F> int padded(int cols) { return (cols + Iterate<F>::PAD - 1) / Iterate<F>::PAD * Iterate<F>::PAD; }
 
 template <class T, class F>
 __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ G, long ldg, long stride_g, int rows, int cols, int pcols,
                                                           const double* __restrict__ part, int parts, double eps, double scale, char* __restrict__ X,
-                                                          long ldx, long stride_x, float* __restrict__ first) {
+                                                          long ldx, long stride_x) {
     const double norm = norm_of(part + blockIdx.y * kParts, parts) + eps;
-    double factor = scale / norm;
-    if constexpr (__is_same(F, mm::Rounded)) {   // a power of two, so that bf16 values pass into f16 as they are; the rest is `first`
-        const int e = isfinite(norm) ? ilogb(norm) : 0;
-        if (isfinite(norm)) factor = ldexp(scale, -e);
-        if (blockIdx.x == 0 && threadIdx.x == 0) first[blockIdx.y] = (float)(ldexp(1.0, e) / norm);
-    }
-    const Factor by(factor);
+    const Factor by(scale / norm);
     each_run(rows, pcols, blockIdx.x * 256L + threadIdx.x, gridDim.x * 256L, [&](int r, int c) {
         T v[8];
         load_run(G + blockIdx.y * stride_g + r * ldg + c, cols - c, v);
@@ -243,7 +188,7 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ 
             float w[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = by.times((float)v[e]);
-            Iterate<F>::store8(x, nullptr, c, w);
+            Iterate<F>::store8(x, c, w);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -263,8 +208,6 @@ struct OrthoArgs {
     int I, J, K, batch;
     double c1, c2;
     const float* diag; float* diag_out;        // min(rows, cols) per matrix
-    const char* Elo; char* Dlo;                // second planes of X, half as wide, or null
-    const float* first;                        // first step: what is missing from X, per matrix
 };
 template <class F, class O, bool LAST, int B, int WR, int WC, int ST, int KG, bool PKC, bool QKC, bool SYM>
 __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) > 128 * 64 ? 1 : 2) void ortho_mm_kernel(const OrthoArgs g) {
@@ -315,66 +258,11 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
     typename Tile::OpQ q = {g.Q + mat * g.sq + (QKC ? j0 * g.ldq : j0 * (long)W), g.ldq, QKC ? min(g.J - j0, B) : min(Jp - j0, B) * WE, g.K};
     Tile t;
     t.clear();
-    one c1 = (one)g.c1, c2 = (one)g.c2;
-    if constexpr (__is_same(F, mm::Rounded)) {
-        if (g.first) {
-            const float m = g.first[mat];
-            c1 *= SYM ? m * m : m;
-            c2 *= m;
-        }
-    }
-    constexpr bool DIAG = !__is_same(F, double), LOW = __is_same(F, mm::Rounded) && !SYM;
+    const one c1 = (one)g.c1, c2 = (one)g.c2;
+    constexpr bool DIAG = !__is_same(F, double);
     const float* diag = DIAG && g.diag ? g.diag + mat * (long)(SYM ? g.I : g.K) : nullptr;
-    if constexpr (LOW) {
-        // a X + diag(d) X: the elements of X that the tile adds are on chip as an operand in the steps whose k are the tile's rows
-        // (QKC: columns), and go to the accumulators from there, so that only the second plane is
-        // read behind the sums (with all of its loads on their way at once: 16 of 1024 x 2816 1319 -> 1236 us)
-        constexpr int TI = Tile::TI, TJ = Tile::TJ, mask = mm::swizzle_mask<_Float16>(B);
-        typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(Tile::wave_id()), r = lane & 15, k4 = lane >> 4 << 2;
-        const int iw = wave / WC * (B / WR), jw = wave % WC * (B / WC);
-        const float ratio = c2 / c1;
-        float f[QKC ? TJ : TI][QKC ? 4 : 1];
-#pragma unroll
-        for (int n = 0; n < (QKC ? TJ : TI); ++n)
-#pragma unroll
-            for (int x = 0; x < (QKC ? 4 : 1); ++x) f[n][x] = ratio + diag[min(QKC ? j0 + jw + 16 * n + k4 + x : i0 + iw + 16 * n + r, g.K - 1)];
-        auto add_x = [&](int s, const char* sp, const char* sq) {
-            if constexpr (!QKC) {
-#pragma unroll
-                for (int i = 0; i < TI; ++i) {
-                    const int row = i0 + iw + 16 * i, k = (row & 63) + r;
-                    if (row >> 6 != s) continue;
-#pragma unroll
-                    for (int j = 0; j < TJ; ++j) {
-                        const int col = jw + 16 * j + k4;
-                        const v4h h = *reinterpret_cast<const v4h*>(sq + k * (B * 2) + (((col >> 4) ^ (mm::strided_swizzle<_Float16>(k) & mask)) << 5) + (col & 15) * 2);
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) t.acc[i][j][x] += f[i][0] * (float)h[x];
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < TJ; ++j) {
-                    const int col = j0 + jw + 16 * j, k = (col & 63) + k4;
-                    if (col >> 6 != s) continue;
-#pragma unroll
-                    for (int i = 0; i < TI; ++i) {
-                        const int row = iw + 16 * i + r;
-                        const v4h h = *reinterpret_cast<const v4h*>(sp + row * 128 + (((k >> 3) ^ (row & 7)) << 4) + (k & 7) * 2);
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) t.acc[i][j][x] += f[j][x] * (float)h[x];
-                    }
-                }
-            }
-        };
-        if constexpr (KG > 1) t.run_groups(lds, p, q, g.K, add_x);
-        else t.run_direct(lds, p, q, g.K, add_x);
-    } else if constexpr (KG > 1) {
-        t.run_groups(lds, p, q, g.K);
-    } else {
-        t.run_direct(lds, p, q, g.K);
-    }
+    if constexpr (KG > 1) t.run_groups(lds, p, q, g.K);
+    else t.run_direct(lds, p, q, g.K);
     const char* E = g.E + mat * g.se;
     char* D = g.D + mat * g.sd;
     if constexpr (!Tile::SWAP) {
@@ -394,16 +282,6 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
         for (int pass = 0; pass < WR; ++pass) {
             const int ib = i0 + pass * R;
             constexpr int RUNS = R * (B / 8), TURNS = (RUNS + NT - 1) / NT;
-            long low[LOW ? TURNS : 1];   // E's second plane: from addresses that exist in any case, without a test that each load would wait behind
-            if constexpr (LOW) {
-                if (g.Elo) {
-#pragma unroll
-                    for (int n = 0; n < TURNS; ++n) {
-                        const int e = threadIdx.x + n * NT, i = min(ib + e / (B / 8), g.I - 1), j = min(j0 + e % (B / 8) * 8, Jp - 8);
-                        low[n] = __builtin_nontemporal_load(reinterpret_cast<const long*>(g.Elo + (mat * g.se + i * g.lde) / 2 + j));
-                    }
-                }
-            }
             __syncthreads();
             t.to_slab(slab, pass);
             __syncthreads();
@@ -420,11 +298,10 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
                     v[x] = c1 * lo[x];
                     v[4 + x] = c1 * hi[x];
                 }
-                if (LOW ? g.Elo != nullptr : c2 != 0.0f || (DIAG && diag)) {
+                if (c2 != 0.0f || (DIAG && diag)) {
                     float by[8];
                     factors(i, j, g.J - j, by);
-                    if constexpr (LOW) Iterate<F>::add8_low(low[n], by, v);
-                    else Iterate<F>::add8(E + i * g.lde, j, by, v);
+                    Iterate<F>::add8(E + i * g.lde, j, by, v);
                 }
                 if constexpr (DIAG && SYM) {
                     if (i >= j && i < j + 8) {
@@ -453,7 +330,7 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
                             if (j + x < g.J) d[x] = (O)v[x];
                     }
                 } else {
-                    Iterate<F>::store8(D + i * g.ldd, LOW && g.Dlo ? g.Dlo + (mat * g.sd + i * g.ldd) / 2 : nullptr, j, v);
+                    Iterate<F>::store8(D + i * g.ldd, j, v);
                 }
             }
             if (SYM && ti != tj) {   // D(j, i): E is symmetric to the bit, so both triangles are
@@ -470,7 +347,7 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
                         factors(j, i, g.I - i, by);
                         Iterate<F>::add8(E + j * g.lde, i, by, v);
                     }
-                    Iterate<F>::store8(D + j * g.ldd, nullptr, i, v);
+                    Iterate<F>::store8(D + j * g.ldd, i, v);
                 }
             }
         }
@@ -498,7 +375,7 @@ __global__ __launch_bounds__(WR * WC * 64 * KG, KG > 1 ? 4 : B * B / (WR * WC) >
 }
 
 struct OrthoWork {   // offsets and strides in bytes; rows of the iterates padded to whole blocks
-    long part, x[2], lo[2], a, b, diag[2], first, total;   // lo: second planes of x; diag: of a and b; first: see OrthoArgs (Rounded)
+    long part, x[2], a, b, diag[2], total;   // diag: of a and b
     long ldx, sx, lda, sa;
 };
 // Rows of a power of two of bytes would meet in few memory channels: the K step of a tile reads 128 bytes of every row.
@@ -517,15 +394,11 @@ template <class F> OrthoWork ortho_work_of(long batch, int rows, int cols) {
     o.part = 0;
     o.x[0] = up(batch * kParts * 8);
     o.x[1] = o.x[0] + up(batch * o.sx);
-    const long low = __is_same(F, mm::Rounded) ? up(batch * o.sx / 2) : 0;
-    o.lo[0] = o.x[1] + up(batch * o.sx);
-    o.lo[1] = o.lo[0] + low;
-    o.a = o.lo[1] + low;
+    o.a = o.x[1] + up(batch * o.sx);
     o.b = o.a + up(batch * o.sa);
     o.diag[0] = o.b + up(batch * o.sa);
     o.diag[1] = o.diag[0] + (__is_same(F, double) ? 0 : up(batch * s * 4));
-    o.first = o.diag[1] + (o.diag[1] - o.diag[0]);
-    o.total = o.first + (__is_same(F, mm::Rounded) ? up(batch * 4) : 0);
+    o.total = o.diag[1] + (o.diag[1] - o.diag[0]);
     return o;
 }
 // The tile of one product of split matrices, by the time it takes: rounds of workgroups over the 256 CUs, each of them K / 32
@@ -534,20 +407,17 @@ template <class F> OrthoWork ortho_work_of(long batch, int rows, int cols) {
 // grid that does not fill the chip waits for memory more than for the matrix cores) 0.55 (0.36) / 4.  Rounds decide: the 136
 // lower 256-tiles of a 4096 x 4096 Gram matrix take as long as all 256, its 253 lower 192-tiles 0.7 of that.
 // Long sums on few 64-tiles: four groups of waves on one tile, 0.30 (0.13) / 6.5 (1024 x 1024: 235 -> 210 us in all, 300 x 2000: 205 -> 187).
-// Products of rounded values: K / 64 steps of 1.5 / 14, 0.95 (0.52) / 5, 0.38 (0.25) / 3, groups 0.25 (0.11) / 6, no 192.
 enum TileChoice { TILE256, TILE128, TILE64, TILE64_GROUPS, TILE192 };
-TileChoice choose_tile(bool split, bool sym, int I, int J, int K, int batch) {
+TileChoice choose_tile(bool sym, int I, int J, int K, int batch) {
     struct Cost { int b; double step, step_alone, rest; };
-    static const Cost of_split[5] = {{256, 2.3, 2.3, 20.0}, {128, 1.4, 0.85, 8.0}, {64, 0.55, 0.36, 4.0}, {64, 0.30, 0.13, 6.5}, {192, 1.65, 1.65, 10.0}};
-    static const Cost of_rounded[4] = {{256, 1.5, 1.5, 14.0}, {128, 0.95, 0.52, 5.0}, {64, 0.38, 0.25, 3.0}, {64, 0.25, 0.11, 6.0}};
-    const Cost* t = split ? of_split : of_rounded;
+    static const Cost t[5] = {{256, 2.3, 2.3, 20.0}, {128, 1.4, 0.85, 8.0}, {64, 0.55, 0.36, 4.0}, {64, 0.30, 0.13, 6.5}, {192, 1.65, 1.65, 10.0}};
     int best = 0;
     double least = 1e300;
-    for (int c = 0; c < (split ? 5 : 4); ++c) {
+    for (int c = 0; c < 5; ++c) {
         const double it = (I + t[c].b - 1) / t[c].b, jt = (J + t[c].b - 1) / t[c].b;
         const double tiles = (sym ? it * (it + 1) / 2 : it * jt) * batch, slots = t[c].b >= 192 || c == TILE64_GROUPS ? 256.0 : 512.0;
         const double step = tiles <= 256.0 ? t[c].step_alone : t[c].step;
-        const double cost = ceil(tiles / slots) * (step * (split ? (K + 31) / 32 : (K + 63) / 64) + t[c].rest);
+        const double cost = ceil(tiles / slots) * (step * ((K + 31) / 32) + t[c].rest);
         if (cost < least) {
             least = cost;
             best = c;
@@ -572,12 +442,12 @@ template <class F, class O, bool LAST, bool PKC, bool QKC, bool SYM> int launch(
         ortho_mm_kernel<F, O, LAST, B, WR, WC, ST, KG, PKC, QKC, SYM><<<(unsigned)grid, WR * WC * 64 * KG, 0, st>>>(g);
     };
     if constexpr (!__is_same(F, double)) {
-        const TileChoice c = choose_tile(mm::Stored<F>::split, SYM, g.I, g.J, g.K, batch);
+        const TileChoice c = choose_tile(SYM, g.I, g.J, g.K, batch);
         if (c == TILE256) GO(256, 2, 4, 2, 1);
         else if (c == TILE128) GO(128, 2, 2, 2, 1);
         else if (c == TILE64) GO(64, 2, 2, 4, 1);
         else if (c == TILE64_GROUPS) GO(64, 2, 2, 2, 4);
-        else if constexpr (mm::Stored<F>::split) GO(192, 2, 4, 2, 1);
+        else GO(192, 2, 4, 2, 1);
     } else {
         // doubles: 64 x 64 tiles cost 4 % on a full chip and are three to four times as many; 32 x 32 where these are few; where those
         // are few too, four groups of waves share a sum (512 x 512: 233 -> 193 us), or 16 single waves that of a 16 x 16 tile
@@ -817,7 +687,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
             float w[8];
 #pragma unroll
             for (int x = 0; x < 8; ++x) w[x] = by.times((float)v[x]);
-            Iterate<mm::Split>::store8(X + row * ldx, nullptr, c, w);
+            Iterate<mm::Split>::store8(X + row * ldx, c, w);
         }
     });
     __syncthreads();
@@ -993,7 +863,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_chunk_kernel(const T* 
                 float w[8];
 #pragma unroll
                 for (int x = 0; x < 8; ++x) w[x] = by.times((float)v[x]);
-                Iterate<mm::Split>::store8(X + row * LDX, nullptr, c, w);
+                Iterate<mm::Split>::store8(X + row * LDX, c, w);
             }
         });
     } else {
@@ -1091,8 +961,7 @@ ChunkPlan chunk_plan(long batch, int rows, int cols) {
 
 OrthoWork ortho_work(int dtype, long batch, int rows, int cols) {
     OrthoWork o = dtype == GPX_F64    ? ortho_work_of<double>(batch, rows, cols)
-                  : dtype == GPX_BF16 ? ortho_work_of<mm::Rounded>(batch, rows, cols)
-                                      : ortho_work_of<mm::Split>(batch, rows, cols);
+                                    : ortho_work_of<mm::Split>(batch, rows, cols);
     if (dtype != GPX_F64) o.total = std::max(o.total, chunk_plan(batch, rows, cols).total);
     return o;
 }
@@ -1107,7 +976,7 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
         bool two = false;
         const long bytes = small_lds(rows, cols, two);
         if (steps > 0 && bytes) {
-            OrthoSmallArgs g = {ldg, stride_g, ldo, stride_o, rows, cols, steps, eps, f.start, {}, {}, {}, {}, {}};   // split planes for bf16 too
+            OrthoSmallArgs g = {ldg, stride_g, ldo, stride_o, rows, cols, steps, eps, f.start, {}, {}, {}, {}, {}};
             for (int k = 0; k < steps; ++k) {
                 g.gram[k] = (float)f.gram[k];
                 g.square[k] = (float)f.square[k];
@@ -1174,31 +1043,25 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
         return GPX_OK;
     }
     char* x[2] = {work + o.x[0], work + o.x[1]};
-    constexpr bool low = __is_same(F, mm::Rounded);
-    float* first = low ? reinterpret_cast<float*>(work + o.first) : nullptr;
     char *a = work + o.a, *b = work + o.b;
-    float *da = reinterpret_cast<float*>(work + o.diag[0]), *db = reinterpret_cast<float*>(work + o.diag[1]);   // (Rounded)
-    ortho_scale_kernel<T, F><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, padded<F>(cols), part, parts, eps, f.start, x[0], o.ldx, o.sx, first);
+    float *da = reinterpret_cast<float*>(work + o.diag[0]), *db = reinterpret_cast<float*>(work + o.diag[1]);
+    ortho_scale_kernel<T, F><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, padded<F>(cols), part, parts, eps, f.start, x[0], o.ldx, o.sx);
     HIP_TRY(hipGetLastError());
     const bool tall = rows > cols;
     const int s = std::min(rows, cols), l = std::max(rows, cols);
     for (int k = 0; k < steps; ++k) {
         char *from = x[k & 1], *to = x[~k & 1];
-        // X_0 is exact in one plane; the last iterate, which one step is left to work on, has no second one either
-        char* from_lo = low && k > 0 && k + 1 < steps ? work + o.lo[k & 1] : nullptr;
-        char* to_lo = low && k + 2 < steps ? work + o.lo[~k & 1] : nullptr;
-        const float* missing = k == 0 ? first : nullptr;
-        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, s, s, l, batch, f.gram[k], 0.0, nullptr, da, nullptr, nullptr, missing};
+        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, s, s, l, batch, f.gram[k], 0.0, nullptr, da};
         int rc = tall ? launch<F, F, false, false, false, true>(st, gram, batch) : launch<F, F, false, true, true, true>(st, gram, batch);
         if (rc) return rc;
         const OrthoArgs poly = {a, a, a, b, o.lda, o.lda, o.lda, o.lda, o.sa, o.sa, o.sa, o.sa, s, s, s, batch,
-                                f.square[k], f.linear[k], da, db, nullptr, nullptr, nullptr};
+                                f.square[k], f.linear[k], da, db};
         if ((rc = launch<F, F, false, true, true, true>(st, poly, batch))) return rc;
         const bool last = k + 1 == steps;
         const long ldd = last ? ldo * (long)sizeof(T) : o.ldx, sd = last ? stride_o * (long)sizeof(T) : o.sx;
         char* d = last ? reinterpret_cast<char*>(O) : to;
-        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k], db, nullptr, from_lo, to_lo, missing}
-                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k], db, nullptr, from_lo, to_lo, missing};
+        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k], db, nullptr}
+                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k], db, nullptr};
         if (tall) rc = last ? launch<F, T, true, true, true, false>(st, apply, batch) : launch<F, F, false, true, true, false>(st, apply, batch);
         else rc = last ? launch<F, T, true, true, false, false>(st, apply, batch) : launch<F, F, false, true, false, false>(st, apply, batch);
         if (rc) return rc;
@@ -1257,7 +1120,7 @@ extern "C" int gpx_orthogonalize(int dtype, int64_t batch, int64_t M, int64_t N,
             return ortho_typed<float, mm::Split>(st, b, r, c, static_cast<const float*>(G), ldg, stride_g, steps, table, eps,
                                              static_cast<float*>(O), ldo, stride_o, w);
         case GPX_BF16:
-            return ortho_typed<__bf16, mm::Rounded>(st, b, r, c, static_cast<const __bf16*>(G), ldg, stride_g, steps, table, eps,
+            return ortho_typed<__bf16, mm::Split>(st, b, r, c, static_cast<const __bf16*>(G), ldg, stride_g, steps, table, eps,
                                               static_cast<__bf16*>(O), ldo, stride_o, w);
         default:
             return ortho_typed<_Float16, mm::Split>(st, b, r, c, static_cast<const _Float16*>(G), ldg, stride_g, steps, table, eps,

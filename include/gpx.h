@@ -105,8 +105,8 @@ int gpx_grouped_gemm_dw(int dtype, int c_dtype, int64_t groups, int64_t T, int64
                         int64_t stride_c, void* work, int64_t work_bytes, void* hip_stream);
 /* batch matrices G_b (M x N column-major at G + b*stride_g): X = G / (|G|_F + eps), then `steps` (0..64) times
  *   A = X X^T,  X = a X + (b A + c A A) X        (the odd polynomial a s + b s^3 + c s^5 of the singular values s)
- * into O.  The iterates of F64 are doubles, of F32 and F16 hold 22 bits or more, and BF16 products take operands rounded to 11
- * bits (the input has 8) except for a X and the diagonal of b A + c A A.  coef: HOST, 3*steps finite values a, b, c of every
+ * into O.  The iterates of F64 are doubles; all others hold each value to 22 bits or to 2^-39 of the largest possible one, the
+ * coarser of the two, sums are taken in 32 bits, and the result is rounded once.  coef: HOST, 3*steps finite values a, b, c of every
  * step; NULL: (3.4445, -4.7750, 2.0315) in each.  Coefficients that could carry singular values past 2^100 are refused,
  * except for F64.  eps >= 1e-300: a zero matrix gives zeros (and so does one of F64 whose squares sum past 1.8e308).  A
  * matrix that holds an infinity or NaN gives non-finite values in its own result only.  O may be G (same ld and stride).
