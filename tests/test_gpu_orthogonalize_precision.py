@@ -51,3 +51,36 @@ def test_16_bit_results_are_rounded_once(dtype, size, steps):
     want = exact(g, steps)
     off = relative(lib.orthogonalize(g, torch.empty_like(g), steps=steps), want)
     assert off <= relative(want.to(dtype), want) + 2 * iterates(steps, max(size))
+
+
+def bound(dtype, want, steps, side):
+    """With few singular values, or few sums, the iterates' error is no mean any more: four times as much.  Doubles: three sums of at most
+    `side` terms a step, each off by at most side 2^-53."""
+    if dtype == torch.float64:
+        return 3 * steps * side * 2.0 ** -53
+    return relative(want.to(dtype), want) + 8 * iterates(steps, side)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("size", [(24, 50, 8000), (8, 8192, 128), (9, 16384, 1), (1, 128, 9000), (5, 3, 30000), (24, 8000, 33)], ids=str)
+def test_short_sides_of_many_columns(dtype, size):
+    """Short sides up to 128 that neither one workgroup nor the chunks of columns take: more chunks than the chip holds at a time, or more
+    partial sums than are worth reading again."""
+    lib = _lib()
+    g = data(1, dtype, *size)
+    for steps in (1, 2, 5):
+        out = lib.orthogonalize(g, torch.empty_like(g), steps=steps)
+        for m in (0, size[0] - 1):
+            want = exact(g[m], steps)
+            assert relative(out[m], want) <= bound(dtype, want, steps, max(size)), (steps, m)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32], ids=str)
+@pytest.mark.parametrize("size", [(1, 3, 66000), (2, 3, 66000), (2, 66000, 3)], ids=str)
+def test_sides_above_65536(dtype, size):
+    lib = _lib()
+    g = data(1, dtype, *size)
+    out = lib.orthogonalize(g, torch.empty_like(g), steps=2)
+    for got, m in zip(out, g):
+        want = exact(m, 2)
+        assert relative(got, want) <= bound(dtype, want, 2, max(size))
