@@ -337,8 +337,9 @@ def chol_solve(A, B=None, want_inverse=False):
 
 # ---- products grouped by expert, orthogonalised update ---------------------------------------------
 # These take torch tensors on the GPU (rows of any stride, the last dimension contiguous), launch on torch's current stream
-# of the tensors' device and return `out`, which overlaps no operand; nothing is recorded for autograd.  torch is
-# imported only when one is called, but has to have been imported before this module: there is one HIP runtime in a process.
+# of the tensors' device and return `out`, which overlaps no operand.  Like torch's own functions with an `out`, they record
+# nothing for autograd, refuse tensors that require a gradient while it records, and count as a change of `out` in place.  torch
+# is imported only when one is called, but has to have been imported before this module: there is one HIP runtime in a process.
 F64, F32, BF16, F16 = 0, 1, 2, 3
 
 lib.gpx_grouped_gemm.argtypes = [_i, _i, _i64, _i64, _i64, _i64, _d, _vp, _i64, _vp, _i64, _i64, _vp, _d, _vp, _i64, _vp]
@@ -352,7 +353,7 @@ _codes = {}
 
 
 def _load_torch():
-    global _torch, _raw_stream
+    global _torch, _raw_stream, _changed, _current_device
     import torch
     # torch brings a HIP runtime of its own; loaded behind another one, it finds no GPU
     with open("/proc/self/maps") as maps:
@@ -361,7 +362,15 @@ def _load_torch():
     _codes.update({torch.float64: F64, torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
     # the handle of torch's current stream of a device; the public way builds a Stream object for it (1 us of a 6 us call)
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    _changed = torch.autograd.graph.increment_version
     _torch = torch
+
+
+def _unrecorded(*tensors):
+    for t in tensors:
+        if t.requires_grad and _torch.is_grad_enabled():
+            raise ValueError("nothing is recorded for autograd: call under torch.no_grad(), or with detached tensors")
 
 
 def _dtype(t, what):
@@ -386,7 +395,7 @@ def _rows(shape, stride, what):
 
 def _one_device(first, *others):
     index = first.get_device()
-    if index < 0 or not first.is_cuda:
+    if index < 0:
         raise ValueError(f"tensors on the GPU are wanted, not on {first.device}")
     for t in others:
         if t.get_device() != index:
@@ -394,16 +403,18 @@ def _one_device(first, *others):
     return index
 
 
-def _launch(fn, what, index, *args):
-    """fn(..., stream) on torch's current stream of device `index`; the null stream belongs to the current device."""
+def _launch(fn, what, index, out, *args):
+    """fn(..., stream), which writes `out`, on torch's current stream of device `index`; the null stream belongs to the current
+    device."""
     stream = _raw_stream(index)
-    if stream or index == _torch.cuda.current_device():
+    if stream or index == _current_device():
         status = fn(*args, stream)
     else:
         with _torch.cuda.device(index):
             status = fn(*args, stream)
     if status:
         check(status, what)
+    _changed(out)   # a backward pass that saved `out` finds out
 
 
 def _offsets(offsets, groups):
@@ -428,6 +439,7 @@ def grouped_gemm(x, w, offsets, out, w_kc=True, alpha=1.0, beta=0.0):
     x (T, K), out (T, N); w (G, N, K) for w_kc, else (G, K, N); offsets (G + 1,) int64 on the device.  The gradient of x is
     grouped_gemm(dy, w, offsets, dx, w_kc=not w_kc); that of w is grouped_gemm_dw."""
     code = _dtype(x, "x")
+    _unrecorded(x, w, out)
     index = _one_device(x, w, offsets, out)
     if w.dtype is not x.dtype or out.dtype is not x.dtype:
         raise ValueError("x, w and out have to be of one type")
@@ -441,7 +453,7 @@ def grouped_gemm(x, w, offsets, out, w_kc=True, alpha=1.0, beta=0.0):
     tw = w.stride()
     ldx, ldw, ldy = _rows(sx, x.stride(), "x"), _rows(sw, tw, "w"), _rows(so, out.stride(), "out")
     _offsets(offsets, groups)
-    _launch(lib.gpx_grouped_gemm, "grouped_gemm", index, code, w_kc, groups, rows, n, k, alpha, x.data_ptr(), ldx, w.data_ptr(),
+    _launch(lib.gpx_grouped_gemm, "grouped_gemm", index, out, code, w_kc, groups, rows, n, k, alpha, x.data_ptr(), ldx, w.data_ptr(),
             ldw, tw[0] if groups > 1 else 0, offsets.data_ptr(), beta, out.data_ptr(), ldy)
     return out
 
@@ -450,6 +462,7 @@ def grouped_gemm_dw(x, dy, offsets, out, alpha=1.0, beta=0.0):
     """out[g] = alpha * dy_g^T x_g + beta * out[g] over the rows of every group: x (T, K), dy (T, N), out (G, N, K) of their type,
     or float32 for 16-bit rows.  For weights in the (G, K, N) layout exchange x and dy."""
     code, code_out = _dtype(x, "x"), _dtype(out, "out")
+    _unrecorded(x, dy, out)
     index = _one_device(x, dy, offsets, out)
     if dy.dtype is not x.dtype:
         raise ValueError("x and dy have to be of one type")
@@ -464,7 +477,7 @@ def grouped_gemm_dw(x, dy, offsets, out, alpha=1.0, beta=0.0):
     ldx, ldz, ldc = _rows(sx, x.stride(), "x"), _rows(sz, dy.stride(), "dy"), _rows(so, tc, "out")
     _offsets(offsets, groups)
     work, size = _work(lib.gpx_grouped_gemm_dw_work, x, code, groups, rows, k, n)
-    _launch(lib.gpx_grouped_gemm_dw, "grouped_gemm_dw", index, code, code_out, groups, rows, k, n, alpha, x.data_ptr(), ldx,
+    _launch(lib.gpx_grouped_gemm_dw, "grouped_gemm_dw", index, out, code, code_out, groups, rows, k, n, alpha, x.data_ptr(), ldx,
             dy.data_ptr(), ldz, offsets.data_ptr(), beta, out.data_ptr(), ldc, tc[0] if groups > 1 else 0,
             work.data_ptr() if size else None, size)
     return out
@@ -474,6 +487,7 @@ def orthogonalize(g, out, steps=5, coef=None, eps=1e-7):
     """The Newton-Schulz update of g (M, N) or (B, M, N) into out (of g's shape and type; g itself is allowed): g / (|g|_F + eps),
     then `steps` times x <- a x + (b A + c A A) x with A = x x^T.  coef: (a, b, c), or one such triple for every step."""
     code = _dtype(g, "g")
+    _unrecorded(g, out)
     index = _one_device(g, out)
     shape = g.shape
     if out.dtype is not g.dtype or out.shape != shape:
@@ -491,7 +505,7 @@ def orthogonalize(g, out, steps=5, coef=None, eps=1e-7):
         elif table.shape != (steps, 3):
             raise ValueError("coef: three values, or three for every step")
     work, size = _work(lib.gpx_orthogonalize_work, g, code, batch, cols, rows)
-    _launch(lib.gpx_orthogonalize, "orthogonalize", index, code, batch, cols, rows, g.data_ptr(), ldg, tg[0] if batch > 1 else 0, steps,
+    _launch(lib.gpx_orthogonalize, "orthogonalize", index, out, code, batch, cols, rows, g.data_ptr(), ldg, tg[0] if batch > 1 else 0, steps,
             table.ctypes.data if table is not None and steps > 0 else None, eps, out.data_ptr(), ldo, to[0] if batch > 1 else 0,
             work.data_ptr() if size else None, size)
     return out
