@@ -629,6 +629,10 @@ extern "C" int gpx_grouped_gemm(int dtype, int w_kc, int64_t groups, int64_t T, 
     if (groups == 0 || T == 0 || N == 0) return GPX_OK;   // no row of Y belongs to a group
     if (!Y || !offsets || (K > 0 && (!X || !W))) return GPX_ERR_ARG;
     if (misaligned(X, e) || misaligned(W, e) || misaligned(Y, e) || misaligned(offsets, 8)) return GPX_ERR_ARG;
+    const ByteRows y = {Y, 1, 0, T, ldy * e, N * e};
+    if (gpx_share_bytes(y, {X, 1, 0, T, ldx * e, K * e}) || gpx_share_bytes(y, {offsets, 1, 0, 1, 0, 8 * (groups + 1)}) ||
+        gpx_share_bytes(y, {W, groups, stride_w * e, w_kc ? N : K, ldw * e, (w_kc ? K : N) * e}))
+        return GPX_ERR_ARG;
     StreamDevice dev(static_cast<hipStream_t>(hip_stream));
     if (dev.status) return dev.status;
     GroupedArgs g = {static_cast<const char*>(X), static_cast<const char*>(W), static_cast<char*>(Y), offsets, ldx * e, ldw * e,
@@ -657,6 +661,11 @@ extern "C" int gpx_grouped_gemm_dw(int dtype, int c_dtype, int64_t groups, int64
     if (misaligned(X, e) || misaligned(Z, e) || misaligned(C, ec) || misaligned(offsets, 8)) return GPX_ERR_ARG;
     const DwPlan plan = dw_plan(e, ec, groups, T, M, N);
     if (plan.part_rows && (!work || misaligned(work, 16) || work_bytes < dw_work_bytes(plan, e, M, N))) return GPX_ERR_ARG;
+    const ByteRows c = {C, groups, stride_c * ec, N, ldc * ec, M * ec}, table = {offsets, 1, 0, 1, 0, 8 * (groups + 1)};
+    const ByteRows x = {X, 1, 0, T, ldx * e, M * e}, z = {Z, 1, 0, T, ldz * e, N * e}, w = {work, 1, 0, 1, 0, dw_work_bytes(plan, e, M, N)};
+    if (gpx_share_bytes(c, x) || gpx_share_bytes(c, z) || gpx_share_bytes(c, table) || gpx_share_bytes(w, x) || gpx_share_bytes(w, z) ||
+        gpx_share_bytes(w, c) || gpx_share_bytes(w, table))
+        return GPX_ERR_ARG;
     StreamDevice dev(static_cast<hipStream_t>(hip_stream));
     if (dev.status) return dev.status;
     const GroupedDwArgs g = {static_cast<const char*>(X), static_cast<const char*>(Z), static_cast<char*>(C), offsets, ldx * e, ldz * e, ldc * ec,

@@ -1104,7 +1104,12 @@ extern "C" int gpx_orthogonalize(int dtype, int64_t batch, int64_t M, int64_t N,
     if (!G || !O || !work) return GPX_ERR_ARG;
     const uintptr_t e = dtype == GPX_F64 ? 8 : dtype == GPX_F32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(G) % e || reinterpret_cast<uintptr_t>(O) % e || reinterpret_cast<uintptr_t>(work) % 16) return GPX_ERR_ARG;
-    if (work_bytes < ortho_work(dtype, batch, (int)N, (int)M).total) return GPX_ERR_ARG;
+    const int64_t need = ortho_work(dtype, batch, (int)N, (int)M).total;
+    if (work_bytes < need) return GPX_ERR_ARG;
+    const int64_t el = (int64_t)e;
+    const ByteRows in = {G, batch, stride_g * el, N, ldg * el, M * el}, out = {O, batch, stride_o * el, N, ldo * el, M * el}, room = {work, 1, 0, 1, 0, need};
+    const bool in_place = G == O && (N == 1 || ldg == ldo) && (batch == 1 || stride_g == stride_o);
+    if ((!in_place && gpx_share_bytes(in, out)) || gpx_share_bytes(room, in) || gpx_share_bytes(room, out)) return GPX_ERR_ARG;
     double table[3 * kMaxSteps];
     for (int k = 0; k < steps; ++k)
         for (int c = 0; c < 3; ++c) {
