@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const T* __restrict__ G
     __shared__ double ws[4];
     if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.y * kParts + blockIdx.x] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
+    if (threadIdx.x == 0) part[blockIdx.y * (long)gridDim.x + blockIdx.x] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
 }
 
 // the norm of one matrix from its partial sums, in every lane
@@ -88,7 +88,7 @@ struct Factor {
 template <class T>
 __global__ __launch_bounds__(256) void ortho_normalize_kernel(const T* G, long ldg, long stride_g, int rows, int cols, const double* __restrict__ part,
                                                               int parts, double eps, T* X, long ldx, long stride_x) {
-    const double norm = norm_of(part + blockIdx.y * kParts, parts) + eps;
+    const double norm = norm_of(part + blockIdx.y * (long)parts, parts) + eps;
     each_run(rows, cols, blockIdx.x * 256L + threadIdx.x, gridDim.x * 256L, [&](int r, int c) {
         T v[8];
         load_run(G + blockIdx.y * stride_g + r * ldg + c, cols - c, v);
@@ -178,7 +178,7 @@ template <class T, class F>
 __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ G, long ldg, long stride_g, int rows, int cols, int pcols,
                                                           const double* __restrict__ part, int parts, double eps, double scale, char* __restrict__ X,
                                                           long ldx, long stride_x) {
-    const double norm = norm_of(part + blockIdx.y * kParts, parts) + eps;
+    const double norm = norm_of(part + blockIdx.y * (long)parts, parts) + eps;
     const Factor by(scale / norm);
     each_run(rows, pcols, blockIdx.x * 256L + threadIdx.x, gridDim.x * 256L, [&](int r, int c) {
         T v[8];
@@ -383,21 +383,23 @@ template <class F> long row_bytes(int cols) {
     const long b = Iterate<F>::bytes(padded<F>(cols));
     return b % 1024 == 0 ? b + 128 : b;
 }
+long up256(long v) { return (v + 255) / 256 * 256; }
+template <class F> long norm_runs(int rows, int cols) { return (long)rows * ((padded<F>(cols) + 7) / 8); }
+template <class F> int norm_parts(int rows, int cols) { return (int)std::min<long>((norm_runs<F>(rows, cols) + 511) / 512, kParts); }
 template <class F> OrthoWork ortho_work_of(long batch, int rows, int cols) {
     const int s = std::min(rows, cols);
-    auto up = [](long v) { return (v + 255) / 256 * 256; };
     OrthoWork o;
     o.ldx = row_bytes<F>(cols);
     o.sx = o.ldx * rows;
     o.lda = row_bytes<F>(s);
     o.sa = o.lda * s;
     o.part = 0;
-    o.x[0] = up(batch * kParts * 8);
-    o.x[1] = o.x[0] + up(batch * o.sx);
-    o.a = o.x[1] + up(batch * o.sx);
-    o.b = o.a + up(batch * o.sa);
-    o.diag[0] = o.b + up(batch * o.sa);
-    o.diag[1] = o.diag[0] + (__is_same(F, double) ? 0 : up(batch * s * 4));
+    o.x[0] = up256(batch * norm_parts<F>(rows, cols) * 8L);
+    o.x[1] = o.x[0] + up256(batch * o.sx);
+    o.a = o.x[1] + up256(batch * o.sx);
+    o.b = o.a + up256(batch * o.sa);
+    o.diag[0] = o.b + up256(batch * o.sa);
+    o.diag[1] = o.diag[0] + (__is_same(F, double) ? 0 : up256(batch * s * 4));
     o.total = o.diag[1] + (o.diag[1] - o.diag[0]);
     return o;
 }
@@ -847,7 +849,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_chunk_kernel(const T* 
         tj[x] = t * 16;
     }
     if (g.first) {
-        const Factor by(g.scale / (norm_of(g.part + mat * kParts, g.parts) + g.eps));
+        const Factor by(g.scale / (norm_of(g.part + mat * (long)g.parts, g.parts) + g.eps));
         for (int e = threadIdx.x; e < K::IMAGE / 16; e += kSmallWaves * 64) reinterpret_cast<mm::v4i*>(X)[e] = mm::v4i{0, 0, 0, 0};
         __syncthreads();
         const T* from = G + mat * g.stride_g + (tall ? c0 * g.ldg : c0);
@@ -937,33 +939,36 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_chunk_kernel(const T* 
 }
 
 struct ChunkPlan { int chunks; long images, sums, total; };   // chunks 0: not this way.  bytes: images of X, one set of sums, workspace
-template <int NB> ChunkPlan chunk_plan_of(long batch, int l) {
+template <int NB> ChunkPlan chunk_plan_of(long batch, int l, long part_bytes) {
     typedef Chunk<NB> K;
     const long chunks = (l + K::LC - 1) / K::LC;
     // Two rounds of workgroups pay for short sides up to 64 (f32 24 x 50 x 4000: 250 -> 140 us), not for longer ones (24 x 128 x 2048:
     // 212 -> 242); every workgroup reads all chunks' sums (1 x 128 x 8192, 2.4 MB: 371 -> 173).
     if (chunks * batch > (NB <= 2 ? 512 : 256) || chunks * K::TILES > 2400) return {0, 0, 0, 0};
-    auto up = [](long v) { return (v + 255) / 256 * 256; };
-    const long images = up(batch * chunks * K::IMAGE), sums = batch * chunks * K::TILES * 1024L;
-    return {(int)chunks, images, sums, up(batch * kParts * 8) + images + 2 * sums};
+    const long images = up256(batch * chunks * K::IMAGE), sums = batch * chunks * K::TILES * 1024L;
+    return {(int)chunks, images, sums, part_bytes + images + 2 * sums};
 }
 ChunkPlan chunk_plan(long batch, int rows, int cols) {
     const int s = std::min(rows, cols), l = std::max(rows, cols);
     bool two;
     if (s > kSmallSide || small_lds(rows, cols, two)) return {0, 0, 0, 0};
+    const long part = ortho_work_of<mm::Split>(batch, rows, cols).x[0];
     switch ((s + 31) / 32) {
-        case 1: return chunk_plan_of<1>(batch, l);
-        case 2: return chunk_plan_of<2>(batch, l);
-        case 3: return chunk_plan_of<3>(batch, l);
-        default: return chunk_plan_of<4>(batch, l);
+        case 1: return chunk_plan_of<1>(batch, l, part);
+        case 2: return chunk_plan_of<2>(batch, l, part);
+        case 3: return chunk_plan_of<3>(batch, l, part);
+        default: return chunk_plan_of<4>(batch, l, part);
     }
 }
 
-OrthoWork ortho_work(int dtype, long batch, int rows, int cols) {
-    OrthoWork o = dtype == GPX_F64    ? ortho_work_of<double>(batch, rows, cols)
-                                    : ortho_work_of<mm::Split>(batch, rows, cols);
-    if (dtype != GPX_F64) o.total = std::max(o.total, chunk_plan(batch, rows, cols).total);
-    return o;
+// bytes of workspace of the path that is taken
+long ortho_work(int dtype, long batch, int rows, int cols) {
+    if (dtype == GPX_F64) return ortho_work_of<double>(batch, rows, cols).total;
+    const OrthoWork o = ortho_work_of<mm::Split>(batch, rows, cols);
+    bool two;
+    if (small_lds(rows, cols, two)) return o.x[0];   // the norms, for no steps at all
+    const ChunkPlan plan = chunk_plan(batch, rows, cols);
+    return plan.chunks ? plan.total : o.total;
 }
 
 // rows x cols row-major (the column-major cols x rows of the C interface)
@@ -1000,15 +1005,15 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
     }
     const OrthoWork o = ortho_work_of<F>(batch, rows, cols);
     double* part = reinterpret_cast<double*>(work + o.part);
-    const long runs = (long)rows * ((padded<F>(cols) + 7) / 8);
-    const int parts = (int)std::min<long>((runs + 511) / 512, kParts);
+    const long runs = norm_runs<F>(rows, cols);
+    const int parts = norm_parts<F>(rows, cols);
     ortho_norm_kernel<T><<<dim3(parts, batch), 256, 0, st>>>(G, ldg, stride_g, rows, cols, part);
     HIP_TRY(hipGetLastError());
     const dim3 grid((unsigned)std::min<long>((runs + 255) / 256, 2048), (unsigned)batch);
     if constexpr (!__is_same(F, double)) {
         const ChunkPlan plan = chunk_plan(batch, rows, cols);
         if (steps > 0 && plan.chunks) {
-            char* images = work + (batch * kParts * 8L + 255) / 256 * 256;
+            char* images = work + o.x[0];
             mm::v4f* sums[2] = {reinterpret_cast<mm::v4f*>(images + plan.images), reinterpret_cast<mm::v4f*>(images + plan.images + plan.sums)};
             OrthoChunkArgs g = {ldg, stride_g, ldo, stride_o, rows, cols, plan.chunks, parts, part, eps, f.start, images};
             auto go = [&](auto blocks) {
@@ -1088,7 +1093,7 @@ bool switched_off(int dtype, int64_t M, int64_t N) { return (dtype == GPX_BF16 |
 extern "C" int gpx_orthogonalize_work(int dtype, int64_t batch, int64_t M, int64_t N, int64_t* work_bytes) {
     if (!work_bytes || !sizes_ok(dtype, batch, M, N)) return GPX_ERR_ARG;
     if (batch && M && N && switched_off(dtype, M, N)) return GPX_ERR_ARG;
-    *work_bytes = batch && M && N ? ortho_work(dtype, batch, (int)N, (int)M).total : 0;
+    *work_bytes = batch && M && N ? ortho_work(dtype, batch, (int)N, (int)M) : 0;
     return GPX_OK;
 }
 
@@ -1104,7 +1109,7 @@ extern "C" int gpx_orthogonalize(int dtype, int64_t batch, int64_t M, int64_t N,
     if (!G || !O || !work) return GPX_ERR_ARG;
     const uintptr_t e = dtype == GPX_F64 ? 8 : dtype == GPX_F32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(G) % e || reinterpret_cast<uintptr_t>(O) % e || reinterpret_cast<uintptr_t>(work) % 16) return GPX_ERR_ARG;
-    const int64_t need = ortho_work(dtype, batch, (int)N, (int)M).total;
+    const int64_t need = ortho_work(dtype, batch, (int)N, (int)M);
     if (work_bytes < need) return GPX_ERR_ARG;
     const int64_t el = (int64_t)e;
     const ByteRows in = {G, batch, stride_g * el, N, ldg * el, M * el}, out = {O, batch, stride_o * el, N, ldo * el, M * el}, room = {work, 1, 0, 1, 0, need};
