@@ -84,3 +84,12 @@ def test_sides_above_65536(dtype, size):
     for got, m in zip(out, g):
         want = exact(m, 2)
         assert relative(got, want) <= bound(dtype, want, 2, max(size))
+
+
+@pytest.mark.parametrize("size", [(60, 2900), (90, 3000), (96, 2000), (2000, 120), (128, 1300), (64, 20), (128, 128)], ids=str)
+@pytest.mark.parametrize("steps", [3, 6])
+def test_float32_keeps_22_bits_on_short_sides(size, steps):
+    """Every number of 32-row blocks of the short side, in chunks of columns and in one workgroup."""
+    lib = _lib()
+    g = data(1, torch.float32, *size)
+    assert relative(lib.orthogonalize(g, torch.empty_like(g), steps=steps), exact(g, steps)) <= iterates(steps, max(size))
