@@ -43,32 +43,91 @@ template <class T> __device__ __forceinline__ void load_run(const T* p, int coun
     }
 }
 
-// Sums of squares in double: neither overflow nor loss for any narrower input, one order of addition.
+// Sums of squares in double: neither overflow nor loss for any narrower input, one order of addition.  Doubles take three sums, of
+// values beyond 2^480, below 2^-480 and between, the outer ones scaled by 2^-600 and 2^600, and leave the root instead.
+template <class T> struct Squares {
+    double s;
+    __device__ __forceinline__ void add(T v) { s = fma(as_double(v), as_double(v), s); }
+    __device__ __forceinline__ void join(int d) { s += __shfl_xor(s, d, 64); }
+    __device__ __forceinline__ void join(const Squares& o) { s += o.s; }
+    __device__ __forceinline__ double part() const { return s; }
+};
+template <> struct Squares<double> {
+    double s, large, little;
+    __device__ __forceinline__ void add(double v) {
+        const double a = fabs(v), b = a > 0x1p480 ? a * 0x1p-600 : a < 0x1p-480 ? a * 0x1p600 : a;
+        const double q = b * b;   // (NaN goes between)
+        if (a > 0x1p480) large += q;
+        else if (a < 0x1p-480) little += q;
+        else s += q;
+    }
+    __device__ __forceinline__ void join(int d) {
+        s += __shfl_xor(s, d, 64);
+        large += __shfl_xor(large, d, 64);
+        little += __shfl_xor(little, d, 64);
+    }
+    __device__ __forceinline__ void join(const Squares& o) {
+        s += o.s;
+        large += o.large;
+        little += o.little;
+    }
+    __device__ __forceinline__ double part() const {
+        return hypot(hypot(sqrt(large) * 0x1p600, sqrt(s)), sqrt(little) * 0x1p-600);
+    }
+};
+
 template <class T>
 __global__ __launch_bounds__(256) void ortho_norm_kernel(const T* __restrict__ G, long ldg, long stride_g, int rows, int cols, double* __restrict__ part) {
     const T* g = G + blockIdx.y * stride_g;
-    double s = 0.0;
+    Squares<T> s = {};
     each_run(rows, cols, blockIdx.x * 256L + threadIdx.x, gridDim.x * 256L, [&](int r, int c) {
         T v[8];
         load_run(g + r * ldg + c, cols - c, v);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) s = fma(as_double(v[x]), as_double(v[x]), s);
+        for (int x = 0; x < 8; ++x) s.add(v[x]);
     });
 #pragma unroll
-    for (int d = 32; d; d /= 2) s += __shfl_xor(s, d, 64);
-    __shared__ double ws[4];
+    for (int d = 32; d; d /= 2) s.join(d);
+    __shared__ Squares<T> ws[4];
     if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.y * (long)gridDim.x + blockIdx.x] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
+    if (threadIdx.x == 0) {
+        Squares<T> a = ws[0], b = ws[2];
+        a.join(ws[1]);
+        b.join(ws[3]);
+        a.join(b);
+        part[blockIdx.y * (long)gridDim.x + blockIdx.x] = a.part();
+    }
 }
 
-// the norm of one matrix from its partial sums, in every lane
-__device__ __forceinline__ double norm_of(const double* part, int parts) {
+// the norm of one matrix of T from its partial sums (or roots), in every lane
+template <class T> __device__ __forceinline__ double norm_of(const double* part, int parts) {
     double s = 0.0;
-    for (int e = threadIdx.x & 63; e < parts; e += 64) s += part[e];
+    if constexpr (__is_same(T, double)) {
+        double most = 0.0;
+        bool finite = true;
+        for (int e = threadIdx.x & 63; e < parts; e += 64) {
+            most = fmax(most, part[e]);
+            finite = finite && isfinite(part[e]);
+            s += part[e];
+        }
 #pragma unroll
-    for (int d = 32; d; d /= 2) s += __shfl_xor(s, d, 64);
-    return sqrt(s);
+        for (int d = 32; d; d /= 2) {
+            most = fmax(most, __shfl_xor(most, d, 64));
+            s += __shfl_xor(s, d, 64);
+        }
+        if (!__all(finite) || most == 0.0) return s;   // an infinity or NaN, or zero
+        s = 0.0;
+        for (int e = threadIdx.x & 63; e < parts; e += 64) s = fma(part[e] / most, part[e] / most, s);
+#pragma unroll
+        for (int d = 32; d; d /= 2) s += __shfl_xor(s, d, 64);
+        return most * sqrt(s);
+    } else {
+        for (int e = threadIdx.x & 63; e < parts; e += 64) s += part[e];
+#pragma unroll
+        for (int d = 32; d; d /= 2) s += __shfl_xor(s, d, 64);
+        return sqrt(s);
+    }
 }
 
 // A positive factor of any size as mantissa and exponent: floats times it without overflow on the way, by the exact power of
@@ -88,7 +147,7 @@ struct Factor {
 template <class T>
 __global__ __launch_bounds__(256) void ortho_normalize_kernel(const T* G, long ldg, long stride_g, int rows, int cols, const double* __restrict__ part,
                                                               int parts, double eps, T* X, long ldx, long stride_x) {
-    const double norm = norm_of(part + blockIdx.y * (long)parts, parts) + eps;
+    const double norm = norm_of<T>(part + blockIdx.y * (long)parts, parts) + eps;
     each_run(rows, cols, blockIdx.x * 256L + threadIdx.x, gridDim.x * 256L, [&](int r, int c) {
         T v[8];
         load_run(G + blockIdx.y * stride_g + r * ldg + c, cols - c, v);
@@ -178,7 +237,7 @@ template <class T, class F>
 __global__ __launch_bounds__(256) void ortho_scale_kernel(const T* __restrict__ G, long ldg, long stride_g, int rows, int cols, int pcols,
                                                           const double* __restrict__ part, int parts, double eps, double scale, char* __restrict__ X,
                                                           long ldx, long stride_x) {
-    const double norm = norm_of(part + blockIdx.y * (long)parts, parts) + eps;
+    const double norm = norm_of<T>(part + blockIdx.y * (long)parts, parts) + eps;
     const Factor by(scale / norm);
     each_run(rows, pcols, blockIdx.x * 256L + threadIdx.x, gridDim.x * 256L, [&](int r, int c) {
         T v[8];
@@ -849,7 +908,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_chunk_kernel(const T* 
         tj[x] = t * 16;
     }
     if (g.first) {
-        const Factor by(g.scale / (norm_of(g.part + mat * (long)g.parts, g.parts) + g.eps));
+        const Factor by(g.scale / (norm_of<T>(g.part + mat * (long)g.parts, g.parts) + g.eps));
         for (int e = threadIdx.x; e < K::IMAGE / 16; e += kSmallWaves * 64) reinterpret_cast<mm::v4i*>(X)[e] = mm::v4i{0, 0, 0, 0};
         __syncthreads();
         const T* from = G + mat * g.stride_g + (tall ? c0 * g.ldg : c0);

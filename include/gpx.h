@@ -109,7 +109,7 @@ int gpx_grouped_gemm_dw(int dtype, int c_dtype, int64_t groups, int64_t T, int64
  * into O.  The iterates of F64 are doubles; all others hold each value to 22 bits or to 2^-39 of the largest possible one, the
  * coarser of the two, sums are taken in 32 bits, and the result is rounded once.  coef: HOST, 3*steps finite values a, b, c of every
  * step; NULL: (3.4445, -4.7750, 2.0315) in each.  Coefficients that could carry singular values past 2^100 are refused,
- * except for F64.  eps >= 1e-300: a zero matrix gives zeros (and so does one of F64 whose squares sum past 1.8e308).  A
+ * except for F64.  eps >= 1e-300: a zero matrix gives zeros (and so does one of F64 whose norm passes 1.8e308).  A
  * matrix that holds an infinity or NaN gives non-finite values in its own result only.  O may be G (same ld and stride).
  * work: as above, gpx_orthogonalize_work bytes.  Sides up to 2^20; BF16 and F16: up to 65536, both calls refuse longer ones. */
 int gpx_orthogonalize_work(int dtype, int64_t batch, int64_t M, int64_t N, int64_t* work_bytes);

@@ -1,5 +1,7 @@
 """GPU tests of how exactly the orthogonalised update is computed: 22 bits of every iterate on each of its paths (one workgroup
 for all steps, chunks of columns with one launch a step, three tiled products a step), and one rounding of the result."""
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -93,3 +95,27 @@ def test_float32_keeps_22_bits_on_short_sides(size, steps):
     lib = _lib()
     g = data(1, torch.float32, *size)
     assert relative(lib.orthogonalize(g, torch.empty_like(g), steps=steps), exact(g, steps)) <= iterates(steps, max(size))
+
+
+@pytest.mark.parametrize("size", [(30, 44), (300, 140), (3, 20000)], ids=str)
+@pytest.mark.parametrize("scale", [-1060, -900, -600, -500, 0, 480, 600, 1000], ids=lambda e: f"2^{e}")
+@pytest.mark.parametrize("steps", [0, 2])
+def test_doubles_of_any_size(size, scale, steps):
+    """Squares of doubles may be out of range where the norm is not: the result is that of the matrix and eps times a power of two."""
+    lib = _lib()
+
+    def times(t, e):   # t 2^e, where 2^e may be out of range
+        return t * 2.0 ** (e // 2) * 2.0 ** (e - e // 2)
+    g = data(1, torch.float64, *size).clamp(-3, 3)
+    g[0, 0] = g[-1, -1] = 2.0 ** -300   # far from the rest
+    g, eps = times(g, scale), 1e-300
+    x = times(g, -scale)   # exact
+    x = x / (torch.linalg.norm(x) + math.ldexp(eps, -scale))
+    tall = size[0] > size[1]
+    x = x.T.contiguous() if tall else x
+    a, b, c = oracle.COEF
+    for _ in range(steps):
+        p = x @ x.T.contiguous()
+        x = a * x + b * (p @ x) + c * (p @ (p @ x))
+    out = lib.orthogonalize(g, torch.empty_like(g), steps=steps, eps=eps)
+    assert relative(out, x.T if tall else x) <= (3 * steps + 1) * max(size) * 2.0 ** -53
