@@ -397,27 +397,29 @@ bool whole_chunks(const void* p, long ld_bytes, long stride_bytes, long extent, 
 
 template <int V> using Int = std::integral_constant<int, V>;
 
+// What a launch takes: less than 2^32 work-items along x (the grids are rounded up to a multiple of 32 workgroups).
+bool one_launch(long workgroups, int threads) { return (workgroups + 31) * threads < 1L << 32; }
 // A row-tile count that is never less than sum of ceil(rows / BM)
 long row_tiles(long T, int groups, int BM) { return T / BM + (groups < T ? groups : T); }
 
 // Which tile: the one whose rounds over the 256 CUs take the least time, by the time of a K step (128 bytes of k) with the
 // chip full and with one workgroup on a CU, and of prologue and epilogue.  us, measured on a full chip:
-struct TileCost { int bm, bn, slots; double step, alone, rest; };
+struct TileCost { int bm, bn, slots, threads; double step, alone, rest; };
 constexpr TileCost kCost16[] = {
-    {256, 256, 256, 1.50, 1.50, 14.0},   // one workgroup of 8 waves a CU: 1.17-1.25 PFLOP/s on 8 x 4096 x 4096 x 7168
-    {128, 128, 512, 1.05, 0.52, 5.0},    // two of 4 waves: 1.00-1.07
-    {64, 64, 512, 0.38, 0.25, 2.3},      // two of 4 waves, four LDS stages: 0.63
-    {32, 128, 512, 0.43, 0.30, 2.0},     // a few rows a group, W in 256-byte runs (n contiguous): the read of W bounds it
-    {32, 64, 768, 0.36, 0.25, 2.0},      // the same, k contiguous: 5.5 TB/s on 32 x 2816 x 2048
-    {32, 64, 256, 0.25, 0.10, 4.0},      // few tiles and long k: four groups of waves share the sum (one of 8192 x 8192: 40 -> 28 us)
-    {64, 64, 256, 0.25, 0.11, 5.0},
-    {32, 16, 256, 0.12, 0.05, 4.0}};     // narrow ones, eight single waves
+    {256, 256, 256, 512, 1.50, 1.50, 14.0},   // one workgroup of 8 waves a CU: 1.17-1.25 PFLOP/s on 8 x 4096 x 4096 x 7168
+    {128, 128, 512, 256, 1.05, 0.52, 5.0},    // two of 4 waves: 1.00-1.07
+    {64, 64, 512, 256, 0.38, 0.25, 2.3},      // two of 4 waves, four LDS stages: 0.63
+    {32, 128, 512, 256, 0.43, 0.30, 2.0},     // a few rows a group, W in 256-byte runs (n contiguous): the read of W bounds it
+    {32, 64, 768, 256, 0.36, 0.25, 2.0},      // the same, k contiguous: 5.5 TB/s on 32 x 2816 x 2048
+    {32, 64, 256, 1024, 0.25, 0.10, 4.0},      // few tiles and long k: four groups of waves share the sum (one of 8192 x 8192: 40 -> 28 us)
+    {64, 64, 256, 1024, 0.25, 0.11, 5.0},
+    {32, 16, 256, 512, 0.12, 0.05, 4.0}};     // narrow ones, eight single waves
 // 4-byte floats and doubles; the last two as above: four groups of four waves (8 groups of 2 rows, 1024 x 1024 in doubles: 35 -> 27 us),
 // eight of one (30 rows, 512 x 8192 in floats, 512 x 4096 in doubles: 87 -> 32 us)
-constexpr TileCost kCost32[] = {{128, 128, 512, 3.30, 2.40, 3.0}, {64, 64, 256, 0.52, 0.52, 1.0}, {32, 64, 256, 0.32, 0.45, 1.0},
-                                 {32, 64, 256, 0.36, 0.33, 2.5}, {32, 16, 256, 0.18, 0.06, 3.0}};
-constexpr TileCost kCost64[] = {{128, 128, 512, 3.90, 2.20, 3.0}, {64, 64, 256, 0.51, 0.51, 1.0}, {32, 64, 256, 0.31, 0.45, 1.0},
-                                 {32, 64, 256, 0.36, 0.33, 2.5}, {32, 16, 256, 0.18, 0.06, 3.0}};
+constexpr TileCost kCost32[] = {{128, 128, 512, 256, 3.30, 2.40, 3.0}, {64, 64, 256, 256, 0.52, 0.52, 1.0}, {32, 64, 256, 256, 0.32, 0.45, 1.0},
+                                 {32, 64, 256, 1024, 0.36, 0.33, 2.5}, {32, 16, 256, 512, 0.18, 0.06, 3.0}};
+constexpr TileCost kCost64[] = {{128, 128, 512, 256, 3.90, 2.20, 3.0}, {64, 64, 256, 256, 0.51, 0.51, 1.0}, {32, 64, 256, 256, 0.31, 0.45, 1.0},
+                                 {32, 64, 256, 1024, 0.36, 0.33, 2.5}, {32, 16, 256, 512, 0.18, 0.06, 3.0}};
 double tile_time(const TileCost& c, double tiles, double steps) {
     const double full = floor(tiles / c.slots), left = tiles - full * c.slots;
     return full * (c.step * steps + c.rest) + (left > 256.0 ? c.step * steps + c.rest : left > 0.0 ? c.alone * steps + c.rest : 0.0);
@@ -437,19 +439,20 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
     auto tiles_of = [&](const TileCost& c) {   // half a row tile of every group is empty on average
         return std::max(busy, g.T / (double)c.bm + 0.5 * busy) * ((g.N + c.bn - 1) / c.bn);
     };
-    auto time_of = [&](const TileCost& c) { return tile_time(c, tiles_of(c), steps); };
+    auto fits = [&](const TileCost& c) { return one_launch(row_tiles(g.T, g.groups, c.bm) * ((g.N + c.bn - 1L) / c.bn), c.threads); };
+    auto time_of = [&](const TileCost& c) { return fits(c) ? tile_time(c, tiles_of(c), steps) : 1e300; };
     int rc = GPX_OK;
     auto go = [&](auto bm, auto bn, auto wr, auto wc, auto stages, auto kgroups, auto rest) {
         constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WR = decltype(wr)::value, WC = decltype(wc)::value, ST = decltype(stages)::value,
                       KG = decltype(kgroups)::value;
         constexpr bool REST = decltype(rest)::value != 0;
-        const long tiles = REST ? 4L * a.most : row_tiles(g.T, g.groups, BM) * ((g.N + BN - 1) / BN);
-        if (tiles >= (1L << 31) - 512) {
+        const long tiles = REST ? 4L * a.most : row_tiles(g.T, g.groups, BM) * ((g.N + BN - 1L) / BN);
+        constexpr int threads = WR * WC * 64 * KG;
+        if (!one_launch(tiles, threads)) {
             rc = GPX_ERR_UNSUPPORTED;
             return;
         }
         const unsigned grid = (unsigned)((tiles + 31) / 32 * 32);   // as many for every XCD (REST: whole tiles)
-        constexpr int threads = WR * WC * 64 * KG;
         if (w_kc && direct) grouped_kernel<T, BM, BN, WR, WC, ST, KG, true, true, REST><<<grid, threads, 0, st>>>(a);
         else if (direct) grouped_kernel<T, BM, BN, WR, WC, ST, KG, false, true, REST><<<grid, threads, 0, st>>>(a);
         else if constexpr (BM == 256 || KG > 1 || REST) rc = GPX_ERR_STATE;   // (never chosen for rows that are not direct)
@@ -499,8 +502,8 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
             case 6: go(Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<4>{}, whole); break;
             default: go(Int<32>{}, Int<16>{}, Int<1>{}, Int<1>{}, Int<3>{}, Int<8>{}, whole);
         }
-    } else if (const long units = row_tiles(g.T, g.groups, 32 * kShortSub) * ((g.N + 63) / 64);
-               direct && g.K * (long)sizeof(T) <= 512 && 32 * g.ldy < (long)mm::kRange && g.K > 0 && units >= 512 && units < (1L << 31) - 512) {
+    } else if (const long units = row_tiles(g.T, g.groups, 32 * kShortSub) * ((g.N + 63L) / 64);
+               direct && g.K * (long)sizeof(T) <= 512 && 32 * g.ldy < (long)mm::kRange && g.K > 0 && units >= 512 && one_launch(units, 256)) {
         // (fewer workgroups than slots on the chip: no better than single tiles)
         const unsigned grid = (unsigned)((units + 7) / 8 * 8);
         if (w_kc) grouped_short_kernel<T, true><<<grid, 256, 0, st>>>(g);
@@ -517,8 +520,9 @@ template <class T> int grouped_typed(hipStream_t st, bool w_kc, const GroupedArg
             default: go(Int<32>{}, Int<16>{}, Int<1>{}, Int<1>{}, Int<3>{}, Int<8>{}, whole);
         }
     }
+    if (rc) return rc;
     HIP_TRY(hipGetLastError());
-    return rc;
+    return GPX_OK;
 }
 
 // The weight gradient's tile and the rows of a part (0: not split), from sizes alone: the workspace follows from it.
@@ -577,8 +581,8 @@ template <class T, class O> int grouped_dw_typed(hipStream_t st, const GroupedDw
     int rc = GPX_OK;
     auto go = [&](auto bm, auto wr, auto wc, auto stages) {
         constexpr int B = decltype(bm)::value, WR = decltype(wr)::value, WC = decltype(wc)::value, ST = decltype(stages)::value;
-        const long tiles = (long)((g.N + B - 1) / B) * ((g.M + B - 1) / B);
-        if (tiles >= 1L << 31) {
+        const long tiles = (long)((g.N + B - 1L) / B) * ((g.M + B - 1L) / B);
+        if (!one_launch(tiles, WR * WC * 64)) {
             rc = GPX_ERR_UNSUPPORTED;
             return;
         }
@@ -605,8 +609,9 @@ template <class T, class O> int grouped_dw_typed(hipStream_t st, const GroupedDw
         if (plan.tile == 0) go(Int<128>{}, Int<2>{}, Int<2>{}, Int<2>{});
         else go(Int<64>{}, Int<2>{}, Int<2>{}, Int<2>{});
     }
+    if (rc) return rc;
     HIP_TRY(hipGetLastError());
-    return rc;
+    return GPX_OK;
 }
 
 constexpr long kMaxExtent = (1L << 31) - 1024;   // row, column and k numbers within one product are 32-bit

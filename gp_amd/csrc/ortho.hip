@@ -489,18 +489,17 @@ TileChoice choose_tile(bool sym, int I, int J, int K, int batch) {
 
 template <int V> using Int = std::integral_constant<int, V>;
 
-template <class F, class O, bool LAST, bool PKC, bool QKC, bool SYM> int launch(hipStream_t st, const OrthoArgs& g, int batch) {
+// dry: only looks whether a launch takes so many workgroups (less than 2^32 work-items)
+template <class F, class O, bool LAST, bool PKC, bool QKC, bool SYM> int launch(hipStream_t st, const OrthoArgs& g, int batch, bool dry) {
 #define GO(B, R, C, S, G) go(Int<B>{}, Int<R>{}, Int<C>{}, Int<S>{}, Int<G>{})
     int rc = GPX_OK;
     auto go = [&](auto tile, auto wr, auto wc, auto stages, auto groups) {
         constexpr int B = decltype(tile)::value, WR = decltype(wr)::value, WC = decltype(wc)::value, ST = decltype(stages)::value, KG = decltype(groups)::value;
         const long it = (g.I + B - 1) / B, jt = (g.J + B - 1) / B;
         const long grid = ((SYM ? it * (it + 1) / 2 : it * jt) * batch + 7) / 8 * 8;   // as many for every XCD
-        if (grid >= 1L << 31) {
-            rc = GPX_ERR_UNSUPPORTED;
-            return;
-        }
-        ortho_mm_kernel<F, O, LAST, B, WR, WC, ST, KG, PKC, QKC, SYM><<<(unsigned)grid, WR * WC * 64 * KG, 0, st>>>(g);
+        constexpr int threads = WR * WC * 64 * KG;
+        if (grid * threads >= 1L << 32) rc = GPX_ERR_UNSUPPORTED;
+        else if (!dry) ortho_mm_kernel<F, O, LAST, B, WR, WC, ST, KG, PKC, QKC, SYM><<<(unsigned)grid, threads, 0, st>>>(g);
     };
     if constexpr (!__is_same(F, double)) {
         const TileChoice c = choose_tile(SYM, g.I, g.J, g.K, batch);
@@ -522,7 +521,7 @@ template <class F, class O, bool LAST, bool PKC, bool QKC, bool SYM> int launch(
         else GO(32, 2, 2, 4, 1);
     }
 #undef GO
-    HIP_TRY(hipGetLastError());
+    if (!dry) HIP_TRY(hipGetLastError());
     return rc;
 }
 
@@ -1066,11 +1065,35 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
     double* part = reinterpret_cast<double*>(work + o.part);
     const long runs = norm_runs<F>(rows, cols);
     const int parts = norm_parts<F>(rows, cols);
+    char* x[2] = {work + o.x[0], work + o.x[1]};
+    char *a = work + o.a, *b = work + o.b;
+    float *da = reinterpret_cast<float*>(work + o.diag[0]), *db = reinterpret_cast<float*>(work + o.diag[1]);
+    const bool tall = rows > cols;
+    const int s = std::min(rows, cols), l = std::max(rows, cols);
+    auto step = [&](int k, bool dry) -> int {
+        char *from = x[k & 1], *to = x[~k & 1];
+        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, s, s, l, batch, f.gram[k], 0.0, nullptr, da};
+        int rc = tall ? launch<F, F, false, false, false, true>(st, gram, batch, dry) : launch<F, F, false, true, true, true>(st, gram, batch, dry);
+        if (rc) return rc;
+        const OrthoArgs poly = {a, a, a, b, o.lda, o.lda, o.lda, o.lda, o.sa, o.sa, o.sa, o.sa, s, s, s, batch,
+                                f.square[k], f.linear[k], da, db};
+        if ((rc = launch<F, F, false, true, true, true>(st, poly, batch, dry))) return rc;
+        const bool last = k + 1 == steps;
+        const long ldd = last ? ldo * (long)sizeof(T) : o.ldx, sd = last ? stride_o * (long)sizeof(T) : o.sx;
+        char* d = last ? reinterpret_cast<char*>(O) : to;
+        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k], db, nullptr}
+                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k], db, nullptr};
+        if (tall) rc = last ? launch<F, T, true, true, true, false>(st, apply, batch, dry) : launch<F, F, false, true, true, false>(st, apply, batch, dry);
+        else rc = last ? launch<F, T, true, true, false, false>(st, apply, batch, dry) : launch<F, F, false, true, false, false>(st, apply, batch, dry);
+        return rc;
+    };
+    const ChunkPlan plan = __is_same(F, double) ? ChunkPlan{} : chunk_plan(batch, rows, cols);
+    if (steps > 0 && !plan.chunks)
+        if (const int rc = step(0, true)) return rc;
     ortho_norm_kernel<T><<<dim3(parts, batch), 256, 0, st>>>(G, ldg, stride_g, rows, cols, part);
     HIP_TRY(hipGetLastError());
     const dim3 grid((unsigned)std::min<long>((runs + 255) / 256, 2048), (unsigned)batch);
     if constexpr (!__is_same(F, double)) {
-        const ChunkPlan plan = chunk_plan(batch, rows, cols);
         if (steps > 0 && plan.chunks) {
             char* images = work + o.x[0];
             mm::v4f* sums[2] = {reinterpret_cast<mm::v4f*>(images + plan.images), reinterpret_cast<mm::v4f*>(images + plan.images + plan.sums)};
@@ -1106,30 +1129,10 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
         HIP_TRY(hipGetLastError());
         return GPX_OK;
     }
-    char* x[2] = {work + o.x[0], work + o.x[1]};
-    char *a = work + o.a, *b = work + o.b;
-    float *da = reinterpret_cast<float*>(work + o.diag[0]), *db = reinterpret_cast<float*>(work + o.diag[1]);
     ortho_scale_kernel<T, F><<<grid, 256, 0, st>>>(G, ldg, stride_g, rows, cols, padded<F>(cols), part, parts, eps, f.start, x[0], o.ldx, o.sx);
     HIP_TRY(hipGetLastError());
-    const bool tall = rows > cols;
-    const int s = std::min(rows, cols), l = std::max(rows, cols);
-    for (int k = 0; k < steps; ++k) {
-        char *from = x[k & 1], *to = x[~k & 1];
-        const OrthoArgs gram = {from, from, from, a, o.ldx, o.ldx, 0, o.lda, o.sx, o.sx, 0, o.sa, s, s, l, batch, f.gram[k], 0.0, nullptr, da};
-        int rc = tall ? launch<F, F, false, false, false, true>(st, gram, batch) : launch<F, F, false, true, true, true>(st, gram, batch);
-        if (rc) return rc;
-        const OrthoArgs poly = {a, a, a, b, o.lda, o.lda, o.lda, o.lda, o.sa, o.sa, o.sa, o.sa, s, s, s, batch,
-                                f.square[k], f.linear[k], da, db};
-        if ((rc = launch<F, F, false, true, true, true>(st, poly, batch))) return rc;
-        const bool last = k + 1 == steps;
-        const long ldd = last ? ldo * (long)sizeof(T) : o.ldx, sd = last ? stride_o * (long)sizeof(T) : o.sx;
-        char* d = last ? reinterpret_cast<char*>(O) : to;
-        const OrthoArgs apply = tall ? OrthoArgs{from, b, from, d, o.ldx, o.lda, o.ldx, ldd, o.sx, o.sa, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k], db, nullptr}
-                                     : OrthoArgs{b, from, from, d, o.lda, o.ldx, o.ldx, ldd, o.sa, o.sx, o.sx, sd, rows, cols, s, batch, f.apply[k], f.keep[k], db, nullptr};
-        if (tall) rc = last ? launch<F, T, true, true, true, false>(st, apply, batch) : launch<F, F, false, true, true, false>(st, apply, batch);
-        else rc = last ? launch<F, T, true, true, false, false>(st, apply, batch) : launch<F, F, false, true, false, false>(st, apply, batch);
-        if (rc) return rc;
-    }
+    for (int k = 0; k < steps; ++k)
+        if (const int rc = step(k, false)) return rc;
     return GPX_OK;
 }
 

@@ -80,8 +80,8 @@ int gpx_dgemm_splitk_noalloc(int a_kc, int b_kc, int64_t M, int64_t N, int64_t K
  * strides up to 2^48 elements.  A result overlaps no operand, and the workspace neither (but see gpx_orthogonalize); an overlap that
  * the addresses, sizes and equal strides show is refused.
  * Products of F64 are summed in 64 bits, all others in 32; results are rounded once to the type they are stored in.
- * No result depends on the order in which workgroups run.  Status 1 (GPX_ERR_ARG): an argument is refused, nothing was
- * launched. */
+ * No result depends on the order in which workgroups run.  Status 1 (GPX_ERR_ARG): an argument is refused; 4
+ * (GPX_ERR_UNSUPPORTED): more tiles than one launch takes (2^32 work-items); nothing was launched. */
 enum { GPX_F64 = 0, GPX_F32 = 1, GPX_BF16 = 2, GPX_F16 = 3 };
 
 /* Rows t (points, K contiguous elements at X + t*ldx) with offsets[g] <= t < offsets[g+1] belong to group g:

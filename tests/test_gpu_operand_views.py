@@ -46,3 +46,17 @@ def test_overlaps_are_refused():
                 lambda: lib.orthogonalize(stack[:1].expand(3, 8, 8), stack)):
         with pytest.raises(lib.GpxError):
             bad()
+
+
+def test_many_groups_of_one_row_and_many_columns():
+    """1024 groups of a row and 2^20 columns: in tiles of 32 x 64 these would be more than a launch takes."""
+    lib = _lib()
+    rows, n, k = 1024, 1 << 20, 16
+    x, w = data(1, torch.bfloat16, rows, k), data(2, torch.bfloat16, 1, n, k)
+    off = torch.arange(rows + 1, device="cuda")
+    y = lib.grouped_gemm(x, w.expand(rows, n, k), off, torch.empty(rows, n, dtype=torch.bfloat16, device="cuda"))
+    for at in range(0, n, n // 8):   # sums of 16 products in 32 bits, and the rounding of the result
+        cols = slice(at, at + n // 8)
+        wt = w[0, cols].double().T.contiguous()
+        want, size = x.double() @ wt, x.double().abs() @ wt.abs()
+        assert bool(((y[:, cols].double() - want).abs() <= (k + 3) * 2.0 ** -23 * size + 2.0 ** -8 * want.abs()).all())
