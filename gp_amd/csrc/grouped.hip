@@ -88,7 +88,7 @@ __device__ RowTile find_tile(const int64_t* offsets, int groups, long T, int nt,
     const GroupScan first(offsets, groups, T, 0, UNIT);
     long total = __shfl(first.sum, 63, 64);
     for (int g0 = 64; g0 < groups; g0 += 64) total += __shfl(GroupScan(offsets, groups, T, g0, UNIT).sum, 63, 64);
-    long all = total * nt, start, last;
+    long all = total * nt, start = 0, last;
     const unsigned xcd = blockIdx.x & 7;
     if (slots) {
         const int left = (int)(all % slots);

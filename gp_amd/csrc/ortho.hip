@@ -793,7 +793,6 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
             for (int x = 0; x < TURNS; ++x) {
                 if (wave + kSmallWaves * x >= TILES) break;
                 SmallAcc c;
-#pragma unroll 4
                 for (int k = 0; k < kx; ++k)
                     c.add(small_frag_kc(X, ldx, tj[x], k, 0, lane), small_frag_kc(X, ldx, tj[x], k, 1, lane), small_frag_kc(X, ldx, ti[x], k, 0, lane),
                           small_frag_kc(X, ldx, ti[x], k, 1, lane));
