@@ -869,7 +869,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void ortho_small_kernel(const T* 
 // Every workgroup keeps LC columns of X, and the launch of a step does, for them: A from the sums of all chunks (in one order),
 // the square factor (again in every workgroup: short products), X <- a X + (b A + c A A) X, and the chunk's part of the next X X^T.
 // Launches and their short dependent products bound it: 3 a step on the general path.  f32: 50 x 1203 (8, three steps) 70 -> 38 us,
-// 128 x 4096 237 -> 126, 16 x 2000 117 -> 34, 128 x 168 95 -> 75; bf16 keeps 22 bits here: 100 x 4000 156 -> 124, 24 of 120 x 1280 135 -> 139.
+// 128 x 4096 237 -> 126, 16 x 2000 117 -> 34, 128 x 168 95 -> 75.
 struct OrthoChunkArgs {
     long ldg, stride_g, ldo, stride_o;   // elements
     int rows, cols, chunks, parts;

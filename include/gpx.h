@@ -72,15 +72,16 @@ int gpx_dgemm_splitk_noalloc(int a_kc, int b_kc, int64_t M, int64_t N, int64_t K
                              int flags, void* hip_stream);
 
 /* ---- products grouped by expert, and the orthogonalised update (no reference counterpart) -----------
- * Local experts (groups of training rows, each with a feature map z = W_g x of its own): all their products in one call,
- * the gradients of both operands, and the Newton-Schulz update of a batch of weight matrices.  All buffers are DEVICE
+ * For callers that train maps z = W_g x of groups of rows: all their products in one call, the gradients of both operands,
+ * and the Newton-Schulz update of a batch of weight matrices.  All buffers are DEVICE
  * memory of hip_stream's device (NULL: the legacy stream of the current device); every call is asynchronous, allocates
  * nothing, waits for nothing and may be captured into a HIP graph; the caller's current device is restored.  Element
  * types: dtype below; pointers are aligned to their element, rows of any length are taken, leading dimensions up to 2^32 and
  * strides up to 2^48 elements.  A result overlaps no operand, and the workspace neither (but see gpx_orthogonalize); an overlap that
  * the addresses, sizes and equal strides show is refused.
  * Products of F64 are summed in 64 bits, all others in 32; results are rounded once to the type they are stored in.
- * No result depends on the order in which workgroups run.  Status 1 (GPX_ERR_ARG): an argument is refused; 4
+ * No result depends on the order in which workgroups run; the order of a sum depends on types and sizes, those of a batch
+ * among them.  Status 1 (GPX_ERR_ARG): an argument is refused; 4
  * (GPX_ERR_UNSUPPORTED): more tiles than one launch takes (2^32 work-items); nothing was launched. */
 enum { GPX_F64 = 0, GPX_F32 = 1, GPX_BF16 = 2, GPX_F16 = 3 };
 
