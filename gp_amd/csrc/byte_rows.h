@@ -8,7 +8,11 @@ struct ByteRows {
     const void* base;
     int64_t mats, stride, rows, ld, width;
 };
-// Whether two of them are seen to share bytes.  Columns beside one another of one larger matrix do not, nor do row blocks beside one
+// Whether they reach less than 2^60 bytes from `base` on, so that no address of theirs wraps.
+static inline bool gpx_reaches(const ByteRows& m) {
+    return m.mats <= 0 || m.rows <= 0 || (m.mats - 1.0) * m.stride + (m.rows - 1.0) * m.ld + m.width < 0x1p60;
+}
+// Whether two of them, which do, are seen to share bytes.  Columns beside one another of one larger matrix do not, nor do row blocks beside one
 // another of every matrix of a stack; where two leading dimensions or strides differ, only the
 // first rows and ranges without gaps are judged.
 static inline bool gpx_share_bytes(ByteRows a, ByteRows b) {

@@ -616,7 +616,7 @@ template <class T, class O> int grouped_dw_typed(hipStream_t st, const GroupedDw
 
 constexpr long kMaxExtent = (1L << 31) - 1024;   // row, column and k numbers within one product are 32-bit
 constexpr int kMaxGroups = 65535;
-constexpr int64_t kMaxLd = 1L << 32, kMaxStride = 1L << 48;   // elements: no product of sizes below passes 63 bits
+constexpr int64_t kMaxLd = 1L << 32, kMaxStride = 1L << 48;   // elements: in bytes they pass no 63 bits
 
 int elem_bytes(int dtype) { return dtype == GPX_F64 ? 8 : dtype == GPX_F32 ? 4 : dtype == GPX_BF16 || dtype == GPX_F16 ? 2 : 0; }
 bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes != 0; }
@@ -631,13 +631,13 @@ extern "C" int gpx_grouped_gemm(int dtype, int w_kc, int64_t groups, int64_t T, 
     if (T > kMaxExtent || N > kMaxExtent || K > kMaxExtent) return GPX_ERR_ARG;
     if (ldx < K || ldw < (w_kc ? K : N) || ldy < N || stride_w < 0) return GPX_ERR_ARG;
     if (ldx > kMaxLd || ldw > kMaxLd || ldy > kMaxLd || stride_w > kMaxStride) return GPX_ERR_ARG;
+    const ByteRows x = {X, 1, 0, T, ldx * e, K * e}, y = {Y, 1, 0, T, ldy * e, N * e};
+    const ByteRows w = {W, groups, stride_w * e, w_kc ? N : K, ldw * e, (w_kc ? K : N) * e}, table = {offsets, 1, 0, 1, 0, 8 * (groups + 1)};
+    if (!gpx_reaches(x) || !gpx_reaches(y) || !gpx_reaches(w)) return GPX_ERR_ARG;
     if (groups == 0 || T == 0 || N == 0) return GPX_OK;   // no row of Y belongs to a group
     if (!Y || !offsets || (K > 0 && (!X || !W))) return GPX_ERR_ARG;
     if (misaligned(X, e) || misaligned(W, e) || misaligned(Y, e) || misaligned(offsets, 8)) return GPX_ERR_ARG;
-    const ByteRows y = {Y, 1, 0, T, ldy * e, N * e};
-    if (gpx_share_bytes(y, {X, 1, 0, T, ldx * e, K * e}) || gpx_share_bytes(y, {offsets, 1, 0, 1, 0, 8 * (groups + 1)}) ||
-        gpx_share_bytes(y, {W, groups, stride_w * e, w_kc ? N : K, ldw * e, (w_kc ? K : N) * e}))
-        return GPX_ERR_ARG;
+    if (gpx_share_bytes(y, x) || gpx_share_bytes(y, w) || gpx_share_bytes(y, table)) return GPX_ERR_ARG;
     StreamDevice dev(static_cast<hipStream_t>(hip_stream));
     if (dev.status) return dev.status;
     GroupedArgs g = {static_cast<const char*>(X), static_cast<const char*>(W), static_cast<char*>(Y), offsets, ldx * e, ldw * e,
@@ -660,14 +660,16 @@ extern "C" int gpx_grouped_gemm_dw(int dtype, int c_dtype, int64_t groups, int64
         return GPX_ERR_ARG;
     if (ldx < M || ldz < N || ldc < M || stride_c < 0 || work_bytes < 0) return GPX_ERR_ARG;
     if (ldx > kMaxLd || ldz > kMaxLd || ldc > kMaxLd || stride_c > kMaxStride) return GPX_ERR_ARG;
+    const ByteRows x = {X, 1, 0, T, ldx * e, M * e}, z = {Z, 1, 0, T, ldz * e, N * e}, c = {C, groups, stride_c * ec, N, ldc * ec, M * ec};
+    const ByteRows table = {offsets, 1, 0, 1, 0, 8 * (groups + 1)};
+    if (!gpx_reaches(x) || !gpx_reaches(z) || !gpx_reaches(c)) return GPX_ERR_ARG;
     if (groups == 0 || M == 0 || N == 0) return GPX_OK;
     if (groups > 1 && stride_c < (N - 1) * ldc + M) return GPX_ERR_ARG;   // results of two groups would overlap
     if (!C || !offsets || (T > 0 && (!X || !Z))) return GPX_ERR_ARG;
     if (misaligned(X, e) || misaligned(Z, e) || misaligned(C, ec) || misaligned(offsets, 8)) return GPX_ERR_ARG;
     const DwPlan plan = dw_plan(e, ec, groups, T, M, N);
     if (plan.part_rows && (!work || misaligned(work, 16) || work_bytes < dw_work_bytes(plan, e, M, N))) return GPX_ERR_ARG;
-    const ByteRows c = {C, groups, stride_c * ec, N, ldc * ec, M * ec}, table = {offsets, 1, 0, 1, 0, 8 * (groups + 1)};
-    const ByteRows x = {X, 1, 0, T, ldx * e, M * e}, z = {Z, 1, 0, T, ldz * e, N * e}, w = {work, 1, 0, 1, 0, dw_work_bytes(plan, e, M, N)};
+    const ByteRows w = {work, 1, 0, 1, 0, dw_work_bytes(plan, e, M, N)};
     if (gpx_share_bytes(c, x) || gpx_share_bytes(c, z) || gpx_share_bytes(c, table) || gpx_share_bytes(w, x) || gpx_share_bytes(w, z) ||
         gpx_share_bytes(w, c) || gpx_share_bytes(w, table))
         return GPX_ERR_ARG;

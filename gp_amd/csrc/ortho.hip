@@ -1137,7 +1137,7 @@ int ortho_typed(hipStream_t st, int batch, int rows, int cols, const T* G, long 
 
 constexpr int kMaxSteps = 64;
 constexpr long kMaxSide = 1L << 20;
-constexpr int64_t kMaxLd = 1L << 32, kMaxStride = 1L << 48;   // elements: no product of sizes below passes 63 bits
+constexpr int64_t kMaxLd = 1L << 32, kMaxStride = 1L << 48;   // elements: in bytes they pass no 63 bits
 constexpr double kLeastEps = 1e-300;                          // 2^15 / eps stays finite: a zero matrix gives zeros
 const double kQuintic[3] = {3.4445, -4.7750, 2.0315};
 
@@ -1164,16 +1164,18 @@ extern "C" int gpx_orthogonalize(int dtype, int64_t batch, int64_t M, int64_t N,
     if (!sizes_ok(dtype, batch, M, N) || steps < 0 || steps > kMaxSteps || !(eps >= kLeastEps) || !std::isfinite(eps)) return GPX_ERR_ARG;
     if (ldg < M || ldo < M || stride_g < 0 || stride_o < 0) return GPX_ERR_ARG;
     if (ldg > kMaxLd || ldo > kMaxLd || stride_g > kMaxStride || stride_o > kMaxStride) return GPX_ERR_ARG;
+    const uintptr_t e = dtype == GPX_F64 ? 8 : dtype == GPX_F32 ? 4 : 2;
+    const int64_t el = (int64_t)e;
+    const ByteRows in = {G, batch, stride_g * el, N, ldg * el, M * el}, out = {O, batch, stride_o * el, N, ldo * el, M * el};
+    if (!gpx_reaches(in) || !gpx_reaches(out)) return GPX_ERR_ARG;
     if (batch == 0 || M == 0 || N == 0) return GPX_OK;
     if (switched_off(dtype, M, N)) return GPX_ERR_ARG;
     if (batch > 1 && stride_o < (N - 1) * ldo + M) return GPX_ERR_ARG;   // results of two matrices would overlap
     if (!G || !O || !work) return GPX_ERR_ARG;
-    const uintptr_t e = dtype == GPX_F64 ? 8 : dtype == GPX_F32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(G) % e || reinterpret_cast<uintptr_t>(O) % e || reinterpret_cast<uintptr_t>(work) % 16) return GPX_ERR_ARG;
     const int64_t need = ortho_work(dtype, batch, (int)N, (int)M);
     if (work_bytes < need) return GPX_ERR_ARG;
-    const int64_t el = (int64_t)e;
-    const ByteRows in = {G, batch, stride_g * el, N, ldg * el, M * el}, out = {O, batch, stride_o * el, N, ldo * el, M * el}, room = {work, 1, 0, 1, 0, need};
+    const ByteRows room = {work, 1, 0, 1, 0, need};
     const bool in_place = G == O && (N == 1 || ldg == ldo) && (batch == 1 || stride_g == stride_o);
     if ((!in_place && gpx_share_bytes(in, out)) || gpx_share_bytes(room, in) || gpx_share_bytes(room, out)) return GPX_ERR_ARG;
     double table[3 * kMaxSteps];

@@ -77,7 +77,7 @@ int gpx_dgemm_splitk_noalloc(int a_kc, int b_kc, int64_t M, int64_t N, int64_t K
  * memory of hip_stream's device (NULL: the legacy stream of the current device); every call is asynchronous, allocates
  * nothing, waits for nothing and may be captured into a HIP graph; the caller's current device is restored.  Element
  * types: dtype below; pointers are aligned to their element, rows of any length are taken, leading dimensions up to 2^32 and
- * strides up to 2^48 elements.  A result overlaps no operand, and the workspace neither (but see gpx_orthogonalize); an overlap that
+ * strides up to 2^48 elements, an operand less than 2^60 bytes in all.  A result overlaps no operand, and the workspace neither (but see gpx_orthogonalize); an overlap that
  * the addresses, sizes and equal strides show is refused.
  * Products of F64 are summed in 64 bits, all others in 32; results are rounded once to the type they are stored in.
  * No result depends on the order in which workgroups run; the order of a sum depends on types and sizes, those of a batch
